@@ -449,6 +449,41 @@ int ftk_debug_lost_wait(int give_up, long long* out, void* stream);
 // 0 sends bfloat16 grouped expert products to the CUDA-core kernels; default 1 (tcgen05).
 int ftk_set_moe_tensor_cores(int enabled);
 int ftk_set_moe_pairs(int enabled);
+// Attention of single tokens where requests share keys (shared_attention.cu, which says what items, members, requests and joins hold).
+typedef struct {
+  const void* q;               // [n_rows, n_q_heads, head_dim]
+  const void* k;               // [num_pages, n_kv_heads, page_size, head_dim]
+  const void* v;
+  void* out;                   // as q; rows that no request names stay as they are
+  const int32_t* block_table;  // [bt_rows, bt_stride]
+  const int32_t* items;        // [n_items, 8]
+  const int32_t* members;
+  const int32_t* requests;     // [n_requests, 8]
+  const int32_t* joins;
+  float* part_o;               // [n_slots, n_q_heads, head_dim]
+  float* part_ml;              // [n_slots, n_q_heads, 2]
+  const float* sink_heads;     // [n_q_heads] or null
+  int dtype, bt_stride, bt_rows, n_items, n_members, n_requests, n_joins, n_slots, n_rows, n_q_heads, n_kv_heads, head_dim, page_size, num_pages;
+  int tile_rows;               // query rows of a piece of shared keys at most: 16, or 256 (tcgen05)
+  int cluster;                 // CTAs that share a request's own keys: 1, 2, 4 or 8
+  float scale;
+  int has_sink;
+  float sink;
+} FtkShared;
+int ftk_shared_attention(const FtkShared* a, void* stream);
+// Copies inside the cache (cache_copy.cu): tensors [entries, blocks, parts, rows, row_bytes], contiguous (a slab: KV heads and tokens of a page; a state:
+// 1 and 1); pairs [n_pairs, pair_ints] int32 on the device: from, to and (pair_ints 3) how many of every part's rows.  No block
+// may be written by one pair and read or written by another; pairs with a block outside the tensor are left out.
+typedef struct {
+  void* base;
+  int entries, blocks, parts, rows, row_bytes;
+} FtkCopyTensor;
+int ftk_copy_blocks(const FtkCopyTensor* tensors, int n_tensors, const int32_t* pairs, int pair_ints, int n_pairs, void* stream);
+// Draws with temperature, top-k, top-p and min-p, several from a row where rows [n_draws] says so (null: draw i from row i), and the drawn tokens' log-probabilities
+// (logprobs may be null).  draws.cu states the rule.
+int ftk_sample_draws(const float* logits, long long row_stride, int n_rows, int vocab, const int32_t* rows, int n_draws,
+                     const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p, const float* u,
+                     int32_t* out, float* logprobs, void* stream);
 int ftk_sample(const float* logits, int n_rows, int vocab, const float* temperature,
                const int32_t* top_k, const float* top_p, const float* u, int32_t* out, void* stream);
 

@@ -1,0 +1,168 @@
+"""Host-side work list of attention over shared keys (``ops.shared_attention``).
+
+Requests that continue one prompt, or that begin with the same system prompt, share the pages of it.  A *span* says so: its
+members read the same pages for the positions ``[start, end)``.  The keys of a span are worked on once, with the query rows of all
+its members together: the members are put into tiles of as many query rows as the kernel takes, and the tiles are cut along the keys
+until they keep every SM busy.  What a request reads outside of spans is its own, and the kernel that joins a request's partial
+results takes it.  Spans may nest (a system prompt under several users' prompts, each under several answers).
+
+Nothing here depends on the requests' lengths but the ``requests`` array and the number of CTAs that share a request's own keys
+(``cluster``, which goes by the longest own part rounded up to a power of two): a decode step replayed from a CUDA graph keeps
+its sizes while the requests grow.  The reference reads shared pages once per request
+(python/freetoken/kernel/triton/attention.py:147-352).
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Dict, List, Optional, Sequence, Tuple
+
+import numpy as np
+import torch
+
+from ..errors import KernelError
+
+ITEM_INTS = 8     # first member, members, block-table row, first key, one past the last key, first slot, 0, 0
+REQUEST_INTS = 8  # query row, block-table row, first own key, one past the last, first join, joins, 0, 0
+ROWS_TILE = 16    # query rows of a piece on the kernels for few rows
+MOST_CLUSTER = 8
+
+Span = Tuple[Sequence[int], int, int]  # members (indices of requests), first position, one past the last
+
+
+@dataclass
+class SharedPlan:
+    """int32 arrays of one step's shared and own keys, and what the launch needs beside them."""
+
+    items: np.ndarray     # [n, 8]
+    members: np.ndarray   # query rows
+    requests: np.ndarray  # [n, 8]
+    joins: np.ndarray     # slots of every request's partial results, in the order of its keys
+    n_slots: int
+    tile_rows: int
+    cluster: int
+    n_rows: int           # rows of q that the plan reads, from the first on
+    n_heads: int
+    n_kv_heads: int
+    head_dim: int
+
+    def key(self) -> Tuple[int, ...]:
+        """What a recorded step's launches depend on."""
+        return (self.items.shape[0], self.members.shape[0], self.requests.shape[0], self.joins.shape[0], self.n_slots, self.tile_rows, self.cluster)
+
+    def sections(self) -> List[Tuple[str, np.ndarray]]:
+        return [("items", self.items), ("members", self.members), ("requests", self.requests), ("joins", self.joins)]
+
+    def bind(self, tensors: Dict[str, torch.Tensor], part_o: Optional[torch.Tensor], part_ml: Optional[torch.Tensor]) -> "SharedDevicePlan":
+        return SharedDevicePlan(tensors["items"], tensors["members"], tensors["requests"], tensors["joins"], part_o, part_ml, self)
+
+    def to(self, device) -> "SharedDevicePlan":
+        """On the device, with scratch of its own: for callers without an engine's buffers.  Two calls that may run at once
+        need a plan each."""
+        tensors = {name: torch.from_numpy(arr).to(device) for name, arr in self.sections()}
+        part_o = part_ml = None
+        if self.n_slots:
+            part_o = torch.empty((self.n_slots, self.n_heads, self.head_dim), dtype=torch.float32, device=device)
+            part_ml = torch.empty((self.n_slots, self.n_heads, 2), dtype=torch.float32, device=device)
+        return self.bind(tensors, part_o, part_ml)
+
+
+@dataclass
+class SharedDevicePlan:
+    items: torch.Tensor
+    members: torch.Tensor
+    requests: torch.Tensor
+    joins: torch.Tensor
+    part_o: Optional[torch.Tensor]   # [slots, heads, head_dim] float32
+    part_ml: Optional[torch.Tensor]  # [slots, heads, 2] float32
+    host: SharedPlan
+
+
+def tile_members(n: int, most: int) -> List[Tuple[int, int]]:
+    """``n`` members in as few tiles of at most ``most`` as there are, of about the same size: (first, members) each."""
+    tiles = -(-n // most)
+    edges = [n * i // tiles for i in range(tiles + 1)]
+    return [(a, b - a) for a, b in zip(edges, edges[1:])]
+
+
+def own_cluster(longest: int, blocks: int, tile: int, sm_count: int) -> int:
+    """CTAs that share one request's own keys: as many as fill the GPU twice, none with less than a tile of keys."""
+    cluster = 1
+    while cluster < MOST_CLUSTER and blocks * cluster < 2 * sm_count and longest > cluster * tile:
+        cluster *= 2
+    return cluster
+
+
+def build_shared_plan(kv_lens: Sequence[int], spans: Sequence[Span], n_heads: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype,
+                      page_size: int, table_rows: Optional[Sequence[int]] = None, sm_count: int = 148) -> SharedPlan:
+    """The work list of one step: request ``i`` has query row ``i``, ``kv_lens[i]`` keys (its own token's among them) and row
+    ``table_rows[i]`` (``i``) of the block table.
+
+    ``spans``: (members, start, end) of keys that the members share: the block-table rows of all of them must name the same pages
+    for these positions (the first member's row is read).  ``end`` may lie inside a page.  The spans of one request must not
+    overlap and leave no positions out in front of them; a span of a single member is that request's own."""
+    n = len(kv_lens)
+    if n_heads < 1 or n_kv_heads < 1 or n_heads % n_kv_heads:
+        raise KernelError(f"shared_attention: {n_heads} query heads on {n_kv_heads} KV heads")
+    rows = list(range(n)) if table_rows is None else [int(r) for r in table_rows]
+    if len(rows) != n:
+        raise KernelError("shared_attention: one block-table row per request")
+    if any(x < 0 for x in kv_lens):
+        raise KernelError("shared_attention: a negative length")
+    group = n_heads // n_kv_heads
+    tile_rows = ROWS_TILE
+    most = max(1, tile_rows // min(group, tile_rows))
+    chunks = -(-group // ROWS_TILE)
+    unit = 64 if dtype == torch.bfloat16 else 32  # keys a kernel works on at a time
+
+    taken: List[List[Tuple[int, int]]] = [[] for _ in range(n)]
+    tiles: List[Tuple[List[int], int, int]] = []
+    for members, start, end in spans:
+        members = [int(m) for m in members]
+        start, end = int(start), int(end)
+        if len(set(members)) != len(members) or any(not 0 <= m < n for m in members):
+            raise KernelError("shared_attention: a span's members are different requests of the step")
+        if start < 0 or any(end > kv_lens[m] for m in members):
+            raise KernelError(f"shared_attention: the span [{start}, {end}) does not lie within its members' keys")
+        if end <= start or len(members) < 2:
+            continue
+        for m in members:
+            if any(a < end and start < b for a, b in taken[m]):
+                raise KernelError(f"shared_attention: request {m} is in two spans that overlap")
+            taken[m].append((start, end))
+        for a, k in tile_members(len(members), most):
+            tiles.append((members[a:a + k], start, end))
+
+    # pieces of about as many units for every CTA that fits
+    heads = n_kv_heads * chunks
+    units = [-(-(end - start) // unit) for _, start, end in tiles]
+    length = max(4, -(-sum(units) * heads // (4 * sm_count)))
+    items, member_rows, slots = [], [], [[] for _ in range(n)]
+    n_slots = 0
+    for (members, start, end), u in zip(tiles, units):
+        first = len(member_rows)
+        member_rows += members
+        for a, k in tile_members(u, length):
+            items.append((first, len(members), rows[members[0]], start + a * unit, min(end, start + (a + k) * unit), n_slots, 0, 0))
+            for i, m in enumerate(members):
+                slots[m].append((start + a * unit, n_slots + i))
+            n_slots += len(members)
+    items.sort(key=lambda it: it[3] - it[4])  # the longest first
+
+    # what is a request's own: one range behind its spans
+    requests, joins, longest = [], [], 1
+    for i in range(n):
+        begin = 0
+        for a, b in sorted(taken[i]):
+            if a != begin:
+                raise KernelError(f"shared_attention: the spans of request {i} leave out positions {begin} to {a}")
+            begin = b
+        own = [s for _, s in sorted(slots[i])]
+        requests.append((i, rows[i], begin, int(kv_lens[i]), len(joins), len(own), 0, 0))
+        joins += own
+        longest = max(longest, int(kv_lens[i]) - begin)
+    blocks = max(1, n * heads)
+    cluster = own_cluster(1 << (longest - 1).bit_length(), blocks, unit, sm_count)
+    as_int = lambda x, w: np.asarray(x, dtype=np.int32).reshape(-1, w) if w else np.asarray(x, dtype=np.int32)  # noqa: E731
+    return SharedPlan(as_int(items, ITEM_INTS), as_int(member_rows, 0), as_int(requests, REQUEST_INTS), as_int(joins, 0), n_slots,
+                      tile_rows, cluster, n, n_heads, n_kv_heads, head_dim)

@@ -20,6 +20,9 @@ moe_gemm2              fused_moe.py:156-302 (route weight on the accumulator, :2
 moe_combine            fused_moe.py:111-153
 act_and_mul            activation.py:67-112
 sample                 python/freetoken/engine/sample.py:24-80, python/freetoken/kernel/triton/sampling.py
+copy_pages, copy_slots no counterpart: cache pages and state slots of requests that begin as copies of others
+shared_attention       no counterpart: decode attention where requests share keys
+sample_draws           no counterpart: several draws from a row, min-p, log-probabilities
 moe_route              router product + router_topk + moe_permute in one launch (short steps)
 add_rmsnorm_routes     moe_combine + add_rmsnorm in one pass
 linear                 python/freetoken/layers/linear.py:66-70 (the library product)
@@ -85,6 +88,17 @@ class _StreamNorm(ctypes.Structure):
 class _AttnExtras(ctypes.Structure):
     _fields_ = [("dist_bias", _vp), ("dist_len", _i), ("kv_split", _i), ("has_sink", _i), ("sink_logit", _f),
                 ("sink_heads", _vp), ("softcap", _f), ("keep_first", _i), ("ahead", _vp), ("ahead_bytes", ctypes.c_longlong)]
+
+
+class _Shared(ctypes.Structure):
+    _fields_ = [(n, _vp) for n in ("q", "k", "v", "out", "block_table", "items", "members", "requests", "joins", "part_o", "part_ml",
+                                   "sink_heads")] + [(n, _i) for n in (
+        "dtype", "bt_stride", "bt_rows", "n_items", "n_members", "n_requests", "n_joins", "n_slots", "n_rows", "n_q_heads", "n_kv_heads",
+        "head_dim", "page_size", "num_pages", "tile_rows", "cluster")] + [("scale", _f), ("has_sink", _i), ("sink", _f)]
+
+
+class _CopyTensor(ctypes.Structure):
+    _fields_ = [("base", _vp), ("entries", _i), ("blocks", _i), ("parts", _i), ("rows", _i), ("row_bytes", _i)]
 
 
 class _StreamStep(ctypes.Structure):
@@ -160,6 +174,9 @@ _SIGNATURES = {
     "ftk_diff_heads": [_vp, _i, _i, _vp, _f, _f, _vp, _i, _i, _i, _vp],
     "ftk_act_and_mul": [_vp, _i, _i, _i, _i, _f, _f, _vp, _vp],
     "ftk_sample": [_vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp],
+    "ftk_shared_attention": [ctypes.POINTER(_Shared), _vp],
+    "ftk_copy_blocks": [ctypes.POINTER(_CopyTensor), _i, _vp, _i, _i, _vp],
+    "ftk_sample_draws": [_vp, ctypes.c_longlong, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
     "ftk_cast": [_vp, _i, _vp, _i, ctypes.c_longlong, _vp],
     "ftk_table_update": [_vp, ctypes.c_longlong, _vp, _i, _vp],
     "ftk_copy_tokens": [_vp, _i, _vp, _vp, _i, _i, _i, _vp],
@@ -418,6 +435,56 @@ def cast(src: torch.Tensor, dst: torch.Tensor) -> None:
                            src.numel(), _stream()), "cast")
 
 
+# --------------------------------------------------------------------------- copies inside the cache
+def _here(t: torch.Tensor, what: str, dtype: Optional[torch.dtype] = None) -> int:
+    """:func:`_dev` of a tensor on the current device, where the kernel will run."""
+    ptr = _dev(t, what, dtype)
+    if t.device.index != torch.cuda.current_device():
+        raise KernelError(f"{what}: tensor is on '{t.device}', the current device is 'cuda:{torch.cuda.current_device()}'")
+    return ptr
+
+
+def _copy_blocks(what: str, tensors: Sequence[torch.Tensor], pairs: torch.Tensor, ints: int, shapes) -> None:
+    if pairs.dim() != 2 or pairs.shape[1] != ints or pairs.dtype != torch.int32:
+        raise KernelError(f"{what}: pairs must be int32 [n, {ints}], got {pairs.dtype} {tuple(pairs.shape)}")
+    if not tensors or not pairs.shape[0]:
+        return
+    arr = (_CopyTensor * len(tensors))()
+    for c, t, (parts, rows) in zip(arr, tensors, shapes):
+        c.base = _here(t, what)
+        c.entries, c.blocks, c.parts, c.rows = t.shape[0], t.shape[1], parts, rows
+        c.row_bytes = t.element_size() * (t.numel() // max(1, t.shape[0] * t.shape[1] * parts * rows))
+    _check(_lib().ftk_copy_blocks(arr, len(tensors), _here(pairs, "pairs", torch.int32), ints, pairs.shape[0], _stream()), what,
+           -(-len(tensors) // 16))
+
+
+def copy_pages(slabs: Sequence[torch.Tensor], pairs: torch.Tensor) -> None:
+    """``slab[e, to, h, :rows] = slab[e, from, h, :rows]`` for every ``(from, to, rows)`` of ``pairs``, every entry and head of every slab.
+
+    ``slabs``: any number of ``[entries, pages, heads, page_size, dim]`` tensors with the same pages (one launch for sixteen of them);
+    ``pairs`` int32 ``[n, 3]`` on the device.  ``rows`` from the page size on is the whole page; rows behind them stay as they are.  A
+    page may be the source of many pairs, but the target of one at most, and no target may be a source: copies are not in order.  A
+    pair that names a page outside the slab, has no rows, or names the same page twice does nothing."""
+    for t in slabs:
+        if t.dim() != 5 or t.shape[1] != slabs[0].shape[1] or t.shape[3] != slabs[0].shape[3]:
+            raise KernelError("copy_pages: slabs must be [entries, pages, heads, page_size, dim] with the same pages")
+        if not t.numel():
+            raise KernelError("copy_pages: an empty slab")
+    _copy_blocks("copy_pages", slabs, pairs, 3, [t.shape[2:4] for t in slabs])
+
+
+def copy_slots(tensors: Sequence[torch.Tensor], pairs: torch.Tensor) -> None:
+    """``tensor[e, to] = tensor[e, from]`` for every ``(from, to)`` of ``pairs`` (int32 ``[n, 2]``, on the device), every entry of every
+    tensor ``[entries, slots, ...]`` of the same slots: the states of requests that begin as copies of others.  The rules about
+    sources and targets are :func:`copy_pages`'."""
+    for t in tensors:
+        if t.dim() < 2 or t.shape[1] != tensors[0].shape[1]:
+            raise KernelError("copy_slots: tensors must be [entries, slots, ...] with the same slots")
+        if not t.numel():
+            raise KernelError("copy_slots: an empty tensor")
+    _copy_blocks("copy_slots", tensors, pairs, 2, [(1, 1)] * len(tensors))
+
+
 # --------------------------------------------------------------------------- attention
 def norm_rope_store(x: torch.Tensor, head_dim: int, rotary_dim: int, positions: torch.Tensor,
                     rope_table: Optional[torch.Tensor], eps: float, gemma: bool,
@@ -641,6 +708,51 @@ def paged_attention(q: torch.Tensor, k_slab: torch.Tensor, v_slab: torch.Tensor,
         _dev(part_o, "part_o", torch.float32), _dev(part_ml, "part_ml", torch.float32), n_slots,
         _dev(out, "out"), Hq, Hkv, D, P, pages, tile_rows, float(scale),
         int(window) if window else 0, _stream()), "paged_attention", 2 if n_slots else 1)
+
+
+def shared_attention(q: torch.Tensor, k_slab: torch.Tensor, v_slab: torch.Tensor, block_table: torch.Tensor, plan: Any,
+                     out: torch.Tensor, scale: float, sink: Any = None) -> None:
+    """Softmax attention of single tokens over paged keys and values, where several requests share keys: what they share is read
+    and multiplied once for all of them.
+
+    ``q, out [T, Hq, D]``; slabs ``[pages, Hkv, page_size, D]``; ``block_table [rows, width]`` page ids; ``plan`` from
+    :func:`freetoken_b200.engine.shared_plan.build_shared_plan`, on the device with its scratch.  Request ``i`` of the plan is row
+    ``i`` of ``q``; it reads all of its keys (its own token's lies among them).  Rows of ``out`` that are no request's stay as they are,
+    a request without keys gets zeros.  float32 and bfloat16, heads of 16 to 256 in steps of 16, any page size and group.  Results do
+    not depend on the order in which blocks run, but on the plan (the order of a request's sums is that of its pieces).
+
+    ``sink``: a logit, a float32 tensor ``[Hq]`` of one per query head, or None, as in :func:`paged_attention`.
+
+    The plan's scratch belongs to one launch at a time: calls that may run at once need plans of their own."""
+    host = plan.host
+    if q.dim() != 3 or k_slab.dim() != 4:
+        raise KernelError("shared_attention: q must be [T, Hq, D], slabs [pages, Hkv, page_size, D]")
+    T, Hq, D = q.shape
+    pages, Hkv, P, D2 = k_slab.shape
+    if D2 != D or v_slab.shape != k_slab.shape or (Hq, Hkv, D) != (host.n_heads, host.n_kv_heads, host.head_dim):
+        raise KernelError("shared_attention: q, slabs and plan do not agree")
+    if out.shape != q.shape or out.dtype != q.dtype or k_slab.dtype != q.dtype or v_slab.dtype != q.dtype:
+        raise KernelError("shared_attention: dtypes or out shape do not agree")
+    if block_table.dim() != 2 or T < host.n_rows:
+        raise KernelError(f"shared_attention: {T} query rows and a block table of {block_table.dim()} dimensions for a plan of {host.n_rows} requests")
+    if not host.n_rows:
+        return
+    n_slots = host.n_slots
+    if n_slots and (plan.part_o is None or plan.part_o.shape != (n_slots, Hq, D) or plan.part_ml is None or plan.part_ml.shape != (n_slots, Hq, 2)):
+        raise KernelError("shared_attention: the plan's scratch must be [slots, Hq, D] and [slots, Hq, 2]")
+    sink_heads = None
+    if isinstance(sink, torch.Tensor):
+        if sink.shape != (Hq,):
+            raise KernelError("shared_attention: a sink per head must be [Hq]")
+        sink_heads, sink = _here(sink, "sink", torch.float32), 0.0
+    i32 = torch.int32
+    a = _Shared(_here(q, "q"), _here(k_slab, "k_slab"), _here(v_slab, "v_slab"), _here(out, "out"), _here(block_table, "block_table", i32),
+                _here(plan.items, "items", i32), _here(plan.members, "members", i32), _here(plan.requests, "requests", i32),
+                _here(plan.joins, "joins", i32), _here(plan.part_o, "part_o", torch.float32) if n_slots else None,
+                _here(plan.part_ml, "part_ml", torch.float32) if n_slots else None, sink_heads, _code(q, "q"), block_table.shape[1],
+                block_table.shape[0], host.items.shape[0], host.members.shape[0], host.requests.shape[0], host.joins.shape[0], n_slots, T, Hq,
+                Hkv, D, P, pages, host.tile_rows, host.cluster, float(scale), 0 if sink is None else 1, 0.0 if sink is None else float(sink))
+    _check(_lib().ftk_shared_attention(ctypes.byref(a), _stream()), "shared_attention", 2 if host.items.shape[0] else 1)
 
 
 def attention_tc_fits(head_dim: int, page_size: int, group: int) -> bool:
@@ -1046,6 +1158,43 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
                              _dev(top_k, "top_k", torch.int32), _dev(top_p, "top_p", torch.float32),
                              _dev(u, "u", torch.float32), _dev(out, "out", torch.int32), _stream()),
            "sample")
+
+
+def sample_draws(logits: torch.Tensor, rows: Optional[torch.Tensor], temperature: torch.Tensor, top_k: torch.Tensor, top_p: torch.Tensor,
+                 min_p: torch.Tensor, u: torch.Tensor, out: torch.Tensor, logprobs: Optional[torch.Tensor] = None) -> None:
+    """One token per draw: draw ``r`` takes row ``rows[r]`` of float32 ``logits [N, V]`` (row ``r`` without ``rows``), so that several
+    requests that continue the same prompt draw from one row.
+
+    ``temperature[r] <= 0``: the lowest index of the largest logit.  Else with ``e = exp((x - max) / T)``: top-k keeps the logits that
+    reach the k-th largest (``top_k <= 0`` or ``>= V``: all); top-p then those that reach the largest value at which the kept mass is
+    ``top_p`` of what top-k left (``>= 1``: all); min-p those with ``e >= min_p`` (``<= 0``: all).  The largest logit always
+    stays, equal logits stay or go together.  ``out[r]`` is the first index whose running kept mass exceeds ``u[r]`` times the
+    kept mass.  ``logprobs[r]`` (float32, optional) is ``log_softmax(x)[out[r]]``, at temperature one and without the filters.
+
+    Sums and exponentials are 64-bit.  NaN counts as ``-inf``; a row of nothing else gives token 0 and ``-inf``.  A draw whose row
+    does not exist gives -1.  ``logits`` may be a view of rows that are farther apart.  :func:`sample` is the same without min-p, several
+    draws a row and log-probabilities, in 32-bit sums; its results are its own."""
+    if logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_cuda or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise KernelError("sample_draws: logits must be float32 rows [N, V] of adjacent elements on the device")
+    N, V = logits.shape
+    R = out.numel()
+    for name, t, dt in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                        ("min_p", min_p, torch.float32), ("u", u, torch.float32), ("rows", rows, torch.int32), ("logprobs", logprobs, torch.float32)):
+        if t is not None and (t.numel() < R or t.dtype != dt):
+            raise KernelError(f"sample_draws: {name} must be {dt} with {R} entries")
+    if V < 1 or (R and N < 1):
+        raise KernelError("sample_draws: no logits")
+    if rows is None and R > N:
+        raise KernelError(f"sample_draws: {R} draws from {N} rows")
+    stride = logits.stride(0) if N > 1 else V
+    if stride < V:
+        raise KernelError("sample_draws: rows of logits overlap")
+    if logits.device.index != torch.cuda.current_device():
+        raise KernelError(f"sample_draws: logits are on '{logits.device}', the current device is 'cuda:{torch.cuda.current_device()}'")
+    _check(_lib().ftk_sample_draws(logits.data_ptr(), stride, N, V, _here(rows, "rows") if rows is not None else None, R,
+                                   _here(temperature, "temperature"), _here(top_k, "top_k"), _here(top_p, "top_p"), _here(min_p, "min_p"),
+                                   _here(u, "u"), _here(out, "out", torch.int32), _here(logprobs, "logprobs") if logprobs is not None else None,
+                                   _stream()), "sample_draws")
 
 
 # --------------------------------------------------------------------------- the 32-bit stream

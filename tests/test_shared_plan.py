@@ -1,0 +1,98 @@
+"""Work lists of attention over shared keys, played through on the host."""
+
+import random
+
+import pytest
+import torch
+
+from freetoken_b200.engine.shared_plan import build_shared_plan, own_cluster, tile_members
+from freetoken_b200.errors import KernelError
+
+
+def covered(plan, n, rows):
+    """Per request: the key ranges of its pieces in the order in which they are joined, then its own."""
+    of_slot = {}
+    for mem0, k, row, kb, ke, slot0, *_ in plan.items.tolist():
+        assert kb < ke and 0 <= mem0 and mem0 + k <= len(plan.members)
+        members = plan.members[mem0:mem0 + k].tolist()
+        assert row == rows[members[0]]
+        for i, m in enumerate(members):
+            assert slot0 + i not in of_slot and slot0 + i < plan.n_slots
+            of_slot[slot0 + i] = (m, kb, ke)
+    assert sorted(of_slot) == list(range(plan.n_slots))
+    out = []
+    for i, (q, row, lo, hi, j0, k, *_) in enumerate(plan.requests.tolist()):
+        assert q == i and row == rows[i]
+        pieces = [of_slot[s] for s in plan.joins[j0:j0 + k].tolist()]
+        assert all(m == i for m, _, _ in pieces)
+        out.append([(a, b) for _, a, b in pieces] + [(lo, hi)])
+    return out
+
+
+@pytest.mark.parametrize("seed", range(30))
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_every_key_of_every_request_is_taken_once(seed, dtype):
+    rng = random.Random(seed)
+    heads, kv_heads = rng.choice([(48, 8), (16, 4), (16, 16), (40, 2), (128, 1)])
+    n = rng.randint(1, 40)
+    system = rng.choice([0, rng.randint(1, 3000)])
+    lens, spans, at = [system + rng.randint(0, 400) for _ in range(n)], [], 0
+    if system:
+        spans.append((list(range(n)), 0, system))
+    while at < n:
+        k = rng.randint(1, 7)
+        members = list(range(at, min(n, at + k)))
+        common = min(lens[m] for m in members)
+        if common > system:
+            spans.append((members, system, rng.randint(system + 1, common)))
+        at += k
+    rows = rng.sample(range(100), n)
+    plan = build_shared_plan(lens, spans, heads, kv_heads, 64, dtype, 16, table_rows=rows, sm_count=rng.choice([1, 16, 148]))
+    for i, pieces in enumerate(covered(plan, n, rows)):
+        edge = 0
+        for a, b in pieces:
+            assert a == edge and b >= a
+            edge = b
+        assert edge == lens[i]
+
+
+def test_lists_keep_their_sizes_while_requests_grow():
+    spans = [([0, 1, 2], 0, 640)]
+    plans = [build_shared_plan([700 + t, 660 + t, 690 + t], spans, 16, 4, 64, torch.bfloat16, 16) for t in range(60)]
+    # own parts of 20 to 119 tokens: the key changes only where the longest passes a power of two
+    assert len({p.key() for p in plans}) <= 2
+    assert len({p.items.tobytes() for p in plans}) == 1
+
+
+def test_members_are_dealt_to_tiles_evenly():
+    assert tile_members(64, 21) == [(0, 16), (16, 16), (32, 16), (48, 16)]
+    assert tile_members(3, 21) == [(0, 3)]
+    assert sum(k for _, k in tile_members(101, 7)) == 101
+
+
+def test_own_keys_are_split_while_the_gpu_is_not_full():
+    assert own_cluster(2048, 8, 64, 148) == 8
+    assert own_cluster(64, 8, 64, 148) == 1      # a tile of keys each at least
+    assert own_cluster(2048, 512, 64, 148) == 1  # enough requests
+    assert own_cluster(256, 200, 64, 148) == 2
+
+
+@pytest.mark.parametrize("lens,spans,what", [
+    ([10, 10], [([0, 2], 0, 5)], "different requests"),
+    ([10, 10], [([0, 0], 0, 5)], "different requests"),
+    ([10, 4], [([0, 1], 0, 5)], "within"),
+    ([10, 10], [([0, 1], -1, 5)], "within"),
+    ([10, 10, 10], [([0, 1], 0, 5), ([1, 2], 4, 6)], "overlap"),
+    ([10, 10], [([0, 1], 2, 5)], "leave out"),
+    ([-1], [], "negative"),
+])
+def test_refusals(lens, spans, what):
+    with pytest.raises(KernelError, match=what):
+        build_shared_plan(lens, spans, 8, 2, 64, torch.float32, 16)
+
+
+def test_refuses_heads_that_do_not_divide():
+    with pytest.raises(KernelError):
+        build_shared_plan([1], [], 7, 2, 64, torch.float32, 16)
+    with pytest.raises(KernelError):
+        build_shared_plan([1, 1], [], 8, 2, 64, torch.float32, 16, table_rows=[0])
