@@ -441,7 +441,7 @@ int ftk_moe_combine(const void* y, int dtype, const int32_t* route_pos, int n_to
 int ftk_variant_counts(char* buf, int cap, int reset);
 int ftk_read_status(int* out);
 // Writes `code` into a status word from the host (unit 0: grouped GEMM, 1: attention, 2: the delta rule's chunks, 3: linear attention's,
-// 4: 32-bit products), so that a caller's handling of a given-up wait can be tested without any wait running out on the device.
+// 4: 32-bit products, 5: attention over shared keys), so that a caller's handling of a given-up wait can be tested without any wait running out on the device.
 int ftk_debug_set_status(int unit, int code);
 // A wait on a barrier that nothing arrives at (give_up: and another warp gives up meanwhile): out[0] = 1 if it ended well, out[1] =
 // the nanoseconds it took (out on the device).
@@ -471,6 +471,8 @@ typedef struct {
   float sink;
 } FtkShared;
 int ftk_shared_attention(const FtkShared* a, void* stream);
+// Whether pieces of 256 query rows are taken (bfloat16).
+int ftk_shared_attention_tc_fits(int head_dim, int page_size, int group);
 // Copies inside the cache (cache_copy.cu): tensors [entries, blocks, parts, rows, row_bytes], contiguous (a slab: KV heads and tokens of a page; a state:
 // 1 and 1); pairs [n_pairs, pair_ints] int32 on the device: from, to and (pair_ints 3) how many of every part's rows.  No block
 // may be written by one pair and read or written by another; pairs with a block outside the tensor are left out.

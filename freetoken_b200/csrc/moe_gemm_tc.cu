@@ -819,27 +819,29 @@ int ftk_moe_gemm2_tc(const void* a, const void* w2, const int32_t* expert_offset
   return run_tc<false>(a, inter, w2, hidden, p, stream, "moe_gemm2 (tcgen05)");
 }
 
-// The files' status words: attention's, the delta rule's chunks', linear attention's, the 32-bit products', and this file's (looked at in
-// this order).
+// The files' status words: attention's, the delta rule's chunks', linear attention's, the 32-bit products', attention's over shared keys, and
+// this file's (looked at in this order).
 namespace ftk {
 int attention_tc_status(int* out);    // attention.cu
 int delta_chunk_status(int* out);     // delta_chunk.cu
 int gla_chunks_status(int* out);      // gla_chunks.cuh
 int moe_gemm_split_status(int* out);  // moe_gemm_split.cuh
+int shared_attention_status(int* out);  // shared_attention.cu
 int attention_tc_set_status(int code);
 int delta_chunk_set_status(int code);
 int gla_chunks_set_status(int code);
 int moe_gemm_split_set_status(int code);
+int shared_attention_set_status(int code);
 static int moe_gemm_tc_status(int* out) { return take_status(g_status, out); }
 static int moe_gemm_tc_set_status(int code) { return set_status(g_status, code); }
 }  // namespace ftk
 
 // Writes a code into a status word from the host, as a kernel whose wait ran out would: unit 0 = the
-// grouped GEMM's word, 1 = the attention kernel's, 2 = the delta rule's, 3 = linear attention's, 4 = the 32-bit products'.  It exists
+// grouped GEMM's word, 1 = the attention kernel's, 2 = the delta rule's, 3 = linear attention's, 4 = the 32-bit products', 5 = attention's over shared keys.  It exists
 // so that the path from a status word to the caller's error can be exercised without making any wait on the device run out.
 extern "C" int ftk_debug_set_status(int unit, int code) {
   int (*const set[])(int) = {ftk::moe_gemm_tc_set_status, ftk::attention_tc_set_status, ftk::delta_chunk_set_status, ftk::gla_chunks_set_status,
-                             ftk::moe_gemm_split_set_status};
+                             ftk::moe_gemm_split_set_status, ftk::shared_attention_set_status};
   constexpr int n = sizeof(set) / sizeof(set[0]);
   if (unit < 0 || unit >= n) {
     set_error("debug_set_status: unit must be 0 to %d, got %d", n - 1, unit);
@@ -855,7 +857,7 @@ extern "C" int ftk_debug_set_status(int unit, int code) {
 // Status of the bounded waits: out[0] = first code recorded since the last call (0 = none),
 // out[1] = block, then cleared.  Synchronises with the device.
 extern "C" int ftk_read_status(int* out) {
-  for (auto read : {ftk::attention_tc_status, ftk::delta_chunk_status, ftk::gla_chunks_status, ftk::moe_gemm_split_status, ftk::moe_gemm_tc_status}) {
+  for (auto read : {ftk::attention_tc_status, ftk::delta_chunk_status, ftk::gla_chunks_status, ftk::moe_gemm_split_status, ftk::shared_attention_status, ftk::moe_gemm_tc_status}) {
     if (read(out) != 0) {
       set_error("read_status: cannot read the status words");
       return 2;

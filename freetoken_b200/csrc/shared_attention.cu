@@ -580,7 +580,16 @@ static int launch_own_keys(const SharedParams& p, cudaStream_t s) {
 
 }  // namespace ftk
 
+#include "shared_attention_tc.cuh"
+
 using namespace ftk;
+
+namespace ftk {
+int shared_attention_status(int* out) { return take_status(g_shared_status, out); }  // (merged into ftk_read_status)
+int shared_attention_set_status(int code) { return set_status(g_shared_status, code); }
+}  // namespace ftk
+
+extern "C" int ftk_shared_attention_tc_fits(int head_dim, int page_size, int group) { return shared_tc_fits(head_dim, page_size, group) ? 1 : 0; }
 
 extern "C" int ftk_shared_attention(const FtkShared* a, void* stream) {
   FTK_REQUIRE(a, "shared_attention: null pointer");
@@ -615,9 +624,14 @@ extern "C" int ftk_shared_attention(const FtkShared* a, void* stream) {
   const int D = p.D;
   int rc = 0;
   if (p.n_items > 0) {
-    FTK_REQUIRE(a->tile_rows == kRows, "shared_attention: pieces of %d query rows are not taken", a->tile_rows);
-    note_variant(a->dtype == FTK_F32 ? "shared attention: float32, 16 rows" : "shared attention: bfloat16 mma.sync, 16 rows");
-    if (a->dtype == FTK_F32)
+    const bool tc = a->tile_rows == 2 * kShRows;
+    FTK_REQUIRE(tc || a->tile_rows == kRows, "shared_attention: pieces of %d query rows are not taken", a->tile_rows);
+    FTK_REQUIRE(!tc || (a->dtype == FTK_BF16 && shared_tc_fits(D, p.P, p.G) && p.scale > 0.f && (long long)p.num_pages * p.Hkv * p.P <= 0x7fffffffLL),
+                "shared_attention: pieces of 256 rows take bfloat16 heads of 64 or 128, pages of a multiple of 16, at most 128 heads per KV head and a positive scale");
+    FTK_REQUIRE(!tc || ((uintptr_t)a->part_o & 31) == 0, "shared_attention: partial results on 32-byte boundaries only");
+    note_variant(tc ? "shared attention: tcgen05, 256 rows" : a->dtype == FTK_F32 ? "shared attention: float32, 16 rows" : "shared attention: bfloat16 mma.sync, 16 rows");
+    if (tc) rc = D == 64 ? launch_shared_tc<64>(p, s) : launch_shared_tc<128>(p, s);
+    else if (a->dtype == FTK_F32)
       rc = D <= 64 ? launch_shared_rows<float, 64>(p, s) : D <= 128 ? launch_shared_rows<float, 128>(p, s) : launch_shared_rows<float, 256>(p, s);
     else
       rc = D <= 64 ? launch_shared_rows<__nv_bfloat16, 64>(p, s) : D <= 128 ? launch_shared_rows<__nv_bfloat16, 128>(p, s) : launch_shared_rows<__nv_bfloat16, 256>(p, s);

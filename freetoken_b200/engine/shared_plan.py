@@ -25,7 +25,14 @@ from ..errors import KernelError
 ITEM_INTS = 8     # first member, members, block-table row, first key, one past the last key, first slot, 0, 0
 REQUEST_INTS = 8  # query row, block-table row, first own key, one past the last, first join, joins, 0, 0
 ROWS_TILE = 16    # query rows of a piece on the kernels for few rows
+WIDE_TILE = 256   # on the tcgen05 kernel: two tiles of 128
+WIDE_KEYS = 128   # keys that kernel works on at a time
 MOST_CLUSTER = 8
+# what a piece costs the tcgen05 kernel: microseconds per key tile with one and with two query tiles, and per piece; and how fast
+# partial results are written and read again
+WIDE_ONE_US, WIDE_TWO_US, WIDE_PIECE_US, JOIN_BYTES_PER_US = 1.35, 2.1, 5.0, 2.5e6
+
+ROWS_KEYS = {torch.bfloat16: 64, torch.float32: 32}  # keys the kernels for few rows work on at a time
 
 Span = Tuple[Sequence[int], int, int]  # members (indices of requests), first position, one past the last
 
@@ -93,30 +100,66 @@ def own_cluster(longest: int, blocks: int, tile: int, sm_count: int) -> int:
     return cluster
 
 
+def takes_wide(dtype: torch.dtype, head_dim: int, page_size: int, group: int) -> bool:
+    """Whether the tcgen05 kernel takes these sizes (``csrc/shared_attention_tc.cuh: shared_tc_fits``)."""
+    return dtype == torch.bfloat16 and head_dim in (64, 128) and page_size % 16 == 0 and page_size >= 16 and group <= WIDE_TILE // 2
+
+
+def piece_lengths(units: np.ndarray, two: np.ndarray, members: np.ndarray, n_kv_heads: int, row_bytes: int, ctas: int) -> int:
+    """The most key tiles a piece of the tcgen05 kernel may have, by the estimated time of the launches: the kernel deals the sorted
+    list out to and fro over its CTAs, the busiest of them decides; partial results are written and read once per piece."""
+    best, best_t = 1, None
+    longest = int(units.max())
+    seen = set()
+    for k in range(1, 65):
+        most = -(-longest // k)
+        if most in seen:
+            continue
+        seen.add(most)
+        n = -(-units // most)
+        low, more = units // n, units % n
+        # of a tile's n pieces `more` have one unit more than the others
+        costs = np.concatenate([np.repeat(low + 1, more), np.repeat(low, n - more)]).astype(np.float64)
+        wide = np.concatenate([np.repeat(two, more), np.repeat(two, n - more)])
+        costs = WIDE_PIECE_US + costs * np.where(wide, WIDE_TWO_US, WIDE_ONE_US)
+        costs = np.sort(np.repeat(costs, n_kv_heads))[::-1]
+        g = min(ctas, costs.shape[0])
+        rounds = -(-costs.shape[0] // g)
+        costs = np.concatenate([costs, np.zeros(rounds * g - costs.shape[0])]).reshape(rounds, g)
+        costs[1::2] = costs[1::2, ::-1].copy()
+        t = float(costs.sum(axis=0).max()) + float((n * members).sum()) * row_bytes / JOIN_BYTES_PER_US
+        if best_t is None or t < best_t * 0.99:
+            best, best_t = most, t
+        if most == 1:
+            break
+    return best
+
+
 def build_shared_plan(kv_lens: Sequence[int], spans: Sequence[Span], n_heads: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype,
-                      page_size: int, table_rows: Optional[Sequence[int]] = None, sm_count: int = 148) -> SharedPlan:
+                      page_size: int, table_rows: Optional[Sequence[int]] = None, sm_count: int = 148,
+                      tile_rows: Optional[int] = None) -> SharedPlan:
     """The work list of one step: request ``i`` has query row ``i``, ``kv_lens[i]`` keys (its own token's among them) and row
     ``table_rows[i]`` (``i``) of the block table.
 
     ``spans``: (members, start, end) of keys that the members share: the block-table rows of all of them must name the same pages
     for these positions (the first member's row is read).  ``end`` may lie inside a page.  The spans of one request must not
-    overlap and leave no positions out in front of them; a span of a single member is that request's own."""
+    overlap and leave no positions out in front of them; a span of a single member is that request's own.
+
+    The tcgen05 kernel takes the shared keys where it takes the sizes, spans begin on multiples of 16 and a set has more query rows than
+    the kernel for few rows takes at a time; ``tile_rows`` (16 or 256) asks for one of the two."""
     n = len(kv_lens)
     if n_heads < 1 or n_kv_heads < 1 or n_heads % n_kv_heads:
         raise KernelError(f"shared_attention: {n_heads} query heads on {n_kv_heads} KV heads")
     rows = list(range(n)) if table_rows is None else [int(r) for r in table_rows]
     if len(rows) != n:
         raise KernelError("shared_attention: one block-table row per request")
+    if dtype not in ROWS_KEYS:
+        raise KernelError(f"shared_attention: dtype {dtype} is not supported (float32 or bfloat16)")
     if any(x < 0 for x in kv_lens):
         raise KernelError("shared_attention: a negative length")
     group = n_heads // n_kv_heads
-    tile_rows = ROWS_TILE
-    most = max(1, tile_rows // min(group, tile_rows))
-    chunks = -(-group // ROWS_TILE)
-    unit = 64 if dtype == torch.bfloat16 else 32  # keys a kernel works on at a time
-
     taken: List[List[Tuple[int, int]]] = [[] for _ in range(n)]
-    tiles: List[Tuple[List[int], int, int]] = []
+    sets: List[Tuple[List[int], int, int]] = []
     for members, start, end in spans:
         members = [int(m) for m in members]
         start, end = int(start), int(end)
@@ -130,24 +173,37 @@ def build_shared_plan(kv_lens: Sequence[int], spans: Sequence[Span], n_heads: in
             if any(a < end and start < b for a, b in taken[m]):
                 raise KernelError(f"shared_attention: request {m} is in two spans that overlap")
             taken[m].append((start, end))
-        for a, k in tile_members(len(members), most):
-            tiles.append((members[a:a + k], start, end))
+        sets.append((members, start, end))
 
-    # pieces of about as many units for every CTA that fits
-    heads = n_kv_heads * chunks
+    wide = takes_wide(dtype, head_dim, page_size, group) and all(start % 16 == 0 for _, start, _ in sets) \
+        and any(len(members) * group > ROWS_TILE for members, _, _ in sets)
+    if tile_rows is not None:
+        if tile_rows not in (ROWS_TILE, WIDE_TILE) or (tile_rows == WIDE_TILE and (not takes_wide(dtype, head_dim, page_size, group) or any(
+                start % 16 for _, start, _ in sets))):
+            raise KernelError(f"shared_attention: pieces of {tile_rows} query rows are not taken at these sizes")
+        wide = tile_rows == WIDE_TILE
+    chunks = -(-group // ROWS_TILE)  # (of the kernels for few rows)
+    most = 2 * (WIDE_TILE // 2 // group) if wide else max(1, ROWS_TILE // min(group, ROWS_TILE))
+    unit = WIDE_KEYS if wide else ROWS_KEYS[dtype]
+    tiles = [(members[a:a + k], start, end) for members, start, end in sets for a, k in tile_members(len(members), most)]
     units = [-(-(end - start) // unit) for _, start, end in tiles]
-    length = max(4, -(-sum(units) * heads // (4 * sm_count)))
+    if wide and tiles:
+        length = piece_lengths(np.array(units), np.array([2 * len(m) > most for m, _, _ in tiles]), np.array([len(m) for m, _, _ in tiles]),
+                               n_kv_heads, 8 * n_heads * head_dim, sm_count)
+    else:  # pieces of about as many units for every CTA that fits
+        length = max(4, -(-sum(units) * n_kv_heads * chunks // (4 * sm_count)))
     items, member_rows, slots = [], [], [[] for _ in range(n)]
     n_slots = 0
     for (members, start, end), u in zip(tiles, units):
         first = len(member_rows)
         member_rows += members
         for a, k in tile_members(u, length):
-            items.append((first, len(members), rows[members[0]], start + a * unit, min(end, start + (a + k) * unit), n_slots, 0, 0))
+            cost = k * (WIDE_TWO_US if 2 * len(members) > most else WIDE_ONE_US) if wide else float(k)
+            items.append((-cost, first, len(members), rows[members[0]], start + a * unit, min(end, start + (a + k) * unit), n_slots, 0, 0))
             for i, m in enumerate(members):
                 slots[m].append((start + a * unit, n_slots + i))
             n_slots += len(members)
-    items.sort(key=lambda it: it[3] - it[4])  # the longest first
+    items = [it[1:] for it in sorted(items, key=lambda it: it[0])]  # the longest first
 
     # what is a request's own: one range behind its spans
     requests, joins, longest = [], [], 1
@@ -161,8 +217,7 @@ def build_shared_plan(kv_lens: Sequence[int], spans: Sequence[Span], n_heads: in
         requests.append((i, rows[i], begin, int(kv_lens[i]), len(joins), len(own), 0, 0))
         joins += own
         longest = max(longest, int(kv_lens[i]) - begin)
-    blocks = max(1, n * heads)
-    cluster = own_cluster(1 << (longest - 1).bit_length(), blocks, unit, sm_count)
+    cluster = own_cluster(1 << (longest - 1).bit_length(), max(1, n * n_kv_heads * chunks), ROWS_KEYS[dtype], sm_count)
     as_int = lambda x, w: np.asarray(x, dtype=np.int32).reshape(-1, w) if w else np.asarray(x, dtype=np.int32)  # noqa: E731
     return SharedPlan(as_int(items, ITEM_INTS), as_int(member_rows, 0), as_int(requests, REQUEST_INTS), as_int(joins, 0), n_slots,
-                      tile_rows, cluster, n, n_heads, n_kv_heads, head_dim)
+                      WIDE_TILE if wide else ROWS_TILE, cluster, n, n_heads, n_kv_heads, head_dim)

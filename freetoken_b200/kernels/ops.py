@@ -174,6 +174,7 @@ _SIGNATURES = {
     "ftk_diff_heads": [_vp, _i, _i, _vp, _f, _f, _vp, _i, _i, _i, _vp],
     "ftk_act_and_mul": [_vp, _i, _i, _i, _i, _f, _f, _vp, _vp],
     "ftk_sample": [_vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp],
+    "ftk_shared_attention_tc_fits": [_i, _i, _i],
     "ftk_shared_attention": [ctypes.POINTER(_Shared), _vp],
     "ftk_copy_blocks": [ctypes.POINTER(_CopyTensor), _i, _vp, _i, _i, _vp],
     "ftk_sample_draws": [_vp, ctypes.c_longlong, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
@@ -278,7 +279,7 @@ def read_status() -> int:
     for the device.  101-104 come from the tensor-core grouped GEMM (producer, accumulator
     hand-back, operand arrival, accumulator arrival), 501-506 from the delta rule's chunks,
     601 and 602 from those of gated linear attention, 701 from
-    the 32-bit expert products."""
+    the 32-bit expert products, 801-809 from attention over shared keys."""
     out = (ctypes.c_int * 2)()
     status = _lib().ftk_read_status(out)
     if status != 0:
@@ -310,7 +311,7 @@ def variant_counts(reset: bool = False) -> dict:
 
 def debug_set_status(unit: int, code: int) -> None:
     """Write ``code`` into a status word from the host (``unit`` 0: grouped GEMM, 1: attention, 2: the delta rule's chunks, 3: gated
-    linear attention's, 4: 32-bit products), as a kernel whose bounded wait ran out would have.  For tests of the error path;
+    linear attention's, 4: 32-bit products, 5: attention over shared keys), as a kernel whose bounded wait ran out would have.  For tests of the error path;
     nothing waits."""
     _check(_lib().ftk_debug_set_status(int(unit), int(code)), "debug_set_status", 0)
 

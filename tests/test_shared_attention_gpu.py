@@ -99,9 +99,9 @@ def run(q, k, v, table, plan, scale, sink=None, fill=7.0):
     return out.cpu()
 
 
-def check(lens, spans, heads, kv_heads, dim, page, dtype, seed=0, sink=None, spread=1.5, sm_count=148):
+def check(lens, spans, heads, kv_heads, dim, page, dtype, seed=0, sink=None, spread=1.5, sm_count=148, tile_rows=None):
     q, k, v, table = case(lens, spans, heads, kv_heads, dim, page, dtype, seed, extra_rows=2, spread=spread)
-    plan = build_shared_plan(lens, spans, heads, kv_heads, dim, dtype, page, sm_count=sm_count).to(DEV)
+    plan = build_shared_plan(lens, spans, heads, kv_heads, dim, dtype, page, sm_count=sm_count, tile_rows=tile_rows).to(DEV)
     scale = dim ** -0.5
     per_head = sink if sink is None or isinstance(sink, torch.Tensor) else torch.full((heads,), sink)
     got = run(q, k, v, table, plan, scale, sink.to(DEV) if isinstance(sink, torch.Tensor) else sink)
@@ -142,6 +142,34 @@ SIZES = [
 @pytest.mark.parametrize("at", range(len(SIZES)))
 def test_sizes(at, dtype):
     check(*SIZES[at], dtype, seed=at)
+
+
+WIDE = [
+    # the tcgen05 kernel: one and two query tiles, pieces that end anywhere in a key tile, several pieces a CTA
+    ([40, 50], [([0, 1], 0, 16)], 16, 4, 128, 16),
+    ([40, 50], [([0, 1], 0, 17)], 4, 4, 64, 16),
+    ([150] * 64, [(list(range(64)), 0, 144)], 6, 1, 128, 16),                                       # two tiles of 16 members each
+    ([600] * 43, [(list(range(42)), 0, 512)], 12, 2, 64, 32),                                       # 42 members: two full tiles
+    ([300] * 5, [(list(range(5)), 0, 272)], 128, 1, 128, 16),                                       # a member a tile
+    ([1300, 1400, 1290, 1288, 1500, 1310], [(list(range(6)), 0, 640), ([0, 1, 2], 640, 1280), ([3, 4, 5], 640, 1288)], 24, 2, 128, 64),
+    ([3000] * 30, [(list(range(30)), 0, 2900)], 48, 8, 128, 16),
+    ([520] * 100, [(list(range(k, 100, 10)), 0, 320 + 16 * k) for k in range(10)], 16, 4, 64, 16),  # many sets of different lengths
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tile_rows,sm_count", [(16, 148), (256, 148), (256, 7)])  # (few SMs in the list's eyes: long pieces)
+@pytest.mark.parametrize("at", range(len(WIDE)))
+def test_both_forms_for_shared_keys(at, tile_rows, sm_count):
+    ops.variant_counts(reset=True)
+    plan = check(*WIDE[at], BF16, seed=at, tile_rows=tile_rows, sm_count=sm_count)
+    assert plan.host.tile_rows == tile_rows
+    assert ops.variant_counts()["shared attention: tcgen05, 256 rows" if tile_rows == 256 else "shared attention: bfloat16 mma.sync, 16 rows"] == 1
+
+
+@pytest.mark.gpu
+def test_large_scores_on_tcgen05():
+    check([1900, 1950] * 10, [(list(range(20)), 0, 1880)], 12, 2, 128, 16, BF16, spread=12.0, tile_rows=256)
 
 
 @pytest.mark.gpu
@@ -248,6 +276,8 @@ def test_refusals():
             ops.shared_attention(*args, 0.125)
     with pytest.raises(KernelError):
         ops.shared_attention(q, k, v, table, plan, out, 0.125, sink=torch.zeros(3, device=DEV))
+    with pytest.raises(KernelError, match="positive scale"):
+        ops.shared_attention(q, k, v, table, build_shared_plan(lens, spans, 8, 2, 64, BF16, 16, tile_rows=256).to(DEV), out, -0.125)
     wide = torch.empty((3, 8, 24), dtype=BF16, device=DEV)
     slab = torch.empty((4, 2, 16, 24), dtype=BF16, device=DEV)
     with pytest.raises(KernelError, match="head_dim"):

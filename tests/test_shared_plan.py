@@ -91,6 +91,24 @@ def test_refusals(lens, spans, what):
         build_shared_plan(lens, spans, 8, 2, 64, torch.float32, 16)
 
 
+def test_the_wide_form_is_taken_where_it_fits():
+    rows = lambda members, heads=16, kv=4, dim=64, dtype=torch.bfloat16, page=16, **kw: build_shared_plan(  # noqa: E731
+        [200] * 40, [(list(range(members)), 0, 160)], heads, kv, dim, dtype, page, **kw).tile_rows
+    assert rows(20) == 256 and rows(20, dim=128) == 256
+    assert rows(4) == 16  # 16 query rows
+    assert rows(20, dtype=torch.float32) == rows(20, dim=48) == rows(20, page=8) == rows(20, heads=516) == 16
+    assert rows(20, tile_rows=16) == 16 and rows(4, tile_rows=256) == 256
+    assert build_shared_plan([200] * 9, [(list(range(9)), 0, 30), (list(range(9)), 30, 160)], 16, 4, 64, torch.bfloat16, 16).tile_rows == 16
+    for kw in (dict(dim=48), dict(dtype=torch.float32), dict(page=8)):
+        with pytest.raises(KernelError):
+            rows(20, tile_rows=256, **kw)
+    with pytest.raises(KernelError):
+        rows(20, tile_rows=64)
+    with pytest.raises(KernelError):
+        build_shared_plan([1], [], 8, 2, 64, torch.float16, 16)
+    assert build_shared_plan([5], [], 8, 2, 64, torch.bfloat16, 16, tile_rows=256).items.shape == (0, 8)
+
+
 def test_refuses_heads_that_do_not_divide():
     with pytest.raises(KernelError):
         build_shared_plan([1], [], 7, 2, 64, torch.float32, 16)
