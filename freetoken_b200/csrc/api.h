@@ -466,6 +466,7 @@ typedef struct {
   int dtype, bt_stride, bt_rows, n_items, n_members, n_requests, n_joins, n_slots, n_rows, n_q_heads, n_kv_heads, head_dim, page_size, num_pages;
   int tile_rows;               // query rows of a piece of shared keys at most: 16, or 256 (tcgen05)
   int cluster;                 // CTAs that share a request's own keys: 1, 2, 4 or 8
+  int own_tiles;               // tiles of 64 own keys (bfloat16) that a CTA has at most
   float scale;
   int has_sink;
   float sink;

@@ -8,7 +8,7 @@
 // values (relative 2^-9 each, independent of one another: as far off as the rounding of the result itself).
 //
 // Two launches.  The first works through pieces of shared keys (engine/shared_plan.py cuts them): items of 8 int32 = first member,
-// members, block-table row, first key, one past the last key, first slot, 0, 0; members[] holds query rows; a member's partial results
+// members, block-table row, first key, one past the last key, first slot, split, 0; members[] holds query rows; a member's partial results
 // lie in slot (first slot + its number in the item).  The second has a cluster of CTAs per (request, KV head): it attends over the
 // request's own keys, split over the cluster, and joins them with the request's slots in the order of its list, so results do not
 // depend on which block came first.  requests[] = query row, block-table row, first own key, one past the last, first entry in joins[], entries, 0, 0.
@@ -43,7 +43,9 @@ struct SharedParams {
   int n_slots;
   int n_rows, Hq, Hkv, G, D, P, num_pages;
   int Gc, chunks;  // query heads of one KV head that a rows16 CTA takes (G, 16 at most), and in how many chunks all are taken
+  int page_shift;  // log2 of the page size, -1 where it is no power of two
   int cluster;     // CTAs that share a request's own keys
+  int stages;      // places for tiles of 64 keys and values: three, or as many as a CTA's own keys take
   float scale;
   int has_sink;
   float sink;
@@ -61,11 +63,12 @@ struct Rows {
 
 struct Piece {
   int mem0, n_mem, bt_row, kb, ke, slot0;
+  bool split;  // (shared_attention_tc.cuh) the members' slots come twice: of even and of odd key tiles
   bool ok;
 };
 __device__ __forceinline__ Piece load_piece(const SharedParams& p, int idx) {
   const int32_t* w = p.items + (size_t)idx * 8;
-  Piece it{w[0], w[1], w[2], w[3], w[4], w[5], false};
+  Piece it{w[0], w[1], w[2], w[3], w[4], w[5], w[6] != 0, false};
   it.ok = it.mem0 >= 0 && it.n_mem > 0 && it.n_mem <= p.n_members - it.mem0 && it.bt_row >= 0 && it.bt_row < p.bt_rows && it.kb >= 0 &&
           it.ke > it.kb && it.slot0 >= 0 && it.n_mem <= p.n_slots - it.slot0;
   return it;
@@ -73,11 +76,11 @@ __device__ __forceinline__ Piece load_piece(const SharedParams& p, int idx) {
 
 // Element offset of key `pos` of block-table row `bt_row` in a [pages, KV heads, P, D] slab, or -1 where the table names no page of it.
 __device__ __forceinline__ long long key_offset(const SharedParams& p, int bt_row, int kvh, int pos) {
-  const int block = pos / p.P;
+  const int block = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.P;
   if (block >= p.bt_stride) return -1;
   const int page = p.block_table[(size_t)bt_row * p.bt_stride + block];
   if (page < 0 || page >= p.num_pages) return -1;
-  return (((long long)page * p.Hkv + kvh) * p.P + pos % p.P) * p.D;
+  return (((long long)page * p.Hkv + kvh) * p.P + (pos - block * p.P)) * p.D;
 }
 
 __device__ __forceinline__ uint32_t sh_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -122,18 +125,17 @@ struct RowsResult {
 
 // ---- bfloat16: the four warps take 16 keys each of a tile of 64, three tiles on their way
 constexpr int kTileKeys = 64, kTileStages = 3;
-template <int DMAX>
-constexpr size_t rows16_bf16_smem(int d) {
-  const size_t tiles = (size_t)(kRows + 2 * kTileStages * kTileKeys) * (d + 8) * 2, merge = (size_t)(10 * kRows + 4 * kRows * d) * 4 + 16;
+inline size_t rows16_bf16_smem(int d, int stages) {
+  const size_t tiles = (size_t)(kRows + 2 * stages * kTileKeys) * (d + 8) * 2, merge = (size_t)(10 * kRows + 4 * kRows * d) * 4 + 16;
   return tiles > merge ? tiles : merge;
 }
 
-template <int DMAX>
+template <int DMAX, bool EXACT>
 __device__ __forceinline__ RowsResult rows16_bf16(const SharedParams& p, const Rows& rw, int bt_row, int kvh, int kb, int ke, unsigned char* smem) {
-  const int D = p.D, ld = D + 8;  // (16 bytes more: ldmatrix without bank conflicts)
+  const int D = EXACT ? DMAX : p.D, ld = D + 8;  // (16 bytes more: ldmatrix without bank conflicts)
   __nv_bfloat16* sq = reinterpret_cast<__nv_bfloat16*>(smem);
   __nv_bfloat16* sk0 = sq + kRows * ld;
-  __nv_bfloat16* sv0 = sk0 + kTileStages * kTileKeys * ld;
+  __nv_bfloat16* sv0 = sk0 + p.stages * kTileKeys * ld;
   __shared__ long long row_off[4][kTileKeys];  // where the keys of tile t lie: row_off[t & 3]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pieces = D >> 3;
   const __nv_bfloat16* q = (const __nv_bfloat16*)p.q;
@@ -159,7 +161,8 @@ __device__ __forceinline__ RowsResult rows16_bf16(const SharedParams& p, const R
       copy16(sv + j * ld + c * 8, vbase + o, there);
     }
   };
-  const int n_tiles = (ke - kb + kTileKeys - 1) / kTileKeys;
+  int n_tiles = (ke - kb + kTileKeys - 1) / kTileKeys;
+  if (p.stages < kTileStages) n_tiles = min(n_tiles, p.stages);  // (fewer places than three are given where they hold every key)
 #pragma unroll
   for (int t = 0; t < 3; ++t) publish(t, look_up(t));
   for (int i = threadIdx.x; i < kRows * pieces; i += kRowThreads) {
@@ -185,6 +188,10 @@ __device__ __forceinline__ RowsResult rows16_bf16(const SharedParams& p, const R
     if (t + 2 < n_tiles) load(t + 2);
     copy_commit();
     const long long next = look_up(t + 3);
+    if (kb + t * kTileKeys + warp * 16 >= ke) {  // (none of this warp's keys is there)
+      publish(t + 3, next);
+      continue;
+    }
     const __nv_bfloat16* sk = sk0 + (t % kTileStages * kTileKeys + warp * 16) * ld;  // this warp's keys
     const __nv_bfloat16* sv = sv0 + (t % kTileStages * kTileKeys + warp * 16) * ld;
     float s[2][4] = {};
@@ -262,6 +269,9 @@ __device__ __forceinline__ RowsResult rows16_bf16(const SharedParams& p, const R
   float* wm = rl + kRows;
   float* wl = wm + 4 * kRows;
   float* wo = wl + 4 * kRows;
+  // (a NaN among scores that are all NaN or not there has no maximum: it must not look like a row without keys)
+  if (l0 != l0 && m0 == -INFINITY) m0 = 0.f;
+  if (l1 != l1 && m1 == -INFINITY) m1 = 0.f;
   if ((lane & 3) == 0) {
     wm[warp * kRows + r0] = m0; wm[warp * kRows + r1] = m1;
     wl[warp * kRows + r0] = l0; wl[warp * kRows + r1] = l1;
@@ -274,19 +284,25 @@ __device__ __forceinline__ RowsResult rows16_bf16(const SharedParams& p, const R
     *reinterpret_cast<float2*>(wo + (warp * kRows + r1) * D + d) = make_float2(o[i][2], o[i][3]);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < kRows * D; i += kRowThreads) {
-    const int r = i / D;
-    float M = -INFINITY, L = 0.f, acc = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, wm[w * kRows + r]);
+  const int quads = D >> 2;
+  for (int i = threadIdx.x; i < rw.n * quads; i += kRowThreads) {
+    const int r = i / quads;
+    float mw[4], M = -INFINITY, L = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float mw = wm[w * kRows + r], f = mw == -INFINITY ? 0.f : exp2_fast(mw - M);
-      L += wl[w * kRows + r] * f;
-      if (f != 0.f) acc += wo[w * kRows * D + i] * f;
+      mw[w] = wm[w * kRows + r];
+      M = fmaxf(M, mw[w]);
     }
-    wo[i] = acc;
-    if (i == r * D) {
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = mw[w] == -INFINITY ? 0.f : exp2_fast(mw[w] - M);
+      const float4 x = *reinterpret_cast<const float4*>(wo + w * kRows * D + i * 4);
+      L += wl[w * kRows + r] * f;
+      acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
+    }
+    *reinterpret_cast<float4*>(wo + i * 4) = acc;
+    if (i == r * quads) {
       rm[r] = M;
       rl[r] = L;
     }
@@ -299,10 +315,10 @@ __device__ __forceinline__ RowsResult rows16_bf16(const SharedParams& p, const R
 constexpr int kF32Keys = 32;
 inline size_t rows16_f32_smem(int d) { return ((size_t)kRows * d + 4 * kF32Keys * (d + 4) + 2 * kRows) * 4; }
 
-template <int DMAX>
+template <int DMAX, bool EXACT>
 __device__ __forceinline__ RowsResult rows16_f32(const SharedParams& p, const Rows& rw, int bt_row, int kvh, int kb, int ke, unsigned char* smem) {
   constexpr int COLS = DMAX / 32, RW = kRows / 4;
-  const int D = p.D, ld = D + 4;
+  const int D = EXACT ? DMAX : p.D, ld = D + 4;
   float* rm = reinterpret_cast<float*>(smem);
   float* rl = rm + kRows;
   float* sq = rl + kRows;             // [16][D] queries, in the end the outputs
@@ -420,7 +436,7 @@ __device__ __forceinline__ RowsResult rows16_f32(const SharedParams& p, const Ro
           if (lane + 32 * i < D) sq[r * D + lane + 32 * i] = acc[f][i];
       }
     if (lane == 0) {
-      rm[r] = me;
+      rm[r] = le != le && me == -INFINITY ? 0.f : me;  // (NaN is not a row without keys)
       rl[r] = le;
     }
   }
@@ -428,10 +444,11 @@ __device__ __forceinline__ RowsResult rows16_f32(const SharedParams& p, const Ro
   return {rm, rl, sq};
 }
 
-template <typename T, int DMAX>
+// EXACT: the head size is DMAX itself, so that rows are taken apart by shifts (a CTA with a few keys is bound by its instructions)
+template <typename T, int DMAX, bool EXACT>
 __device__ __forceinline__ RowsResult rows16(const SharedParams& p, const Rows& rw, int bt_row, int kvh, int kb, int ke, unsigned char* smem) {
-  if constexpr (sizeof(T) == 2) return rows16_bf16<DMAX>(p, rw, bt_row, kvh, kb, ke, smem);
-  else return rows16_f32<DMAX>(p, rw, bt_row, kvh, kb, ke, smem);
+  if constexpr (sizeof(T) == 2) return rows16_bf16<DMAX, EXACT>(p, rw, bt_row, kvh, kb, ke, smem);
+  else return rows16_f32<DMAX, EXACT>(p, rw, bt_row, kvh, kb, ke, smem);
 }
 // maxima are of scores times log2 e in bfloat16, of scores in 32 bits
 template <typename T>
@@ -441,7 +458,7 @@ __device__ __forceinline__ float weight(float m, float M) {
 }
 
 // ================================================================= shared keys, 16 rows a CTA
-template <typename T, int DMAX>
+template <typename T, int DMAX, bool EXACT>
 __global__ void __launch_bounds__(kRowThreads) shared_rows_kernel(const __grid_constant__ SharedParams p) {
   pdl_wait();
   pdl_trigger();
@@ -451,11 +468,12 @@ __global__ void __launch_bounds__(kRowThreads) shared_rows_kernel(const __grid_c
   const int heads = min(p.Gc, p.G - chunk * p.Gc);
   if (!it.ok || it.n_mem * heads > kRows) return;
   const Rows rw{p.members + it.mem0, 0, heads, kvh * p.G + chunk * p.Gc, it.n_mem * heads};
-  const RowsResult res = rows16<T, DMAX>(p, rw, it.bt_row, kvh, it.kb, it.ke, smem);
-  for (int i = threadIdx.x; i < rw.n * (p.D >> 2); i += kRowThreads) {
-    const int r = i / (p.D >> 2), d = i % (p.D >> 2) * 4;
+  const RowsResult res = rows16<T, DMAX, EXACT>(p, rw, it.bt_row, kvh, it.kb, it.ke, smem);
+  const int D = EXACT ? DMAX : p.D, quads = D >> 2;
+  for (int i = threadIdx.x; i < rw.n * quads; i += kRowThreads) {
+    const int r = i / quads, d = i % quads * 4;
     const size_t at = (size_t)(it.slot0 + r / heads) * p.Hq + rw.head(r);
-    *reinterpret_cast<float4*>(p.part_o + at * p.D + d) = *reinterpret_cast<const float4*>(res.o + r * p.D + d);
+    *reinterpret_cast<float4*>(p.part_o + at * D + d) = *reinterpret_cast<const float4*>(res.o + r * D + d);
     if (d == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(res.m[r], res.l[r]);
   }
 }
@@ -486,13 +504,17 @@ __device__ __forceinline__ void store4(T* to, float4 v) {
   else *reinterpret_cast<uint2*>(to) = make_uint2(two_bf16(v.x, v.y), two_bf16(v.z, v.w));
 }
 
-template <typename T, int DMAX>
+constexpr int kJoinRun = 32;  // shared pieces whose maxima and sums are fetched together
+
+template <typename T, int DMAX, bool EXACT>
 __global__ void __launch_bounds__(kRowThreads) own_keys_kernel(const __grid_constant__ SharedParams p) {
   // With shared pieces in front of it this kernel starts while they run: queries, keys and values were written in front of them,
   // and only their partial results are waited for.
   if (!p.early) pdl_wait();
   extern __shared__ __align__(16) unsigned char smem[];
-  const int C = p.cluster, rank = blockIdx.x % C;
+  __shared__ int slots[kJoinRun];
+  __shared__ float2 ml[kJoinRun][kRows];
+  const int C = p.cluster, rank = blockIdx.x % C, tid = threadIdx.x;
   int work = blockIdx.x / C;
   const int chunk = work % p.chunks;
   work /= p.chunks;
@@ -502,80 +524,133 @@ __global__ void __launch_bounds__(kRowThreads) own_keys_kernel(const __grid_cons
   const int heads = min(p.Gc, p.G - chunk * p.Gc), head0 = kvh * p.G + chunk * p.Gc;
   const bool ok = tok >= 0 && tok < p.n_rows && bt_row >= 0 && bt_row < p.bt_rows && from >= 0 && join0 >= 0 && w[5] >= 0 && w[5] <= p.n_joins - join0;
   const int n_join = ok ? w[5] : 0;
+  if (tid < kJoinRun) slots[tid] = tid < n_join ? p.joins[join0 + tid] : -1;
   // this CTA's share of the keys, in whole tiles
   const int tile = sizeof(T) == 2 ? kTileKeys : kF32Keys;
   const int own = ok ? max(0, to - from) : 0, share = ((own + C - 1) / C + tile - 1) / tile * tile;
   const int kb = from + min(own, rank * share), ke = from + min(own, rank * share + share);
   const Rows rw{nullptr, tok, heads, head0, ok ? heads : 0};
-  const RowsResult res = rows16<T, DMAX>(p, rw, bt_row, kvh, kb, ke, smem);
+  const RowsResult res = rows16<T, DMAX, EXACT>(p, rw, bt_row, kvh, kb, ke, smem);
   if (p.early) pdl_wait();
   pdl_trigger();
+  // A row's 32-bit results are spread over the cluster's threads, four columns each; its shared pieces come first, in their order.
+  const int D = EXACT ? DMAX : p.D;
+  constexpr int kQuads = DMAX * kRows / 4 / kRowThreads;
+  const int quads = D >> 2, at0 = rank * kRowThreads + tid;
+  float M[kQuads], L[kQuads];
+  float4 acc[kQuads];
+#pragma unroll
+  for (int u = 0; u < kQuads; ++u) {
+    M[u] = -INFINITY;
+    L[u] = 0.f;
+    acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  auto scale = [&](int u, float m) {  // a new maximum
+    const float f = weight<T>(M[u], m);
+    L[u] *= f;
+    acc[u].x *= f; acc[u].y *= f; acc[u].z *= f; acc[u].w *= f;
+    M[u] = m;
+  };
+  auto add = [&](int u, float m, float l, float4 o) {
+    const float f = weight<T>(m, M[u]);
+    if (f != 0.f) {  // (a piece of weight 0 may hold anything)
+      L[u] += l * f;
+      acc[u].x += o.x * f; acc[u].y += o.y * f; acc[u].z += o.z * f; acc[u].w += o.w * f;
+    }
+  };
+  for (int j0 = 0; j0 < n_join; j0 += kJoinRun) {
+    const int n = min(kJoinRun, n_join - j0);
+    if (j0 > 0) {
+      __syncthreads();
+      if (tid < kJoinRun) slots[tid] = tid < n ? p.joins[join0 + j0 + tid] : -1;
+      __syncthreads();
+    }
+    for (int i = tid; i < n * kRows; i += kRowThreads) {
+      const int j = i / kRows, r = i % kRows, slot = slots[j];
+      if (r < heads)
+        ml[j][r] = slot >= 0 && slot < p.n_slots ? *reinterpret_cast<const float2*>(p.part_ml + ((size_t)slot * p.Hq + head0 + r) * 2) : make_float2(-INFINITY, 0.f);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kQuads; ++u) {
+      const int i = at0 + u * C * kRowThreads;
+      if (i >= rw.n * quads) break;
+      const int r = i / quads, d = i % quads * 4;
+      const float* o = p.part_o + (size_t)(head0 + r) * D + d;
+      float m = M[u];
+      for (int j = 0; j < n; ++j) m = fmaxf(m, ml[j][r].x);
+      scale(u, m);
+      for (int j = 0; j < n; j += 8) {  // eight loads on their way before the first use
+        float4 x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int slot = j + e < n ? slots[j + e] : -1;
+          x[e] = slot >= 0 && slot < p.n_slots ? __ldcg(reinterpret_cast<const float4*>(o + (size_t)slot * p.Hq * D)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (j + e < n) add(u, ml[j + e][r].x, ml[j + e][r].y, x[e]);
+      }
+    }
+  }
   if (C > 1) cluster_barrier();
   const uint32_t my_m = sh_addr(res.m), my_l = sh_addr(res.l), my_o = sh_addr(res.o);  // (at the same place in every CTA)
-  const int quads = p.D >> 2;
-  for (int i = rank * kRowThreads + threadIdx.x; i < rw.n * quads; i += C * kRowThreads) {
+#pragma unroll
+  for (int u = 0; u < kQuads; ++u) {
+    const int i = at0 + u * C * kRowThreads;
+    if (i >= rw.n * quads) break;
     const int r = i / quads, d = i % quads * 4, head = head0 + r;
-    float M = -INFINITY;
-    for (int c = 0; c < C; ++c) M = fmaxf(M, C > 1 ? cluster_f32(of_rank(my_m + r * 4, c)) : res.m[r]);
-    for (int j = 0; j < n_join; ++j) {
-      const int slot = p.joins[join0 + j];
-      if (slot >= 0 && slot < p.n_slots) M = fmaxf(M, p.part_ml[((size_t)slot * p.Hq + head) * 2]);
-    }
-    float L = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](float m, float l, float4 o) {
-      const float f = weight<T>(m, M);
-      if (f != 0.f) {
-        L += l * f;
-        acc.x += o.x * f; acc.y += o.y * f; acc.z += o.z * f; acc.w += o.w * f;
-      }
-    };
-    for (int j = 0; j < n_join; ++j) {
-      const int slot = p.joins[join0 + j];
-      if (slot < 0 || slot >= p.n_slots) continue;
-      const size_t at = (size_t)slot * p.Hq + head;
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-      add(ml.x, ml.y, *reinterpret_cast<const float4*>(p.part_o + at * p.D + d));
-    }
+    float m = M[u];
+    for (int c = 0; c < C; ++c) m = fmaxf(m, C > 1 ? cluster_f32(of_rank(my_m + r * 4, c)) : res.m[r]);
+    scale(u, m);
     for (int c = 0; c < C; ++c) {
       if (C > 1)
-        add(cluster_f32(of_rank(my_m + r * 4, c)), cluster_f32(of_rank(my_l + r * 4, c)), cluster_f32x4(of_rank(my_o + (r * p.D + d) * 4, c)));
+        add(u, cluster_f32(of_rank(my_m + r * 4, c)), cluster_f32(of_rank(my_l + r * 4, c)), cluster_f32x4(of_rank(my_o + (r * D + d) * 4, c)));
       else
-        add(res.m[r], res.l[r], *reinterpret_cast<const float4*>(res.o + r * p.D + d));
+        add(u, res.m[r], res.l[r], *reinterpret_cast<const float4*>(res.o + r * D + d));
     }
-    if (p.has_sink) {  // a key without a value; a row of nothing else gives zeros
-      const float s = (p.sink_heads ? __ldg(p.sink_heads + head) : p.sink) - (M == -INFINITY ? 0.f : sizeof(T) == 2 ? M / kLog2e : M);
-      if (M != -INFINITY) L += expf(s);
-    }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
-    store4((T*)p.out + ((size_t)tok * p.Hq + head) * p.D + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+    // a sink is a key without a value; a row of nothing else gives zeros
+    if (p.has_sink && m != -INFINITY) L[u] += expf((p.sink_heads ? __ldg(p.sink_heads + head) : p.sink) - (sizeof(T) == 2 ? m / kLog2e : m));
+    const float inv = L[u] == 0.f ? 0.f : 1.f / L[u];  // (NaN stays)
+    store4((T*)p.out + ((size_t)tok * p.Hq + head) * D + d, make_float4(acc[u].x * inv, acc[u].y * inv, acc[u].z * inv, acc[u].w * inv));
   }
   if (C > 1) cluster_barrier();  // nobody leaves while its shared memory is read
 }
 
-template <typename T, int DMAX>
-static size_t rows_smem(int d) {
-  if constexpr (sizeof(T) == 2) return rows16_bf16_smem<DMAX>(d);
+template <typename T>
+static size_t rows_smem(int d, int stages) {
+  if constexpr (sizeof(T) == 2) return rows16_bf16_smem(d, stages);
   else return rows16_f32_smem(d);
 }
 
-template <typename T, int DMAX>
+template <typename T, int DMAX, bool EXACT>
 static int launch_shared_rows(const SharedParams& p, cudaStream_t s) {
-  const size_t smem = rows_smem<T, DMAX>(p.D);
-  auto kern = shared_rows_kernel<T, DMAX>;
+  const size_t smem = rows_smem<T>(p.D, p.stages);
+  auto kern = shared_rows_kernel<T, DMAX, EXACT>;
   if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return 2;
   FTK_LAUNCH(kern, dim3(p.n_items, p.Hkv * p.chunks), kRowThreads, smem, s, p);
   return 0;
 }
-template <typename T, int DMAX>
+template <typename T, int DMAX, bool EXACT>
 static int launch_own_keys(const SharedParams& p, cudaStream_t s) {
-  const size_t smem = rows_smem<T, DMAX>(p.D);
-  auto kern = own_keys_kernel<T, DMAX>;
+  const size_t smem = rows_smem<T>(p.D, p.stages);
+  auto kern = own_keys_kernel<T, DMAX, EXACT>;
   if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return 2;
   const dim3 grid((unsigned)(p.n_requests * p.Hkv * p.chunks * p.cluster));
   if (p.cluster > 1) launch_kernel_clusters(kern, p.cluster, grid, dim3(kRowThreads), smem, s, p);
   else FTK_LAUNCH(kern, grid, kRowThreads, smem, s, p);
   return 0;
+}
+
+template <typename T>
+static int launch_rows(const SharedParams& p, cudaStream_t s) {
+  return p.D == 64 ? launch_shared_rows<T, 64, true>(p, s) : p.D == 128 ? launch_shared_rows<T, 128, true>(p, s)
+         : p.D < 128 ? launch_shared_rows<T, 128, false>(p, s) : launch_shared_rows<T, 256, false>(p, s);
+}
+template <typename T>
+static int launch_own(const SharedParams& p, cudaStream_t s) {
+  return p.D == 64 ? launch_own_keys<T, 64, true>(p, s) : p.D == 128 ? launch_own_keys<T, 128, true>(p, s)
+         : p.D < 128 ? launch_own_keys<T, 128, false>(p, s) : launch_own_keys<T, 256, false>(p, s);
 }
 
 }  // namespace ftk
@@ -617,6 +692,10 @@ extern "C" int ftk_shared_attention(const FtkShared* a, void* stream) {
   p.chunks = (p.G + p.Gc - 1) / p.Gc;
   p.cluster = a->cluster;
   p.scale = a->scale; p.has_sink = a->has_sink; p.sink = a->sink; p.sink_heads = a->sink_heads;
+  p.stages = kTileStages;
+  p.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (p.P == 1 << i) p.page_shift = i;
   p.early = a->n_items > 0;
   FTK_REQUIRE((long long)p.Hkv * p.chunks <= 65535 && (long long)p.n_requests * p.Hkv * p.chunks * p.cluster <= 0x7fffffffLL, "shared_attention: %d requests of %d KV heads",
               p.n_requests, p.Hkv);
@@ -631,18 +710,13 @@ extern "C" int ftk_shared_attention(const FtkShared* a, void* stream) {
     FTK_REQUIRE(!tc || ((uintptr_t)a->part_o & 31) == 0, "shared_attention: partial results on 32-byte boundaries only");
     note_variant(tc ? "shared attention: tcgen05, 256 rows" : a->dtype == FTK_F32 ? "shared attention: float32, 16 rows" : "shared attention: bfloat16 mma.sync, 16 rows");
     if (tc) rc = D == 64 ? launch_shared_tc<64>(p, s) : launch_shared_tc<128>(p, s);
-    else if (a->dtype == FTK_F32)
-      rc = D <= 64 ? launch_shared_rows<float, 64>(p, s) : D <= 128 ? launch_shared_rows<float, 128>(p, s) : launch_shared_rows<float, 256>(p, s);
-    else
-      rc = D <= 64 ? launch_shared_rows<__nv_bfloat16, 64>(p, s) : D <= 128 ? launch_shared_rows<__nv_bfloat16, 128>(p, s) : launch_shared_rows<__nv_bfloat16, 256>(p, s);
+    else rc = a->dtype == FTK_F32 ? launch_rows<float>(p, s) : launch_rows<__nv_bfloat16>(p, s);
     FTK_REQUIRE(rc == 0, "shared_attention: cannot set up the kernel for shared keys (%d)", rc);
     FTK_LAUNCH_CHECK("shared_attention");
   }
+  if (a->own_tiles < kTileStages) p.stages = a->own_tiles > 1 ? a->own_tiles : 1;
   note_variant(a->dtype == FTK_F32 ? "shared attention: float32, own keys" : "shared attention: bfloat16 mma.sync, own keys");
-  if (a->dtype == FTK_F32)
-    rc = D <= 64 ? launch_own_keys<float, 64>(p, s) : D <= 128 ? launch_own_keys<float, 128>(p, s) : launch_own_keys<float, 256>(p, s);
-  else
-    rc = D <= 64 ? launch_own_keys<__nv_bfloat16, 64>(p, s) : D <= 128 ? launch_own_keys<__nv_bfloat16, 128>(p, s) : launch_own_keys<__nv_bfloat16, 256>(p, s);
+  rc = a->dtype == FTK_F32 ? launch_own<float>(p, s) : launch_own<__nv_bfloat16>(p, s);
   FTK_REQUIRE(rc == 0, "shared_attention: cannot set up the kernel for own keys (%d)", rc);
   FTK_LAUNCH_CHECK("shared_attention (own keys)");
   return 0;

@@ -9,7 +9,10 @@
 //                 running maximum moves only when it grew by more than 8 (a factor of 256: l and o stay far from the ends of 32 bits), so
 //                 that the accumulator is rescaled a few times a row;
 //   O += P V      P from tensor memory, V from shared memory as it lies in the pages.
-// The issuing warp takes the tiles in turn, so the tensor pipe works on one while the other's softmax runs.  One CTA an SM works through
+// The issuing warp takes the tiles in turn, so the tensor pipe works on one while the other's softmax runs.  A piece with members for
+// one query tile only may be *split*: both tiles then hold the same rows, tile A works through the even key tiles and B through the
+// odd ones, and each leaves partial results of its own (the chain scores - softmax - product of one tile keeps neither pipe busy).
+// One CTA an SM works through
 // its share of the list, to and fro (the list is sorted by length); loads, products and softmax run through it on their own.  A
 // piece's queries are gathered as soon as the scores of the piece before are done, under its last product.
 //
@@ -26,6 +29,45 @@ constexpr int kShHalf = 128 * 64 * 2;                           // bytes of a [1
 constexpr int kShRegsFew = 72, kShRegsMany = 216;               // of 384 x 168: what 128 threads give, 256 take
 constexpr int kShStages(int d) { return d == 128 ? 2 : 4; }     // key and value tiles in flight
 constexpr int kShSmem(int d) { return (2 + 2 * kShStages(d)) * (d / 64) * kShHalf + 1024; }
+
+// Exponentials: the special-function unit gives 16 an SM and cycle, 2,048 cycles for the 32,768 of a key tile and two query tiles, as much
+// as the products take.  Of every eight columns kShPoly pairs go another way: 2^x = 2^n 2^r with n = x rounded to the nearest integer (by adding and
+// taking off 1.5 2^23) and 2^r on [-1/2, 1/2] by a polynomial of degree four, the minimax fit of the relative error by Lawson's
+// iteration (2.7e-6 evaluated in 32 bits; the probability is rounded to 2^-9 right behind), two numbers an instruction.
+constexpr int kShPoly = 1;
+__device__ __forceinline__ uint64_t sh_pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void sh_unpair(uint64_t p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ uint64_t sh_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float sh_max3(float a, float b, float c) {  // (NaN if one of them is)
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 2^x of two numbers, x at most 100 or so; below -126 as for -126
+__device__ __forceinline__ void sh_exp2_poly(uint64_t x, float& e0, float& e1) {
+  float x0, x1, t0, t1;
+  sh_unpair(x, x0, x1);
+  x = sh_pair(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+  const uint64_t magic = sh_pair(12582912.f, 12582912.f), back = sh_pair(-12582912.f, -12582912.f), minus = sh_pair(-1.f, -1.f);
+  const uint64_t t = f2_add(x, magic), r = sh_fma2(f2_add(t, back), minus, x);
+  uint64_t p = sh_pair(9.570101276e-03f, 9.570101276e-03f);
+  p = sh_fma2(p, r, sh_pair(5.591785908e-02f, 5.591785908e-02f));
+  p = sh_fma2(p, r, sh_pair(2.402474433e-01f, 2.402474433e-01f));
+  p = sh_fma2(p, r, sh_pair(6.931217909e-01f, 6.931217909e-01f));
+  p = sh_fma2(p, r, sh_pair(9.999992847e-01f, 9.999992847e-01f));
+  sh_unpair(t, t0, t1);
+  sh_unpair(p, e0, e1);
+  e0 = __int_as_float(__float_as_int(e0) + (__float_as_int(t0) << 23));
+  e1 = __int_as_float(__float_as_int(e1) + (__float_as_int(t1) << 23));
+}
 
 template <int N> __device__ __forceinline__ void sh_regs_give() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void sh_regs_take() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -107,7 +149,8 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   auto tiles_of = [](const Piece& it) { return it.ok ? (it.ke - it.kb + kShKeys - 1) / kShKeys : 0; };
   auto piece_of = [&](int w) {
     Piece it = load_piece(p, w / p.Hkv);
-    it.ok = it.ok && it.n_mem <= 2 * tpt && it.kb % 16 == 0;
+    it.ok = it.ok && it.n_mem <= 2 * tpt && it.kb % 16 == 0 &&
+            (!it.split || (it.n_mem <= tpt && it.ke - it.kb > kShKeys && 2 * it.n_mem <= p.n_slots - it.slot0));
     return it;
   };
   auto fail = [&](int code) {
@@ -178,12 +221,14 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         const Piece it = piece_of(w);
         const int n_tiles = tiles_of(it);
         if (n_tiles == 0) continue;
+        const bool split = it.split;
         const int n_q = it.n_mem > tpt ? 2 : 1;
         bool fine = true;  // this lane's waits; the warp votes on them once a key tile
-        auto scores = [&](int x, int j) {
+        // S_x = Q_x K(j)^T, the jj-th product of this kind of query tile x in this piece
+        auto scores = [&](int x, int j, int jj) {
           const int g = g0 + j, ks = g % kStages;
-          if (x == 0 && !mbar_wait(&k_full[ks], (uint32_t)(g / kStages) & 1u, abortp)) { fail(803); fine = false; }
-          if (j == 0 && !mbar_wait(&q_full[x], (uint32_t)(px[x] & 1), abortp)) { fail(804); fine = false; }
+          if ((split || x == 0) && !mbar_wait(&k_full[ks], (uint32_t)(g / kStages) & 1u, abortp)) { fail(803); fine = false; }
+          if (jj == 0 && !mbar_wait(&q_full[x], (uint32_t)(px[x] & 1), abortp)) { fail(804); fine = false; }
           __syncwarp();
           tc_fence_after();
           if (elect_one()) if (fine) {
@@ -195,14 +240,14 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
               tc_mma(d, a, b, idesc_qk, kk != 0);
             }
             tc_commit(&s_full[x]);
-            if (x == n_q - 1) tc_commit(&k_empty[ks]);
+            if (split || x == n_q - 1) tc_commit(&k_empty[ks]);
           }
           __syncwarp();
         };
-        auto product = [&](int x, int j) {
+        auto product = [&](int x, int j, int jj) {
           const int g = g0 + j, vs = g % kStages;
-          if (!mbar_wait(&p_full[x], (uint32_t)((gx[x] + j) & 1), abortp)) { fail(805); fine = false; }
-          if (x == 0) {
+          if (!mbar_wait(&p_full[x], (uint32_t)((gx[x] + jj) & 1), abortp)) { fail(805); fine = false; }
+          if (split || x == 0) {
             if (!mbar_wait(&v_full[vs], (uint32_t)(g / kStages) & 1u, abortp)) { fail(805); fine = false; }
             const int live = it.ke - (it.kb + j * kShKeys);  // keys of the piece in this tile
             if (live < kShKeys) {  // behind them: zeros, whatever the page or the stage holds there
@@ -213,7 +258,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
               fence_async_smem();
             }
           }
-          if (j == 0 && !mbar_wait(&o_free[x], (uint32_t)(px[x] & 1) ^ 1u, abortp)) { fail(806); fine = false; }
+          if (jj == 0 && !mbar_wait(&o_free[x], (uint32_t)(px[x] & 1) ^ 1u, abortp)) { fail(806); fine = false; }
           __syncwarp();
           tc_fence_after();
           if (elect_one()) if (fine) {
@@ -222,24 +267,34 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             for (int kk = 0; kk < 8; ++kk) {  // 16 keys per product
               const uint32_t a = tmem + (uint32_t)(x * kShKeys + kk * 8);
               const uint64_t b = smem_desc_mn(v_s + vs * kTile + kk * 2048, kShHalf);
-              tc_mma_ts(d, a, b, idesc_pv, (j | kk) != 0);
+              tc_mma_ts(d, a, b, idesc_pv, (jj | kk) != 0);
             }
             tc_commit(&pv_done[x]);
-            if (x == n_q - 1) tc_commit(&v_empty[vs]);
+            if (split || x == n_q - 1) tc_commit(&v_empty[vs]);
           }
           __syncwarp();
         };
-        for (int x = 0; x < n_q; ++x) scores(x, 0);
-        for (int j = 0; j < n_tiles && ok; ++j) {
-          for (int x = 0; x < n_q; ++x) {
-            product(x, j);
-            if (j + 1 < n_tiles) scores(x, j + 1);
+        if (split) {
+          scores(0, 0, 0);
+          scores(1, 1, 0);
+          for (int j = 0; j < n_tiles && ok; ++j) {
+            product(j & 1, j, j >> 1);
+            if (j + 2 < n_tiles) scores(j & 1, j + 2, (j >> 1) + 1);
+            ok = all_of_warp(fine);
           }
-          ok = all_of_warp(fine);
+        } else {
+          for (int x = 0; x < n_q; ++x) scores(x, 0, 0);
+          for (int j = 0; j < n_tiles && ok; ++j) {
+            for (int x = 0; x < n_q; ++x) {
+              product(x, j, j);
+              if (j + 1 < n_tiles) scores(x, j + 1, j + 1);
+            }
+            ok = all_of_warp(fine);
+          }
         }
         g0 += n_tiles;
-        for (int x = 0; x < n_q; ++x) {
-          gx[x] += n_tiles;
+        for (int x = 0; x < (split ? 2 : n_q); ++x) {
+          gx[x] += split ? (n_tiles + 1 - x) >> 1 : n_tiles;
           ++px[x];
         }
       }
@@ -258,9 +313,9 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         const int w = work_of(i);
         if (w >= n_work) continue;
         const Piece it = piece_of(w);
-        if (!it.ok || it.n_mem <= X * tpt) continue;
-        const int R = min(tpt, it.n_mem - X * tpt) * G, head0 = w % p.Hkv * G;
-        const int32_t* mem = p.members + it.mem0 + X * tpt;
+        if (!it.ok || (!it.split && it.n_mem <= X * tpt)) continue;
+        const int mem0 = it.split ? 0 : X * tpt, R = min(tpt, it.n_mem - mem0) * G, head0 = w % p.Hkv * G;
+        const int32_t* mem = p.members + it.mem0 + mem0;
         constexpr int kPer = 8 * kHalves;  // 16-byte words of a row
 #pragma unroll
         for (int u = 0; u < 32; u += 32 / kPer) {
@@ -284,8 +339,8 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     for (int i = load_queries(0); i < n_rounds && ok;) {
       const int w = work_of(i);
       const Piece it = piece_of(w);
-      const int kvh = w % p.Hkv, n_tiles = tiles_of(it);
-      const int R = min(tpt, it.n_mem - X * tpt) * G;
+      const int kvh = w % p.Hkv, mem0 = it.split ? 0 : X * tpt, R = min(tpt, it.n_mem - mem0) * G;
+      const int n_tiles = it.split ? (tiles_of(it) + 1 - X) >> 1 : tiles_of(it);  // this query tile's
       float m_used = -INFINITY, l = 0.f;
       for (int j = 0; j < n_tiles && ok; ++j) {
         const int g = gx + j;
@@ -301,7 +356,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         sh_ld32(s_addr + 64, v + 64);
         sh_ld32(s_addr + 96, v + 96);
         sh_ld_wait(v);
-        const int live = it.ke - (it.kb + j * kShKeys);
+        const int live = it.ke - (it.kb + (it.split ? 2 * j + X : j) * kShKeys);
         if (live < kShKeys) {
 #pragma unroll
           for (int n = 0; n < 128; ++n)
@@ -309,13 +364,10 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         }
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int n = 0; n < 128; n += 4) {
-          mx4[0] = fmaxf(mx4[0], v[n]);
-          mx4[1] = fmaxf(mx4[1], v[n + 1]);
-          mx4[2] = fmaxf(mx4[2], v[n + 2]);
-          mx4[3] = fmaxf(mx4[3], v[n + 3]);
-        }
-        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;  // (the scale is positive)
+        for (int n = 0; n < 128; n += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx4[e] = sh_max3(mx4[e], v[n + 2 * e], v[n + 2 * e + 1]);
+        const float mx = sh_max3(sh_max3(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]) * sl2;  // (the scale is positive)
         float alpha = 1.f;
         if (mx > m_used + 8.f || (m_used == -INFINITY && mx > -INFINITY)) {
           alpha = m_used == -INFINITY ? 0.f : exp2_fast(m_used - mx);
@@ -341,19 +393,31 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           }
         }
         const float mb = m_used == -INFINITY ? 0.f : m_used;
-        float sum = 0.f;
+        const uint64_t sl22 = sh_pair(sl2, sl2), mb2 = sh_pair(-mb, -mb);
+        uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t pk[16];
 #pragma unroll
           for (int n = 0; n < 32; n += 2) {
-            const float p0 = exp2_fast(fmaf(v[c * 32 + n], sl2, -mb));  // (0 for keys that are not there)
-            const float p1 = exp2_fast(fmaf(v[c * 32 + n + 1], sl2, -mb));
-            sum += p0 + p1;
-            pk[n >> 1] = two_bf16(p0, p1);
+            const uint64_t x = sh_fma2(sh_pair(v[c * 32 + n], v[c * 32 + n + 1]), sl22, mb2);
+            float e0, e1;
+            if ((n >> 1 & 3) >= 4 - kShPoly) {
+              sh_exp2_poly(x, e0, e1);
+            } else {
+              sh_unpair(x, e0, e1);
+              e0 = exp2_fast(e0);  // (0 for keys that are not there)
+              e1 = exp2_fast(e1);
+            }
+            sum2[n >> 1 & 1] = f2_add(sum2[n >> 1 & 1], sh_pair(e0, e1));
+            pk[n >> 1] = two_bf16(e0, e1);
           }
           sh_st16(s_addr + (uint32_t)(c * 16), pk);
         }
+        float sum, sum_odd;
+        sh_unpair(f2_add(sum2[0], sum2[1]), sum, sum_odd);
+        sum += sum_odd;
+        if (!(mx < INFINITY)) sum = NAN;  // a score that is NaN or infinite: so is every output of the row
         l += sum;
         sh_st_wait();
         tc_fence_before();
@@ -370,7 +434,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         tc_fence_after();
       }
       if (ok) {
-        const size_t at = (size_t)(it.slot0 + X * tpt + r / G) * p.Hq + kvh * G + r % G;
+        const size_t at = (size_t)(it.slot0 + (it.split ? X * it.n_mem : mem0) + r / G) * p.Hq + kvh * G + r % G;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           float o[32];
@@ -381,7 +445,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             for (int n = 0; n < 32; n += 8) sh_store8(p.part_o + at * D + c * 32 + n, o + n);
           }
         }
-        if (r < R) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m_used, l);
+        if (r < R) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(l != l && m_used == -INFINITY ? 0.f : m_used, l);  // (NaN is not a row without keys)
       }
       tc_fence_before();
       __syncwarp();

@@ -22,7 +22,7 @@ import torch
 
 from ..errors import KernelError
 
-ITEM_INTS = 8     # first member, members, block-table row, first key, one past the last key, first slot, 0, 0
+ITEM_INTS = 8     # first member, members, block-table row, first key, one past the last key, first slot, split, 0
 REQUEST_INTS = 8  # query row, block-table row, first own key, one past the last, first join, joins, 0, 0
 ROWS_TILE = 16    # query rows of a piece on the kernels for few rows
 WIDE_TILE = 256   # on the tcgen05 kernel: two tiles of 128
@@ -48,6 +48,7 @@ class SharedPlan:
     n_slots: int
     tile_rows: int
     cluster: int
+    own_tiles: int        # tiles of keys that one CTA of a cluster has at most
     n_rows: int           # rows of q that the plan reads, from the first on
     n_heads: int
     n_kv_heads: int
@@ -55,7 +56,7 @@ class SharedPlan:
 
     def key(self) -> Tuple[int, ...]:
         """What a recorded step's launches depend on."""
-        return (self.items.shape[0], self.members.shape[0], self.requests.shape[0], self.joins.shape[0], self.n_slots, self.tile_rows, self.cluster)
+        return (self.items.shape[0], self.members.shape[0], self.requests.shape[0], self.joins.shape[0], self.n_slots, self.tile_rows, self.cluster, self.own_tiles)
 
     def sections(self) -> List[Tuple[str, np.ndarray]]:
         return [("items", self.items), ("members", self.members), ("requests", self.requests), ("joins", self.joins)]
@@ -199,10 +200,12 @@ def build_shared_plan(kv_lens: Sequence[int], spans: Sequence[Span], n_heads: in
         member_rows += members
         for a, k in tile_members(u, length):
             cost = k * (WIDE_TWO_US if 2 * len(members) > most else WIDE_ONE_US) if wide else float(k)
-            items.append((-cost, first, len(members), rows[members[0]], start + a * unit, min(end, start + (a + k) * unit), n_slots, 0, 0))
-            for i, m in enumerate(members):
-                slots[m].append((start + a * unit, n_slots + i))
-            n_slots += len(members)
+            split = wide and 2 * len(members) <= most and k > 1  # one query tile: both halves of the kernel, half of the key tiles each
+            items.append((-cost, first, len(members), rows[members[0]], start + a * unit, min(end, start + (a + k) * unit), n_slots, int(split), 0))
+            for half in range(2 if split else 1):
+                for i, m in enumerate(members):
+                    slots[m].append((start + (a + half) * unit, n_slots + half * len(members) + i))
+            n_slots += (2 if split else 1) * len(members)
     items = [it[1:] for it in sorted(items, key=lambda it: it[0])]  # the longest first
 
     # what is a request's own: one range behind its spans
@@ -217,7 +220,8 @@ def build_shared_plan(kv_lens: Sequence[int], spans: Sequence[Span], n_heads: in
         requests.append((i, rows[i], begin, int(kv_lens[i]), len(joins), len(own), 0, 0))
         joins += own
         longest = max(longest, int(kv_lens[i]) - begin)
-    cluster = own_cluster(1 << (longest - 1).bit_length(), max(1, n * n_kv_heads * chunks), ROWS_KEYS[dtype], sm_count)
+    longest = 1 << (longest - 1).bit_length()
+    cluster = own_cluster(longest, max(1, n * n_kv_heads * chunks), ROWS_KEYS[dtype], sm_count)
     as_int = lambda x, w: np.asarray(x, dtype=np.int32).reshape(-1, w) if w else np.asarray(x, dtype=np.int32)  # noqa: E731
     return SharedPlan(as_int(items, ITEM_INTS), as_int(member_rows, 0), as_int(requests, REQUEST_INTS), as_int(joins, 0), n_slots,
-                      WIDE_TILE if wide else ROWS_TILE, cluster, n, n_heads, n_kv_heads, head_dim)
+                      WIDE_TILE if wide else ROWS_TILE, cluster, -(-longest // (cluster * ROWS_KEYS[dtype])), n, n_heads, n_kv_heads, head_dim)

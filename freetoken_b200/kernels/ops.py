@@ -94,7 +94,7 @@ class _Shared(ctypes.Structure):
     _fields_ = [(n, _vp) for n in ("q", "k", "v", "out", "block_table", "items", "members", "requests", "joins", "part_o", "part_ml",
                                    "sink_heads")] + [(n, _i) for n in (
         "dtype", "bt_stride", "bt_rows", "n_items", "n_members", "n_requests", "n_joins", "n_slots", "n_rows", "n_q_heads", "n_kv_heads",
-        "head_dim", "page_size", "num_pages", "tile_rows", "cluster")] + [("scale", _f), ("has_sink", _i), ("sink", _f)]
+        "head_dim", "page_size", "num_pages", "tile_rows", "cluster", "own_tiles")] + [("scale", _f), ("has_sink", _i), ("sink", _f)]
 
 
 class _CopyTensor(ctypes.Structure):
@@ -752,7 +752,7 @@ def shared_attention(q: torch.Tensor, k_slab: torch.Tensor, v_slab: torch.Tensor
                 _here(plan.joins, "joins", i32), _here(plan.part_o, "part_o", torch.float32) if n_slots else None,
                 _here(plan.part_ml, "part_ml", torch.float32) if n_slots else None, sink_heads, _code(q, "q"), block_table.shape[1],
                 block_table.shape[0], host.items.shape[0], host.members.shape[0], host.requests.shape[0], host.joins.shape[0], n_slots, T, Hq,
-                Hkv, D, P, pages, host.tile_rows, host.cluster, float(scale), 0 if sink is None else 1, 0.0 if sink is None else float(sink))
+                Hkv, D, P, pages, host.tile_rows, host.cluster, host.own_tiles, float(scale), 0 if sink is None else 1, 0.0 if sink is None else float(sink))
     _check(_lib().ftk_shared_attention(ctypes.byref(a), _stream()), "shared_attention", 2 if host.items.shape[0] else 1)
 
 

@@ -203,6 +203,28 @@ def test_infinities_and_nan_stay_with_their_request():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("dtype,tile_rows", [(F32, 16), (BF16, 16), (BF16, 256)])
+def test_nan_and_infinite_scores_reach_who_reads_them(dtype, tile_rows, value):
+    """Every place of a key tile in turn: as a shared key, and as the only key that a request has of its own."""
+    lens, spans = [257, 258, 300], [([0, 1], 0, 256)]
+    q, k, v, table = case(lens, spans, 16, 2, 128, 16, dtype)
+    q[:, :, 0] = q[:, :, 0].abs() + 0.1  # (an infinite key gives +infinity to every query)
+    scale = 128 ** -0.5
+    plan = build_shared_plan(lens, spans, 16, 2, 128, dtype, 16, tile_rows=tile_rows).to(DEV)
+    clean = run(q, k, v, table, plan, scale)
+    assert torch.isfinite(clean).all()
+    for pos in list(range(0, 256, 37)) + list(range(128, 160)):
+        bad = k.clone()
+        bad[table[0, pos // 16].long(), 1, pos % 16, 0] = value
+        got = run(q, bad, v, table, plan, scale)
+        assert torch.isnan(got[:2, 8:]).all() and torch.equal(got[:2, :8], clean[:2, :8]) and torch.equal(got[2], clean[2]), pos
+    k[table[0, 16].long(), 1, 0, 0] = value
+    got = run(q, k, v, table, plan, scale)
+    assert torch.isnan(got[0, 8:]).all() and torch.equal(got[0, :8], clean[0, :8]) and torch.equal(got[1:], clean[1:])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_captured_replayed_and_on_another_stream(dtype):
     lens, spans = [300, 257, 256, 290], [([0, 1, 2, 3], 0, 256)]

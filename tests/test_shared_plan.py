@@ -12,13 +12,14 @@ from freetoken_b200.errors import KernelError
 def covered(plan, n, rows):
     """Per request: the key ranges of its pieces in the order in which they are joined, then its own."""
     of_slot = {}
-    for mem0, k, row, kb, ke, slot0, *_ in plan.items.tolist():
+    for mem0, k, row, kb, ke, slot0, split, _ in plan.items.tolist():
         assert kb < ke and 0 <= mem0 and mem0 + k <= len(plan.members)
         members = plan.members[mem0:mem0 + k].tolist()
         assert row == rows[members[0]]
-        for i, m in enumerate(members):
+        assert not split or (plan.tile_rows == 256 and ke - kb > 128)
+        for i, m in enumerate(members * (2 if split else 1)):  # (a split piece: even and odd key tiles, the second without a range of its own)
             assert slot0 + i not in of_slot and slot0 + i < plan.n_slots
-            of_slot[slot0 + i] = (m, kb, ke)
+            of_slot[slot0 + i] = (m, kb, ke) if i < k else (m, ke, ke)
     assert sorted(of_slot) == list(range(plan.n_slots))
     out = []
     for i, (q, row, lo, hi, j0, k, *_) in enumerate(plan.requests.tolist()):
