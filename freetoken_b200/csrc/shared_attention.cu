@@ -74,13 +74,13 @@ __device__ __forceinline__ Piece load_piece(const SharedParams& p, int idx) {
   return it;
 }
 
-// Element offset of key `pos` of block-table row `bt_row` in a [pages, KV heads, P, D] slab, or -1 where the table names no page of it.
-__device__ __forceinline__ long long key_offset(const SharedParams& p, int bt_row, int kvh, int pos) {
+// Row of key `pos` of block-table row `bt_row` among a slab's [pages, KV heads, P] rows of D, or -1 where the table names no page of it.
+__device__ __forceinline__ int key_row(const SharedParams& p, int bt_row, int kvh, int pos) {
   const int block = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.P;
   if (block >= p.bt_stride) return -1;
   const int page = p.block_table[(size_t)bt_row * p.bt_stride + block];
   if (page < 0 || page >= p.num_pages) return -1;
-  return (((long long)page * p.Hkv + kvh) * p.P + (pos - block * p.P)) * p.D;
+  return (page * p.Hkv + kvh) * p.P + (pos - block * p.P);
 }
 
 __device__ __forceinline__ uint32_t sh_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -136,27 +136,27 @@ __device__ __forceinline__ RowsResult rows16_bf16(const SharedParams& p, const R
   __nv_bfloat16* sq = reinterpret_cast<__nv_bfloat16*>(smem);
   __nv_bfloat16* sk0 = sq + kRows * ld;
   __nv_bfloat16* sv0 = sk0 + p.stages * kTileKeys * ld;
-  __shared__ long long row_off[4][kTileKeys];  // where the keys of tile t lie: row_off[t & 3]
+  __shared__ int key_rows[4][kTileKeys];  // where the keys of tile t lie: key_rows[t & 3]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pieces = D >> 3;
   const __nv_bfloat16* q = (const __nv_bfloat16*)p.q;
   const __nv_bfloat16* kbase = (const __nv_bfloat16*)p.k;
   const __nv_bfloat16* vbase = (const __nv_bfloat16*)p.v;
 
-  auto look_up = [&](int t) -> long long {
+  auto look_up = [&](int t) -> int {
     const int pos = kb + t * kTileKeys + (int)threadIdx.x;
-    return threadIdx.x < kTileKeys && pos < ke ? key_offset(p, bt_row, kvh, pos) : -1;
+    return threadIdx.x < kTileKeys && pos < ke ? key_row(p, bt_row, kvh, pos) : -1;
   };
-  auto publish = [&](int t, long long off) {
-    if (threadIdx.x < kTileKeys) row_off[t & 3][threadIdx.x] = off;
+  auto publish = [&](int t, int row) {
+    if (threadIdx.x < kTileKeys) key_rows[t & 3][threadIdx.x] = row;
   };
   auto load = [&](int t) {
     __nv_bfloat16* sk = sk0 + t % kTileStages * kTileKeys * ld;
     __nv_bfloat16* sv = sv0 + t % kTileStages * kTileKeys * ld;
     for (int i = threadIdx.x; i < kTileKeys * pieces; i += kRowThreads) {
       const int j = i / pieces, c = i - j * pieces;
-      const long long off = row_off[t & 3][j];
-      const bool there = off >= 0;
-      const long long o = there ? off + c * 8 : 0;
+      const int row = key_rows[t & 3][j];
+      const bool there = row >= 0;
+      const size_t o = (size_t)(there ? row : 0) * D + c * 8;
       copy16(sk + j * ld + c * 8, kbase + o, there);
       copy16(sv + j * ld + c * 8, vbase + o, there);
     }
@@ -187,7 +187,7 @@ __device__ __forceinline__ RowsResult rows16_bf16(const SharedParams& p, const R
     __syncthreads();  // tile t has landed for everyone, and everyone is done with tile t - 1
     if (t + 2 < n_tiles) load(t + 2);
     copy_commit();
-    const long long next = look_up(t + 3);
+    const int next = look_up(t + 3);
     if (kb + t * kTileKeys + warp * 16 >= ke) {  // (none of this warp's keys is there)
       publish(t + 3, next);
       continue;
@@ -211,7 +211,7 @@ __device__ __forceinline__ RowsResult rows16_bf16(const SharedParams& p, const R
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const bool there = row_off[t & 3][j0 + n * 8 + e] >= 0;
+        const bool there = key_rows[t & 3][j0 + n * 8 + e] >= 0;
         s[n][e] = there ? s[n][e] * sl2 : -INFINITY;
         s[n][2 + e] = there ? s[n][2 + e] * sl2 : -INFINITY;
         mx0 = fmaxf(mx0, s[n][e]);
@@ -324,26 +324,26 @@ __device__ __forceinline__ RowsResult rows16_f32(const SharedParams& p, const Ro
   float* sq = rl + kRows;             // [16][D] queries, in the end the outputs
   float* sk0 = sq + kRows * D;        // two tiles of keys, two of values
   float* sv0 = sk0 + 2 * kF32Keys * ld;
-  __shared__ long long row_off[4][kF32Keys];
+  __shared__ int key_rows[4][kF32Keys];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pieces = D >> 2;
   const float* q = (const float*)p.q;
   const float* kbase = (const float*)p.k;
   const float* vbase = (const float*)p.v;
-  auto look_up = [&](int t) -> long long {
+  auto look_up = [&](int t) -> int {
     const int pos = kb + t * kF32Keys + (int)threadIdx.x;
-    return threadIdx.x < kF32Keys && pos < ke ? key_offset(p, bt_row, kvh, pos) : -1;
+    return threadIdx.x < kF32Keys && pos < ke ? key_row(p, bt_row, kvh, pos) : -1;
   };
-  auto publish = [&](int t, long long off) {
-    if (threadIdx.x < kF32Keys) row_off[t & 3][threadIdx.x] = off;
+  auto publish = [&](int t, int row) {
+    if (threadIdx.x < kF32Keys) key_rows[t & 3][threadIdx.x] = row;
   };
   auto load = [&](int t) {
     float* sk = sk0 + (t & 1) * kF32Keys * ld;
     float* sv = sv0 + (t & 1) * kF32Keys * ld;
     for (int i = threadIdx.x; i < kF32Keys * pieces; i += kRowThreads) {
       const int j = i / pieces, c = i - j * pieces;
-      const long long off = row_off[t & 3][j];
-      const bool there = off >= 0;
-      const long long o = there ? off + c * 4 : 0;
+      const int row = key_rows[t & 3][j];
+      const bool there = row >= 0;
+      const size_t o = (size_t)(there ? row : 0) * D + c * 4;
       copy16(sk + j * ld + c * 4, kbase + o, there);
       copy16(sv + j * ld + c * 4, vbase + o, there);
     }
@@ -369,7 +369,7 @@ __device__ __forceinline__ RowsResult rows16_f32(const SharedParams& p, const Ro
   }
   const bool any = warp * RW < rw.n;
   for (int t = 0; t < n_tiles; ++t) {
-    const long long next = look_up(t + 2);
+    const int next = look_up(t + 2);
     if (t + 1 < n_tiles) load(t + 1);
     copy_commit();
     copy_wait<1>();
@@ -377,7 +377,7 @@ __device__ __forceinline__ RowsResult rows16_f32(const SharedParams& p, const Ro
     const float* sk = sk0 + (t & 1) * kF32Keys * ld;
     const float* sv = sv0 + (t & 1) * kF32Keys * ld;
     if (any) {
-      const bool there = row_off[t & 3][lane] >= 0;
+      const bool there = key_rows[t & 3][lane] >= 0;
       float dot[RW] = {};
 #pragma unroll 4
       for (int d = 0; d < D; d += 4) {
@@ -504,17 +504,17 @@ __device__ __forceinline__ void store4(T* to, float4 v) {
   else *reinterpret_cast<uint2*>(to) = make_uint2(two_bf16(v.x, v.y), two_bf16(v.z, v.w));
 }
 
-constexpr int kJoinRun = 32;  // shared pieces whose maxima and sums are fetched together
+constexpr int kJoinRun = 32;  // partial results that are weighed together, one a lane
 
 template <typename T, int DMAX, bool EXACT>
-__global__ void __launch_bounds__(kRowThreads) own_keys_kernel(const __grid_constant__ SharedParams p) {
+__global__ void __launch_bounds__(kRowThreads, DMAX <= 128 ? 4 : 2) own_keys_kernel(const __grid_constant__ SharedParams p) {
   // With shared pieces in front of it this kernel starts while they run: queries, keys and values were written in front of them,
   // and only their partial results are waited for.
   if (!p.early) pdl_wait();
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ int slots[kJoinRun];
-  __shared__ float2 ml[kJoinRun][kRows];
-  const int C = p.cluster, rank = blockIdx.x % C, tid = threadIdx.x;
+  __shared__ float weights[kJoinRun][kRows], before[kRows], norm[kRows];  // of a run's partial results; of what was summed up in front of it
+  const int C = p.cluster, rank = blockIdx.x % C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int work = blockIdx.x / C;
   const int chunk = work % p.chunks;
   work /= p.chunks;
@@ -524,95 +524,114 @@ __global__ void __launch_bounds__(kRowThreads) own_keys_kernel(const __grid_cons
   const int heads = min(p.Gc, p.G - chunk * p.Gc), head0 = kvh * p.G + chunk * p.Gc;
   const bool ok = tok >= 0 && tok < p.n_rows && bt_row >= 0 && bt_row < p.bt_rows && from >= 0 && join0 >= 0 && w[5] >= 0 && w[5] <= p.n_joins - join0;
   const int n_join = ok ? w[5] : 0;
-  if (tid < kJoinRun) slots[tid] = tid < n_join ? p.joins[join0 + tid] : -1;
   // this CTA's share of the keys, in whole tiles
   const int tile = sizeof(T) == 2 ? kTileKeys : kF32Keys;
   const int own = ok ? max(0, to - from) : 0, share = ((own + C - 1) / C + tile - 1) / tile * tile;
   const int kb = from + min(own, rank * share), ke = from + min(own, rank * share + share);
   const Rows rw{nullptr, tok, heads, head0, ok ? heads : 0};
   const RowsResult res = rows16<T, DMAX, EXACT>(p, rw, bt_row, kvh, kb, ke, smem);
-  if (p.early) pdl_wait();
-  pdl_trigger();
-  // A row's 32-bit results are spread over the cluster's threads, four columns each; its shared pieces come first, in their order.
-  const int D = EXACT ? DMAX : p.D;
-  constexpr int kQuads = DMAX * kRows / 4 / kRowThreads;
-  const int quads = D >> 2, at0 = rank * kRowThreads + tid;
-  float M[kQuads], L[kQuads];
-  float4 acc[kQuads];
-#pragma unroll
-  for (int u = 0; u < kQuads; ++u) {
-    M[u] = -INFINITY;
-    L[u] = 0.f;
-    acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-  }
-  auto scale = [&](int u, float m) {  // a new maximum
-    const float f = weight<T>(M[u], m);
-    L[u] *= f;
-    acc[u].x *= f; acc[u].y *= f; acc[u].z *= f; acc[u].w *= f;
-    M[u] = m;
-  };
-  auto add = [&](int u, float m, float l, float4 o) {
-    const float f = weight<T>(m, M[u]);
-    if (f != 0.f) {  // (a piece of weight 0 may hold anything)
-      L[u] += l * f;
-      acc[u].x += o.x * f; acc[u].y += o.y * f; acc[u].z += o.z * f; acc[u].w += o.w * f;
-    }
-  };
-  for (int j0 = 0; j0 < n_join; j0 += kJoinRun) {
-    const int n = min(kJoinRun, n_join - j0);
-    if (j0 > 0) {
-      __syncthreads();
-      if (tid < kJoinRun) slots[tid] = tid < n ? p.joins[join0 + j0 + tid] : -1;
-      __syncthreads();
-    }
-    for (int i = tid; i < n * kRows; i += kRowThreads) {
-      const int j = i / kRows, r = i % kRows, slot = slots[j];
-      if (r < heads)
-        ml[j][r] = slot >= 0 && slot < p.n_slots ? *reinterpret_cast<const float2*>(p.part_ml + ((size_t)slot * p.Hq + head0 + r) * 2) : make_float2(-INFINITY, 0.f);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < kQuads; ++u) {
-      const int i = at0 + u * C * kRowThreads;
-      if (i >= rw.n * quads) break;
-      const int r = i / quads, d = i % quads * 4;
-      const float* o = p.part_o + (size_t)(head0 + r) * D + d;
-      float m = M[u];
-      for (int j = 0; j < n; ++j) m = fmaxf(m, ml[j][r].x);
-      scale(u, m);
-      for (int j = 0; j < n; j += 8) {  // eight loads on their way before the first use
-        float4 x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int slot = j + e < n ? slots[j + e] : -1;
-          x[e] = slot >= 0 && slot < p.n_slots ? __ldcg(reinterpret_cast<const float4*>(o + (size_t)slot * p.Hq * D)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (j + e < n) add(u, ml[j + e][r].x, ml[j + e][r].y, x[e]);
-      }
-    }
-  }
   if (C > 1) cluster_barrier();
   const uint32_t my_m = sh_addr(res.m), my_l = sh_addr(res.l), my_o = sh_addr(res.o);  // (at the same place in every CTA)
+  if (p.early) pdl_wait();
+  pdl_trigger();
+  // All partial results of the request: the shared pieces' in their order, then the cluster's.  A run of 32 at a time a warp weighs a row's,
+  // a lane each; then every thread sums up four columns of a row (the rows' 32-bit results are spread over the cluster).
+  const int D = EXACT ? DMAX : p.D;
+  constexpr int kQuads = DMAX * kRows / 4 / kRowThreads;
+  const int quads = D >> 2, at0 = rank * kRowThreads + tid, parts = rw.n ? n_join + C : 0;
+  float4 acc[kQuads];
+#pragma unroll
+  for (int u = 0; u < kQuads; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float M[kRows / 4], L[kRows / 4];  // of rows warp, warp + 4, ...
+#pragma unroll
+  for (int e = 0; e < kRows / 4; ++e) {
+    M[e] = -INFINITY;
+    L[e] = 0.f;
+  }
+  for (int j0 = 0; j0 < parts; j0 += kJoinRun) {
+    const int n = min(kJoinRun, parts - j0), n_slots = max(0, min(n, n_join - j0)), part = j0 + lane;
+    int slot = part < n_join ? p.joins[join0 + part] : -1;
+    if (slot >= p.n_slots) slot = -1;
+    if (warp == 0) slots[lane] = slot;
+#pragma unroll
+    for (int e = 0; e < kRows / 4; ++e) {
+      const int r = warp + 4 * e;
+      if (r >= heads) break;
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (slot >= 0) ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + ((size_t)slot * p.Hq + head0 + r) * 2));
+      else if (part >= n_join && lane < n)
+        ml = C > 1 ? make_float2(cluster_f32(of_rank(my_m + r * 4, part - n_join)), cluster_f32(of_rank(my_l + r * 4, part - n_join))) : make_float2(res.m[r], res.l[r]);
+      const float m = fmaxf(M[e], warp_max(ml.x)), f = weight<T>(M[e], m), wgt = weight<T>(ml.x, m);
+      L[e] = L[e] * f + warp_sum(wgt != 0.f ? ml.y * wgt : 0.f);
+      M[e] = m;
+      weights[lane][r] = wgt;
+      if (lane == 0) {
+        before[r] = f;
+        if (j0 + kJoinRun >= parts) {  // the last run; a sink is a key without a value, and a row of nothing else gives zeros
+          float sum = L[e];
+          if (p.has_sink && m != -INFINITY) sum += expf((p.sink_heads ? __ldg(p.sink_heads + head0 + r) : p.sink) - (sizeof(T) == 2 ? m / kLog2e : m));
+          norm[r] = sum == 0.f ? 0.f : 1.f / sum;  // (NaN stays)
+        }
+      }
+    }
+    __syncthreads();
+    // a batch of pieces for all of the thread's columns: every load is on its way before the first use
+    constexpr int kBatch = kQuads > 4 ? 2 : kQuads > 2 ? 4 : 8;
+    if (j0 > 0) {
+#pragma unroll
+      for (int u = 0; u < kQuads; ++u) {
+        const int i = at0 + u * C * kRowThreads;
+        if (i >= rw.n * quads) break;
+        const float f = before[i / quads];
+        acc[u].x *= f; acc[u].y *= f; acc[u].z *= f; acc[u].w *= f;
+      }
+    }
+    auto add = [&](int u, float f, float4 x) {
+      if (f != 0.f) {  // (a part of weight 0 may hold anything)
+        acc[u].x = fmaf(x.x, f, acc[u].x); acc[u].y = fmaf(x.y, f, acc[u].y);
+        acc[u].z = fmaf(x.z, f, acc[u].z); acc[u].w = fmaf(x.w, f, acc[u].w);
+      }
+    };
+#pragma unroll 1
+    for (int j = 0; j < n_slots; j += kBatch) {
+      float4 x[kQuads][kBatch];
+#pragma unroll
+      for (int u = 0; u < kQuads; ++u) {
+        const int i = at0 + u * C * kRowThreads;
+        if (i >= rw.n * quads) break;
+        const float* o = p.part_o + (size_t)(head0 + i / quads) * D + i % quads * 4;
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {
+          const int at = slots[(j + e) % kJoinRun];
+          if (j + e < n_slots && at >= 0) x[u][e] = __ldcg(reinterpret_cast<const float4*>(o + (size_t)at * p.Hq * D));
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kQuads; ++u) {
+        const int i = at0 + u * C * kRowThreads;
+        if (i >= rw.n * quads) break;
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e)
+          if (j + e < n_slots) add(u, weights[(j + e) % kJoinRun][i / quads], x[u][e]);
+      }
+    }
+#pragma unroll 1
+    for (int j = n_slots; j < n; ++j) {  // the cluster's
+#pragma unroll
+      for (int u = 0; u < kQuads; ++u) {
+        const int i = at0 + u * C * kRowThreads;
+        if (i >= rw.n * quads) break;
+        add(u, weights[j][i / quads], C > 1 ? cluster_f32x4(of_rank(my_o + i * 16, j0 + j - n_join)) : *reinterpret_cast<const float4*>(res.o + i * 4));
+      }
+    }
+    __syncthreads();
+  }
 #pragma unroll
   for (int u = 0; u < kQuads; ++u) {
     const int i = at0 + u * C * kRowThreads;
     if (i >= rw.n * quads) break;
-    const int r = i / quads, d = i % quads * 4, head = head0 + r;
-    float m = M[u];
-    for (int c = 0; c < C; ++c) m = fmaxf(m, C > 1 ? cluster_f32(of_rank(my_m + r * 4, c)) : res.m[r]);
-    scale(u, m);
-    for (int c = 0; c < C; ++c) {
-      if (C > 1)
-        add(u, cluster_f32(of_rank(my_m + r * 4, c)), cluster_f32(of_rank(my_l + r * 4, c)), cluster_f32x4(of_rank(my_o + (r * D + d) * 4, c)));
-      else
-        add(u, res.m[r], res.l[r], *reinterpret_cast<const float4*>(res.o + r * D + d));
-    }
-    // a sink is a key without a value; a row of nothing else gives zeros
-    if (p.has_sink && m != -INFINITY) L[u] += expf((p.sink_heads ? __ldg(p.sink_heads + head) : p.sink) - (sizeof(T) == 2 ? m / kLog2e : m));
-    const float inv = L[u] == 0.f ? 0.f : 1.f / L[u];  // (NaN stays)
-    store4((T*)p.out + ((size_t)tok * p.Hq + head) * D + d, make_float4(acc[u].x * inv, acc[u].y * inv, acc[u].z * inv, acc[u].w * inv));
+    const float f = norm[i / quads];
+    store4((T*)p.out + ((size_t)tok * p.Hq + head0) * D + i * 4, make_float4(acc[u].x * f, acc[u].y * f, acc[u].z * f, acc[u].w * f));
   }
   if (C > 1) cluster_barrier();  // nobody leaves while its shared memory is read
 }
@@ -699,13 +718,14 @@ extern "C" int ftk_shared_attention(const FtkShared* a, void* stream) {
   p.early = a->n_items > 0;
   FTK_REQUIRE((long long)p.Hkv * p.chunks <= 65535 && (long long)p.n_requests * p.Hkv * p.chunks * p.cluster <= 0x7fffffffLL, "shared_attention: %d requests of %d KV heads",
               p.n_requests, p.Hkv);
+  FTK_REQUIRE((long long)p.num_pages * p.Hkv * p.P <= 0x7fffffffLL, "shared_attention: a slab of 2^31 rows or more");
   cudaStream_t s = (cudaStream_t)stream;
   const int D = p.D;
   int rc = 0;
   if (p.n_items > 0) {
     const bool tc = a->tile_rows == 2 * kShRows;
     FTK_REQUIRE(tc || a->tile_rows == kRows, "shared_attention: pieces of %d query rows are not taken", a->tile_rows);
-    FTK_REQUIRE(!tc || (a->dtype == FTK_BF16 && shared_tc_fits(D, p.P, p.G) && p.scale > 0.f && (long long)p.num_pages * p.Hkv * p.P <= 0x7fffffffLL),
+    FTK_REQUIRE(!tc || (a->dtype == FTK_BF16 && shared_tc_fits(D, p.P, p.G) && p.scale > 0.f),
                 "shared_attention: pieces of 256 rows take bfloat16 heads of 64 or 128, pages of a multiple of 16, at most 128 heads per KV head and a positive scale");
     FTK_REQUIRE(!tc || ((uintptr_t)a->part_o & 31) == 0, "shared_attention: partial results on 32-byte boundaries only");
     note_variant(tc ? "shared attention: tcgen05, 256 rows" : a->dtype == FTK_F32 ? "shared attention: float32, 16 rows" : "shared attention: bfloat16 mma.sync, 16 rows");

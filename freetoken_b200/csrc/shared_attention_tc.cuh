@@ -14,7 +14,7 @@
 // odd ones, and each leaves partial results of its own (the chain scores - softmax - product of one tile keeps neither pipe busy).
 // One CTA an SM works through
 // its share of the list, to and fro (the list is sorted by length); loads, products and softmax run through it on their own.  A
-// piece's queries are gathered as soon as the scores of the piece before are done, under its last product.
+// piece's queries are fetched as soon as the scores of the piece before are done, under its last product.
 //
 // Every wait is bounded: a timeout records a code in g_shared_status, lets copies land, frees tensor memory and returns.
 #pragma once
@@ -27,8 +27,9 @@ __device__ int g_shared_status[4];  // [0] first error code, [1] block; 0 = fine
 constexpr int kShRows = 128, kShKeys = 128, kShThreads = 384;   // a warpgroup of 2 loaders + 1 issuer (+ 1 idle), 2 x 4 softmax warps
 constexpr int kShHalf = 128 * 64 * 2;                           // bytes of a [128 rows x 64 elements] column of 128-byte rows
 constexpr int kShRegsFew = 72, kShRegsMany = 216;               // of 384 x 168: what 128 threads give, 256 take
-constexpr int kShStages(int d) { return d == 128 ? 2 : 4; }     // key and value tiles in flight
-constexpr int kShSmem(int d) { return (2 + 2 * kShStages(d)) * (d / 64) * kShHalf + 1024; }
+constexpr int kShKStages(int d) { return d == 128 ? 3 : 5; }    // key and value tiles in flight: what fits beside the queries
+constexpr int kShVStages(int d) { return d == 128 ? 2 : 5; }
+constexpr int kShSmem(int d) { return (2 + kShKStages(d) + kShVStages(d)) * (d / 64) * kShHalf + 1024; }
 
 // Exponentials: the special-function unit gives 16 an SM and cycle, 2,048 cycles for the 32,768 of a key tile and two query tiles, as much
 // as the products take.  Of every eight columns kShPoly pairs go another way: 2^x = 2^n 2^r with n = x rounded to the nearest integer (by adding and
@@ -69,6 +70,10 @@ __device__ __forceinline__ void sh_exp2_poly(uint64_t x, float& e0, float& e1) {
   e1 = __int_as_float(__float_as_int(e1) + (__float_as_int(t1) << 23));
 }
 
+template <int N>
+struct IntC {
+  static constexpr int value = N;
+};
 template <int N> __device__ __forceinline__ void sh_regs_give() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void sh_regs_take() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
@@ -110,10 +115,10 @@ __device__ __forceinline__ void sh_store8(float* to, const float* v) {
 template <int D>
 __global__ void __launch_bounds__(kShThreads, 1)
 shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ SharedParams p) {
-  constexpr int kHalves = D / 64, kTile = kHalves * kShHalf, kStages = kShStages(D);
+  constexpr int kHalves = D / 64, kTile = kHalves * kShHalf, kKStages = kShKStages(D), kVStages = kShVStages(D);
   constexpr uint32_t kLoaders = 8 * kHalves, kLoaderMask = (1u << kLoaders) - 1u;  // lanes of a loading warp: one per box
   extern __shared__ unsigned char dyn_smem[];
-  __shared__ uint64_t q_full[2], o_free[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], p_full[2], pv_done[2];
+  __shared__ uint64_t q_full[2], o_free[2], k_full[kKStages], k_empty[kKStages], v_full[kVStages], v_empty[kVStages], s_full[2], p_full[2], pv_done[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
 
@@ -123,11 +128,13 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   auto work_of = [&](int i) { return i * (int)gridDim.x + ((i & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x); };
   const uint32_t base = (smem_addr(dyn_smem) + 1023u) & ~1023u;
   unsigned char* tiles = dyn_smem + (base - smem_addr(dyn_smem));
-  const uint32_t q_s = base, k_s = base + 2 * kTile, v_s = base + (2 + kStages) * kTile;
+  const uint32_t q_s = base, k_s = base + 2 * kTile, v_s = base + (2 + kKStages) * kTile;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < kKStages; ++s) {
       mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1);
+    }
+    for (int s = 0; s < kVStages; ++s) {
       mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1);
     }
     for (int x = 0; x < 2; ++x) {
@@ -141,8 +148,8 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  pdl_wait();
-  pdl_trigger();
+  if (warp < 4) pdl_wait();  // (the softmax warps have something to do in front of it)
+  if (warp == 1) pdl_trigger();  // (behind the wait: the kernel after this one counts on the one before being over)
   const uint32_t tmem = tmem_slot;
   volatile int* abortp = &abort_flag;
   const int G = p.G, tpt = kShRows / G;  // members of one query tile
@@ -167,7 +174,8 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         const CUtensorMap* map = kv ? &map_v : &map_k;
         uint64_t* full = kv ? v_full : k_full;
         uint64_t* empty = kv ? v_empty : k_empty;
-        unsigned char* stage0 = tiles + (kv ? 2 + kStages : 2) * kTile + h * kShHalf + box * 2048;
+        unsigned char* stage0 = tiles + (kv ? 2 + kKStages : 2) * kTile + h * kShHalf + box * 2048;
+        const int stages = kv ? kVStages : kKStages;
         bool ok = true;
         int g = 0;  // key tiles of all pieces so far
         for (int i = 0; i < n_rounds && ok; ++i) {
@@ -190,13 +198,13 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           };
           int page_next = page_of(0);
           for (int j = 0; j < n_tiles && ok; ++j, ++g) {
-            const int st = g % kStages;
+            const int st = g % stages;
             const int key0 = it.kb + j * kShKeys;
             const int n_box = min(8, (it.ke - key0 + 15) >> 4);  // boxes that hold keys of the piece
             const int page = page_next;
             page_next = page_of(j + 1);
             const int row = (page * p.Hkv + kvh) * p.P + (key0 + 16 * box) % p.P;
-            if (!__all_sync(kLoaderMask, mbar_wait(&empty[st], (uint32_t)((g / kStages) & 1) ^ 1u, abortp))) {
+            if (!__all_sync(kLoaderMask, mbar_wait(&empty[st], (uint32_t)((g / stages) & 1) ^ 1u, abortp))) {
               if (lane == 0) fail(801 + kv);
               ok = false;
               break;
@@ -209,93 +217,119 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       }
     } else if (warp == 1) {
       // ---------------------------------------------------------- issuer; the warp zeroes value rows past the piece's end
+      // What a piece is comes through a shuffle: the compiler then knows that stages, parities and descriptors are the warp's, and
+      // products leave one after the other.  (An issuing warp for each tile lets both tiles' softmax run at the same time and then wait for
+      // the tensor pipe together: 2.05 us a key tile and pair against 1.70 where the keys are there.)
       constexpr uint32_t idesc_qk = instr_desc(kShKeys);
       constexpr uint32_t idesc_pv = instr_desc(D) | kMnMajorB;
+      const uint64_t q_desc = smem_desc(q_s), k_desc = smem_desc(k_s), v_desc = smem_desc_mn(v_s, kShHalf);  // (addresses add to them, in 16-byte words)
       bool ok = true;
-      int g0 = 0;          // key tiles of the pieces before this one
-      int gx[2] = {0, 0};  // key tiles that query tile x has worked through, pieces it took part in
-      int px[2] = {0, 0};
+      int g0 = 0;           // key tiles of the pieces before this one
+      int gx0 = 0, gx1 = 0;  // key tiles that query tile A, B has worked through, pieces it took part in
+      int px0 = 0, px1 = 0;
       for (int i = 0; i < n_rounds && ok; ++i) {
         const int w = work_of(i);
         if (w >= n_work) continue;
         const Piece it = piece_of(w);
-        const int n_tiles = tiles_of(it);
+        const int n_tiles = __shfl_sync(0xffffffffu, tiles_of(it), 0), n_keys = __shfl_sync(0xffffffffu, it.ke - it.kb, 0);
+        const bool split = __shfl_sync(0xffffffffu, (int)it.split, 0) != 0, two = __shfl_sync(0xffffffffu, it.n_mem, 0) > tpt;
         if (n_tiles == 0) continue;
-        const bool split = it.split;
-        const int n_q = it.n_mem > tpt ? 2 : 1;
         bool fine = true;  // this lane's waits; the warp votes on them once a key tile
-        // S_x = Q_x K(j)^T, the jj-th product of this kind of query tile x in this piece
-        auto scores = [&](int x, int j, int jj) {
-          const int g = g0 + j, ks = g % kStages;
-          if ((split || x == 0) && !mbar_wait(&k_full[ks], (uint32_t)(g / kStages) & 1u, abortp)) { fail(803); fine = false; }
-          if (jj == 0 && !mbar_wait(&q_full[x], (uint32_t)(px[x] & 1), abortp)) { fail(804); fine = false; }
+        auto wait = [&](uint64_t* bar, int parity, int code) {
+          if (!mbar_wait(bar, (uint32_t)(parity & 1), abortp)) { fail(code); fine = false; }
+        };
+        auto keys_there = [&](int j) { wait(&k_full[(g0 + j) % kKStages], (g0 + j) / kKStages, 803); };
+        // the values of tile j are there; rows behind the piece's end are zeros then, whatever the page or the stage holds in them
+        auto values_there = [&](int j) {
+          const int vs = (g0 + j) % kVStages, live = n_keys - j * kShKeys;
+          wait(&v_full[vs], (g0 + j) / kVStages, 805);
+          if (live < kShKeys) {
+            for (int z = lane; z < (kShKeys - live) * 8 * kHalves; z += 32) {
+              const int r = live + z / (8 * kHalves), h = (z / 8) % kHalves, c = z & 7;
+              *reinterpret_cast<uint4*>(tiles + (2 + kKStages + vs) * kTile + h * kShHalf + r * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_async_smem();
+          }
+        };
+        // S_x = Q_x K(j)^T; `last`: no other query tile needs these keys
+        auto scores = [&](auto xc, int j, bool last) {
+          constexpr int x = decltype(xc)::value;
+          const int ks = (g0 + j) % kKStages;
           __syncwarp();
           tc_fence_after();
           if (elect_one()) if (fine) {
-            const uint32_t d = tmem + (uint32_t)(x * kShKeys);
+            const uint64_t a = q_desc + x * (kTile >> 4), b = k_desc + ks * (kTile >> 4);
 #pragma unroll
-            for (int kk = 0; kk < 4 * kHalves; ++kk) {  // 16 elements of the head dimension per product
-              const uint64_t a = smem_desc(q_s + x * kTile + (kk >> 2) * kShHalf) + 2 * (kk & 3);
-              const uint64_t b = smem_desc(k_s + ks * kTile + (kk >> 2) * kShHalf) + 2 * (kk & 3);
-              tc_mma(d, a, b, idesc_qk, kk != 0);
-            }
+            for (int kk = 0; kk < 4 * kHalves; ++kk)  // 16 elements of the head dimension per product
+              tc_mma(tmem + (uint32_t)(x * kShKeys), a + (kk >> 2) * (kShHalf >> 4) + 2 * (kk & 3), b + (kk >> 2) * (kShHalf >> 4) + 2 * (kk & 3),
+                     idesc_qk, kk != 0);
             tc_commit(&s_full[x]);
-            if (split || x == n_q - 1) tc_commit(&k_empty[ks]);
+            if (last) tc_commit(&k_empty[ks]);
           }
           __syncwarp();
         };
-        auto product = [&](int x, int j, int jj) {
-          const int g = g0 + j, vs = g % kStages;
-          if (!mbar_wait(&p_full[x], (uint32_t)((gx[x] + jj) & 1), abortp)) { fail(805); fine = false; }
-          if (split || x == 0) {
-            if (!mbar_wait(&v_full[vs], (uint32_t)(g / kStages) & 1u, abortp)) { fail(805); fine = false; }
-            const int live = it.ke - (it.kb + j * kShKeys);  // keys of the piece in this tile
-            if (live < kShKeys) {  // behind them: zeros, whatever the page or the stage holds there
-              for (int z = lane; z < (kShKeys - live) * 8 * kHalves; z += 32) {
-                const int r = live + z / (8 * kHalves), h = (z / 8) % kHalves, c = z & 7;
-                *reinterpret_cast<uint4*>(tiles + (2 + kStages + vs) * kTile + h * kShHalf + r * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
-              }
-              fence_async_smem();
-            }
-          }
-          if (jj == 0 && !mbar_wait(&o_free[x], (uint32_t)(px[x] & 1) ^ 1u, abortp)) { fail(806); fine = false; }
+        // O_x += P_x V(j), the jj-th of this query tile in this piece
+        auto product = [&](auto xc, int j, int jj, bool last) {
+          constexpr int x = decltype(xc)::value;
+          const int vs = (g0 + j) % kVStages;
+          wait(&p_full[x], (x ? gx1 : gx0) + jj, 805);
+          if (jj == 0) wait(&o_free[x], (x ? px1 : px0) + 1, 806);
           __syncwarp();
           tc_fence_after();
           if (elect_one()) if (fine) {
-            const uint32_t d = tmem + (uint32_t)((2 + x) * kShKeys);
+            const uint64_t b = v_desc + vs * (kTile >> 4);
 #pragma unroll
-            for (int kk = 0; kk < 8; ++kk) {  // 16 keys per product
-              const uint32_t a = tmem + (uint32_t)(x * kShKeys + kk * 8);
-              const uint64_t b = smem_desc_mn(v_s + vs * kTile + kk * 2048, kShHalf);
-              tc_mma_ts(d, a, b, idesc_pv, (jj | kk) != 0);
-            }
+            for (int kk = 0; kk < 8; ++kk)  // 16 keys per product
+              tc_mma_ts(tmem + (uint32_t)((2 + x) * kShKeys), tmem + (uint32_t)(x * kShKeys + kk * 8), b + kk * (2048 >> 4), idesc_pv, (jj | kk) != 0);
             tc_commit(&pv_done[x]);
-            if (split || x == n_q - 1) tc_commit(&v_empty[vs]);
+            if (last) tc_commit(&v_empty[vs]);
           }
           __syncwarp();
         };
+        const IntC<0> A;
+        const IntC<1> B;
+        keys_there(0);
+        wait(&q_full[0], px0, 804);
+        scores(A, 0, split || !two);
+        if (split) keys_there(1);
+        if (split || two) {
+          wait(&q_full[1], px1, 804);
+          scores(B, split ? 1 : 0, true);
+        }
         if (split) {
-          scores(0, 0, 0);
-          scores(1, 1, 0);
-          for (int j = 0; j < n_tiles && ok; ++j) {
-            product(j & 1, j, j >> 1);
-            if (j + 2 < n_tiles) scores(j & 1, j + 2, (j >> 1) + 1);
+          for (int j = 0; j < n_tiles && ok; j += 2) {
+            values_there(j);
+            if (j + 2 < n_tiles) keys_there(j + 2);
+            product(A, j, j >> 1, true);
+            if (j + 2 < n_tiles) scores(A, j + 2, true);
+            if (j + 1 < n_tiles) {
+              values_there(j + 1);
+              if (j + 3 < n_tiles) keys_there(j + 3);
+              product(B, j + 1, j >> 1, true);
+              if (j + 3 < n_tiles) scores(B, j + 3, true);
+            }
             ok = all_of_warp(fine);
           }
         } else {
-          for (int x = 0; x < n_q; ++x) scores(x, 0, 0);
           for (int j = 0; j < n_tiles && ok; ++j) {
-            for (int x = 0; x < n_q; ++x) {
-              product(x, j, j);
-              if (j + 1 < n_tiles) scores(x, j + 1, j + 1);
+            const bool more = j + 1 < n_tiles;
+            values_there(j);  // (what is waited for under the softmax anyway goes in front of the probabilities)
+            if (more) keys_there(j + 1);
+            product(A, j, j, !two);
+            if (more) scores(A, j + 1, !two);
+            if (two) {
+              product(B, j, j, true);
+              if (more) scores(B, j + 1, true);
             }
             ok = all_of_warp(fine);
           }
         }
         g0 += n_tiles;
-        for (int x = 0; x < (split ? 2 : n_q); ++x) {
-          gx[x] += split ? (n_tiles + 1 - x) >> 1 : n_tiles;
-          ++px[x];
+        gx0 += split ? (n_tiles + 1) >> 1 : n_tiles;
+        ++px0;
+        if (split || two) {
+          gx1 += split ? n_tiles >> 1 : n_tiles;
+          ++px1;
         }
       }
     }
@@ -307,44 +341,54 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
     const uint32_t s_addr = lane_addr + (uint32_t)(X * kShKeys);        // scores, then probabilities over their first half
     const uint32_t o_addr = lane_addr + (uint32_t)((2 + X) * kShKeys);
-    // this warp's 32 rows of the queries of the first piece from round `i` on that has some for this tile; returns that round
-    auto load_queries = [&](int i) {
+    // This warp's 32 rows of the queries of the first piece from round `i` on that has some for this tile, on their way to shared memory;
+    // returns that round.  (A lane looks its own row's place up, all copies leave together: looked up copy by copy they took 17,000 cycles.)
+    auto fetch_queries = [&](int i) {
       for (; i < n_rounds; ++i) {
         const int w = work_of(i);
         if (w >= n_work) continue;
         const Piece it = piece_of(w);
         if (!it.ok || (!it.split && it.n_mem <= X * tpt)) continue;
-        const int mem0 = it.split ? 0 : X * tpt, R = min(tpt, it.n_mem - mem0) * G, head0 = w % p.Hkv * G;
-        const int32_t* mem = p.members + it.mem0 + mem0;
+        const int mem0 = it.split ? 0 : X * tpt, R = min(tpt, it.n_mem - mem0) * G;
+        const int tok = r < R ? p.members[it.mem0 + mem0 + r / G] : -1;
+        const int row = tok >= 0 && tok < p.n_rows ? tok * p.Hq + w % p.Hkv * G + r % G : -1;  // of the queries' rows; -1: zeros
         constexpr int kPer = 8 * kHalves;  // 16-byte words of a row
-#pragma unroll
+        const int c = lane % kPer;
+        unsigned char* to = tiles + X * kTile + (c >> 3) * kShHalf;
+#pragma unroll 4
         for (int u = 0; u < 32; u += 32 / kPer) {
-          const int rr = quad * 32 + u + lane / kPer, c = lane % kPer;
-          if (rr < R) {
-            const int tok = mem[rr / G];
-            uint4 x = make_uint4(0u, 0u, 0u, 0u);
-            if (tok >= 0 && tok < p.n_rows) x = *(reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.q + ((size_t)tok * p.Hq + head0 + rr % G) * D) + c);
-            *reinterpret_cast<uint4*>(tiles + X * kTile + (c >> 3) * kShHalf + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = x;
-          }
+          const int mine = u + lane / kPer, rr = quad * 32 + mine, from = __shfl_sync(0xffffffffu, row, mine);
+          if (rr < R)
+            copy16(to + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), (const __nv_bfloat16*)p.q + (size_t)max(from, 0) * D + c * 8, from >= 0);
         }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&q_full[X]);
+        copy_commit();
         break;
       }
       return i;
     };
+    auto queries_there = [&](int i) {
+      if (i >= n_rounds) return;
+      copy_wait<0>();
+      fence_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[X]);
+    };
     bool ok = true;
     int gx = 0;  // key tiles this query tile has worked through
-    for (int i = load_queries(0); i < n_rounds && ok;) {
-      const int w = work_of(i);
-      const Piece it = piece_of(w);
+    // The first round is dry: a key tile's arithmetic on whatever tensor memory holds, which brings its instructions to the SM (7,000
+    // cycles where they come from L2) while the kernel before this one ends and the first keys are on their way.
+    bool dry = true;
+    for (int i = -1; i < n_rounds && ok;) {
+      const int w = dry ? 0 : work_of(i);
+      Piece it = {};
+      if (!dry) it = piece_of(w);
       const int kvh = w % p.Hkv, mem0 = it.split ? 0 : X * tpt, R = min(tpt, it.n_mem - mem0) * G;
-      const int n_tiles = it.split ? (tiles_of(it) + 1 - X) >> 1 : tiles_of(it);  // this query tile's
+      const int n_tiles = dry ? 1 : it.split ? (tiles_of(it) + 1 - X) >> 1 : tiles_of(it);  // this query tile's
       float m_used = -INFINITY, l = 0.f;
       for (int j = 0; j < n_tiles && ok; ++j) {
         const int g = gx + j;
-        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[X], (uint32_t)(g & 1), abortp))) {
+        if (!dry && !__all_sync(0xffffffffu, mbar_wait(&s_full[X], (uint32_t)(g & 1), abortp))) {
           if (lane == 0) fail(807);
           ok = false;
           break;
@@ -422,10 +466,17 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         sh_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[X]);
+        if (lane == 0 && !dry) mbar_arrive(&p_full[X]);
       }
+      if (dry) pdl_wait();
       // the scores of the piece's last tile are done, so its queries have been read: the next piece's take their place
-      const int next = ok ? load_queries(i + 1) : n_rounds;
+      const int next = ok ? fetch_queries(i + 1) : n_rounds;
+      if (dry) {
+        queries_there(next);
+        dry = false;
+        i = next;
+        continue;
+      }
       if (ok) {
         if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[X], (uint32_t)((gx + n_tiles - 1) & 1), abortp))) {
           if (lane == 0) fail(808);
@@ -450,6 +501,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&o_free[X]);  // the next piece's first product may overwrite the output
+      if (ok) queries_there(next);
       gx += n_tiles;
       i = next;
     }
