@@ -440,23 +440,26 @@ def cast(src: torch.Tensor, dst: torch.Tensor) -> None:
 def _here(t: torch.Tensor, what: str, dtype: Optional[torch.dtype] = None) -> int:
     """:func:`_dev` of a tensor on the current device, where the kernel will run."""
     ptr = _dev(t, what, dtype)
-    if t.device.index != torch.cuda.current_device():
-        raise KernelError(f"{what}: tensor is on '{t.device}', the current device is 'cuda:{torch.cuda.current_device()}'")
+    if t.device.index != torch._C._cuda_getDevice():
+        raise KernelError(f"{what}: tensor is on '{t.device}', the current device is 'cuda:{torch._C._cuda_getDevice()}'")
     return ptr
 
 
-def _copy_blocks(what: str, tensors: Sequence[torch.Tensor], pairs: torch.Tensor, ints: int, shapes) -> None:
-    if pairs.dim() != 2 or pairs.shape[1] != ints or pairs.dtype != torch.int32:
+def _copy_blocks(what: str, tensors: Sequence[torch.Tensor], pairs: torch.Tensor, ints: int) -> None:
+    if pairs.dtype != torch.int32 or pairs.dim() != 2 or pairs.shape[1] != ints:
         raise KernelError(f"{what}: pairs must be int32 [n, {ints}], got {pairs.dtype} {tuple(pairs.shape)}")
-    if not tensors or not pairs.shape[0]:
+    n = pairs.shape[0]
+    if not tensors or not n:
         return
     arr = (_CopyTensor * len(tensors))()
-    for c, t, (parts, rows) in zip(arr, tensors, shapes):
+    for c, t in zip(arr, tensors):
+        shape, size = t.shape, t.element_size()
         c.base = _here(t, what)
-        c.entries, c.blocks, c.parts, c.rows = t.shape[0], t.shape[1], parts, rows
-        c.row_bytes = t.element_size() * (t.numel() // max(1, t.shape[0] * t.shape[1] * parts * rows))
-    _check(_lib().ftk_copy_blocks(arr, len(tensors), _here(pairs, "pairs", torch.int32), ints, pairs.shape[0], _stream()), what,
-           -(-len(tensors) // 16))
+        if ints == 3:
+            c.entries, c.blocks, c.parts, c.rows, c.row_bytes = shape[0], shape[1], shape[2], shape[3], shape[4] * size
+        else:
+            c.entries, c.blocks, c.parts, c.rows, c.row_bytes = shape[0], shape[1], 1, 1, t.numel() // (shape[0] * shape[1]) * size
+    _check(_lib().ftk_copy_blocks(arr, len(tensors), _here(pairs, "pairs"), ints, n, _stream()), what, -(-len(tensors) // 16))
 
 
 def copy_pages(slabs: Sequence[torch.Tensor], pairs: torch.Tensor) -> None:
@@ -466,12 +469,15 @@ def copy_pages(slabs: Sequence[torch.Tensor], pairs: torch.Tensor) -> None:
     ``pairs`` int32 ``[n, 3]`` on the device.  ``rows`` from the page size on is the whole page; rows behind them stay as they are.  A
     page may be the source of many pairs, but the target of one at most, and no target may be a source: copies are not in order.  A
     pair that names a page outside the slab, has no rows, or names the same page twice does nothing."""
+    like = None
     for t in slabs:
-        if t.dim() != 5 or t.shape[1] != slabs[0].shape[1] or t.shape[3] != slabs[0].shape[3]:
+        shape = t.shape
+        if len(shape) != 5 or (like is not None and (shape[1] != like[1] or shape[3] != like[3])):
             raise KernelError("copy_pages: slabs must be [entries, pages, heads, page_size, dim] with the same pages")
         if not t.numel():
             raise KernelError("copy_pages: an empty slab")
-    _copy_blocks("copy_pages", slabs, pairs, 3, [t.shape[2:4] for t in slabs])
+        like = like or shape
+    _copy_blocks("copy_pages", slabs, pairs, 3)
 
 
 def copy_slots(tensors: Sequence[torch.Tensor], pairs: torch.Tensor) -> None:
@@ -483,7 +489,7 @@ def copy_slots(tensors: Sequence[torch.Tensor], pairs: torch.Tensor) -> None:
             raise KernelError("copy_slots: tensors must be [entries, slots, ...] with the same slots")
         if not t.numel():
             raise KernelError("copy_slots: an empty tensor")
-    _copy_blocks("copy_slots", tensors, pairs, 2, [(1, 1)] * len(tensors))
+    _copy_blocks("copy_slots", tensors, pairs, 2)
 
 
 # --------------------------------------------------------------------------- attention
@@ -725,35 +731,58 @@ def shared_attention(q: torch.Tensor, k_slab: torch.Tensor, v_slab: torch.Tensor
     ``sink``: a logit, a float32 tensor ``[Hq]`` of one per query head, or None, as in :func:`paged_attention`.
 
     The plan's scratch belongs to one launch at a time: calls that may run at once need plans of their own."""
+    fixed = plan.fixed
+    if fixed is None:
+        fixed = plan.fixed = _shared_fixed(plan)
     host = plan.host
-    if q.dim() != 3 or k_slab.dim() != 4:
+    shape, slab = q.shape, k_slab.shape
+    if len(shape) != 3 or len(slab) != 4:
         raise KernelError("shared_attention: q must be [T, Hq, D], slabs [pages, Hkv, page_size, D]")
-    T, Hq, D = q.shape
-    pages, Hkv, P, D2 = k_slab.shape
-    if D2 != D or v_slab.shape != k_slab.shape or (Hq, Hkv, D) != (host.n_heads, host.n_kv_heads, host.head_dim):
+    T, Hq, D = shape
+    if slab[3] != D or v_slab.shape != slab or (Hq, slab[1], D) != (host.n_heads, host.n_kv_heads, host.head_dim):
         raise KernelError("shared_attention: q, slabs and plan do not agree")
-    if out.shape != q.shape or out.dtype != q.dtype or k_slab.dtype != q.dtype or v_slab.dtype != q.dtype:
+    dtype = q.dtype
+    if out.shape != shape or out.dtype != dtype or k_slab.dtype != dtype or v_slab.dtype != dtype:
         raise KernelError("shared_attention: dtypes or out shape do not agree")
     if block_table.dim() != 2 or T < host.n_rows:
         raise KernelError(f"shared_attention: {T} query rows and a block table of {block_table.dim()} dimensions for a plan of {host.n_rows} requests")
     if not host.n_rows:
         return
+    a = _Shared.from_buffer_copy(fixed)
+    if sink is not None:
+        a.has_sink = 1
+        if isinstance(sink, torch.Tensor):
+            if sink.shape != (Hq,):
+                raise KernelError("shared_attention: a sink per head must be [Hq]")
+            a.sink_heads = _here(sink, "sink", torch.float32)
+        else:
+            a.sink = float(sink)
+    a.q, a.k, a.v, a.out = _here(q, "q"), _here(k_slab, "k_slab"), _here(v_slab, "v_slab"), _here(out, "out")
+    a.block_table = _here(block_table, "block_table", torch.int32)
+    a.dtype, a.bt_rows, a.bt_stride = _code(q, "q"), block_table.shape[0], block_table.shape[1]
+    a.n_rows, a.page_size, a.num_pages, a.scale = T, slab[2], slab[0], scale
+    _check(_lib().ftk_shared_attention(ctypes.byref(a), _stream()), "shared_attention", 2 if a.n_items else 1)
+
+
+def _shared_fixed(plan: Any) -> _Shared:
+    """What a plan's launches have in common, checked once."""
+    host, i32 = plan.host, torch.int32
     n_slots = host.n_slots
-    if n_slots and (plan.part_o is None or plan.part_o.shape != (n_slots, Hq, D) or plan.part_ml is None or plan.part_ml.shape != (n_slots, Hq, 2)):
+    if n_slots and (plan.part_o is None or plan.part_o.shape != (n_slots, host.n_heads, host.head_dim) or plan.part_ml is None
+                    or plan.part_ml.shape != (n_slots, host.n_heads, 2)):
         raise KernelError("shared_attention: the plan's scratch must be [slots, Hq, D] and [slots, Hq, 2]")
-    sink_heads = None
-    if isinstance(sink, torch.Tensor):
-        if sink.shape != (Hq,):
-            raise KernelError("shared_attention: a sink per head must be [Hq]")
-        sink_heads, sink = _here(sink, "sink", torch.float32), 0.0
-    i32 = torch.int32
-    a = _Shared(_here(q, "q"), _here(k_slab, "k_slab"), _here(v_slab, "v_slab"), _here(out, "out"), _here(block_table, "block_table", i32),
-                _here(plan.items, "items", i32), _here(plan.members, "members", i32), _here(plan.requests, "requests", i32),
-                _here(plan.joins, "joins", i32), _here(plan.part_o, "part_o", torch.float32) if n_slots else None,
-                _here(plan.part_ml, "part_ml", torch.float32) if n_slots else None, sink_heads, _code(q, "q"), block_table.shape[1],
-                block_table.shape[0], host.items.shape[0], host.members.shape[0], host.requests.shape[0], host.joins.shape[0], n_slots, T, Hq,
-                Hkv, D, P, pages, host.tile_rows, host.cluster, host.own_tiles, float(scale), 0 if sink is None else 1, 0.0 if sink is None else float(sink))
-    _check(_lib().ftk_shared_attention(ctypes.byref(a), _stream()), "shared_attention", 2 if host.items.shape[0] else 1)
+    a = _Shared()
+    for name in ("items", "members", "requests", "joins"):
+        t, arr = getattr(plan, name), getattr(host, name)
+        if t.numel() < arr.size:
+            raise KernelError(f"shared_attention: the plan's {name} are shorter on the device than on the host")
+        setattr(a, name, _here(t, name, i32))
+        setattr(a, "n_" + name, arr.shape[0])
+    if n_slots:
+        a.part_o, a.part_ml = _here(plan.part_o, "part_o", torch.float32), _here(plan.part_ml, "part_ml", torch.float32)
+    a.n_slots, a.n_q_heads, a.n_kv_heads, a.head_dim = n_slots, host.n_heads, host.n_kv_heads, host.head_dim
+    a.tile_rows, a.cluster, a.own_tiles = host.tile_rows, host.cluster, host.own_tiles
+    return a
 
 
 def attention_tc_fits(head_dim: int, page_size: int, group: int) -> bool:
@@ -1179,10 +1208,16 @@ def sample_draws(logits: torch.Tensor, rows: Optional[torch.Tensor], temperature
         raise KernelError("sample_draws: logits must be float32 rows [N, V] of adjacent elements on the device")
     N, V = logits.shape
     R = out.numel()
-    for name, t, dt in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
-                        ("min_p", min_p, torch.float32), ("u", u, torch.float32), ("rows", rows, torch.int32), ("logprobs", logprobs, torch.float32)):
-        if t is not None and (t.numel() < R or t.dtype != dt):
-            raise KernelError(f"sample_draws: {name} must be {dt} with {R} entries")
+    f32 = torch.float32
+    ptrs = []
+    for name, t, dt in (("rows", rows, torch.int32), ("temperature", temperature, f32), ("top_k", top_k, torch.int32), ("top_p", top_p, f32),
+                        ("min_p", min_p, f32), ("u", u, f32), ("out", out, torch.int32), ("logprobs", logprobs, f32)):
+        if t is None and name in ("rows", "logprobs"):
+            ptrs.append(None)
+            continue
+        if t.numel() < R:
+            raise KernelError(f"sample_draws: {name} has fewer than {R} entries")
+        ptrs.append(_here(t, name, dt))
     if V < 1 or (R and N < 1):
         raise KernelError("sample_draws: no logits")
     if rows is None and R > N:
@@ -1190,12 +1225,9 @@ def sample_draws(logits: torch.Tensor, rows: Optional[torch.Tensor], temperature
     stride = logits.stride(0) if N > 1 else V
     if stride < V:
         raise KernelError("sample_draws: rows of logits overlap")
-    if logits.device.index != torch.cuda.current_device():
-        raise KernelError(f"sample_draws: logits are on '{logits.device}', the current device is 'cuda:{torch.cuda.current_device()}'")
-    _check(_lib().ftk_sample_draws(logits.data_ptr(), stride, N, V, _here(rows, "rows") if rows is not None else None, R,
-                                   _here(temperature, "temperature"), _here(top_k, "top_k"), _here(top_p, "top_p"), _here(min_p, "min_p"),
-                                   _here(u, "u"), _here(out, "out", torch.int32), _here(logprobs, "logprobs") if logprobs is not None else None,
-                                   _stream()), "sample_draws")
+    if logits.device.index != torch._C._cuda_getDevice():
+        raise KernelError(f"sample_draws: logits are on '{logits.device}', the current device is 'cuda:{torch._C._cuda_getDevice()}'")
+    _check(_lib().ftk_sample_draws(logits.data_ptr(), stride, N, V, ptrs[0], R, *ptrs[1:], _stream()), "sample_draws")
 
 
 # --------------------------------------------------------------------------- the 32-bit stream
