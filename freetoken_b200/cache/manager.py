@@ -14,8 +14,9 @@ reference spreads the same duties over ``CacheManager`` / ``TableManager``
 (python/freetoken/scheduler/cache.py:32-63,256-332,533-571, python/freetoken/scheduler/table.py:4-30),
 the pools (python/freetoken/kvcache/mha_pool.py:12-148) and the group specs
 (python/freetoken/models/config.py:87-111); it has no prefix reuse here (its ``naive`` cache,
-python/freetoken/kvcache/naive_cache.py:16-45): everything a request holds returns to the free
-lists when it ends.
+python/freetoken/kvcache/naive_cache.py:16-45).  A request may be forked: its copies hold the same full
+pages, and pages of their own from the last, partly filled one on.  What a request alone holds returns to the
+free lists when it ends.
 """
 
 from __future__ import annotations
@@ -130,6 +131,16 @@ class _Request:
 
 
 @dataclass
+class ForkCopies:
+    """What a fork leaves to do on the device, in this order or any: pairs for ``ops.copy_pages`` per paged group (from, to,
+    rows), for ``ops.copy_slots`` on the state tensors and on the block tables (from, to)."""
+
+    pages: List[List[Tuple[int, int, int]]]
+    slots: List[Tuple[int, int]]
+    rows: List[Tuple[int, int]]
+
+
+@dataclass
 class StepCachePlan:
     """Result of :meth:`CacheManager.begin_step` (host side)."""
 
@@ -187,6 +198,8 @@ class CacheManager:
         self._rows: List[int] = list(range(max_requests - 1, -1, -1))
         self.requests: Dict[Hashable, _Request] = {}
         self._in_step: List[Tuple[Hashable, int]] = []
+        self.forks = 0  # forks so far: without one no page is shared
+        self._spans: Dict[Any, List[Any]] = {}  # shared_spans of the requests asked about, while nobody forks or moves pages
 
     # ------------------------------------------------------------------ sizing
     @staticmethod
@@ -274,6 +287,105 @@ class CacheManager:
             g.table_host[req.row, first:n_blocks] = NULL_PAGE
         self.slots.free(req.state_slot)
         self._rows.append(req.row)
+        self._spans.clear()
+
+    # ------------------------------------------------------------------ requests that share
+    def fork_needs(self, rid: Hashable, n: int = 1) -> List[int]:
+        """Pages per paged group that ``n`` forks of ``rid`` take at once: one each where its last page is partly filled."""
+        partly = int(self.requests[rid].length % self.page_size != 0)
+        return [n * partly for _ in self.paged]
+
+    def fork(self, rid: Hashable, copies: Sequence[Hashable]) -> ForkCopies:
+        """Open ``copies`` as requests that have read what ``rid`` has, all or nothing: they hold its full pages with it, a page of their own
+        for the last, partly filled one, and a state slot of their own.  What has to be copied for that is returned."""
+        if rid not in self.requests:
+            raise CacheError(f"request {rid!r} is not open")
+        if any(r == rid for r, _ in self._in_step):
+            raise CacheError(f"request {rid!r} is part of the step in flight")
+        if len(set(copies)) != len(copies) or any(c in self.requests for c in copies):
+            raise CacheError(f"forks of request {rid!r} need names of their own")
+        if len(copies) > len(self._rows):
+            raise CacheError(f"no request slots free for {len(copies)} forks ({len(self._rows)} of {self.max_requests})")
+        for g, need in zip(self.paged, self.fork_needs(rid, len(copies))):
+            if need > g.pool.free_count:
+                raise CacheError(f"out of pages in cache group {g.index}: the forks need {need}, {g.pool.free_count} are free of {g.pool.num_pages}")
+        src = self.requests[rid]
+        full, partly = divmod(src.length, self.page_size)
+        out = ForkCopies([[] for _ in self.paged], [], [])
+        for name in copies:
+            self.open(name)
+            dst = self.requests[name]
+            dst.length = src.length
+            out.slots.append((src.state_slot, dst.state_slot))
+            out.rows.append((src.row, dst.row))
+            for g, pairs in zip(self.paged, out.pages):
+                g.first_live[dst.row] = g.first_live[src.row]
+                pages = g.table_host[src.row, :full]
+                g.table_host[dst.row, :full] = pages
+                g.pool.share(pages[pages != NULL_PAGE].tolist())
+                if partly:
+                    page = g.pool.alloc(1)[0]
+                    pairs.append((int(g.table_host[src.row, full]), page, partly))
+                    g.set_entry(dst.row, full, page)  # (behind the copied row on the device: updates go out with the next step)
+        self.forks += len(copies)
+        self._spans.clear()
+        return out
+
+    def shared_spans(self, group: PagedGroup, rids: Sequence[Hashable]) -> List[Tuple[List[int], int, int]]:
+        """Which of ``rids`` (by their places) read the same pages of ``group`` for which positions: (members, start, end), the outermost
+        first, positions in whole pages."""
+        if not self.forks or group.need.window is not None:  # (a window passes pages by: its requests read them each for itself)
+            return []
+        rows = tuple(self.requests[r].row for r in rids)
+        key = (group.index, rows)
+        known = self._spans.get(key)
+        if known is not None:
+            return known
+        lengths = [self.requests[r].length // self.page_size for r in rids]  # full pages: the others are nobody else's
+        table = group.table_host[list(rows)]
+        spans: List[Tuple[List[int], int, int]] = []
+
+        def divide(members: List[int], at: int) -> None:
+            """Spans of requests that agree in front of block ``at``."""
+            by_page: Dict[int, List[int]] = {}
+            for m in members:
+                if at < lengths[m] and table[m, at] != NULL_PAGE:
+                    by_page.setdefault(int(table[m, at]), []).append(m)
+            for together in by_page.values():
+                if len(together) < 2:
+                    continue
+                most = min(lengths[m] for m in together)
+                same = (table[together, at:most] == table[together[0], at:most]).all(axis=0) & (table[together[0], at:most] != NULL_PAGE)
+                end = most if same.all() else at + int(np.argmin(same))
+                spans.append((together, at * self.page_size, end * self.page_size))
+                divide(together, end)
+
+        divide(list(range(len(rows))), 0)
+        if len(self._spans) >= 64:
+            self._spans.clear()
+        self._spans[key] = spans
+        return spans
+
+    def compact(self) -> List[List[Tuple[int, int, int]]]:
+        """Give the pages in use the lowest numbers, in every paged group; block tables follow, on the host and the device.  Returns
+        the whole-page copies to make (pairs for ``ops.copy_pages``, per group; no target is a source)."""
+        if self._in_step:
+            raise CacheError("pages cannot move while a step is in flight")
+        out = []
+        for g in self.paged:
+            used = np.unique(g.table_host[g.table_host != NULL_PAGE])
+            places = np.setdiff1d(np.arange(1, used.size + 1, dtype=used.dtype), used, assume_unique=True)
+            moved = dict(zip(used[used > used.size].tolist(), places.tolist()))
+            out.append([(a, b, self.page_size) for a, b in moved.items()])
+            if moved:
+                number = np.arange(g.pool.num_pages + 1, dtype=np.int32)
+                number[list(moved)] = list(moved.values())
+                g.table_host[:] = number[g.table_host]
+                g.table_dev.copy_(torch.from_numpy(g.table_host))
+                g.updates = []
+            g.pool.renumber(moved)
+        self._spans.clear()
+        return out
 
     # ------------------------------------------------------------------ steps
     def begin_step(self, entries: Sequence[Tuple[Hashable, int]]) -> StepCachePlan:
@@ -303,8 +415,11 @@ class CacheManager:
             if g.need.window is not None:
                 for rid, n in entries:
                     r = self.requests[rid]
-                    reclaim += max(0, min(g.dead_blocks(r.length), -(-r.length // self.page_size))
-                                   - max(g.first_live[r.row], g.kept_blocks))
+                    lo, hi = max(g.first_live[r.row], g.kept_blocks), min(g.dead_blocks(r.length), -(-r.length // self.page_size))
+                    if self.forks:  # (what others hold too does not come back)
+                        reclaim += sum(p != NULL_PAGE and g.pool.holders(p) == 1 for p in g.table_host[r.row, lo:hi].tolist())
+                    else:
+                        reclaim += max(0, hi - lo)
             if want > g.pool.free_count + reclaim:
                 raise CacheError(
                     f"out of pages in cache group {g.index}: the step needs {want}, "

@@ -10,7 +10,7 @@ this one lives on the host and block-table changes travel with the step's metada
 
 from __future__ import annotations
 
-from typing import Iterable, List
+from typing import Dict, Iterable, List
 
 from ..errors import CacheError
 
@@ -24,7 +24,7 @@ class PagePool:
             raise CacheError(f"a page pool needs at least one page, got {num_pages}")
         self.num_pages = num_pages
         self._free: List[int] = list(range(num_pages, 0, -1))
-        self._held = [False] * (num_pages + 1)
+        self._held = [0] * (num_pages + 1)  # holders
         self.handed_out = 0  # pages ever handed out (reuse shows as handed_out > num_pages)
 
     @property
@@ -38,9 +38,21 @@ class PagePool:
             raise CacheError(f"out of pages: {n} wanted, {len(self._free)} free of {self.num_pages}")
         out = [self._free.pop() for _ in range(n)]
         for p in out:
-            self._held[p] = True
+            self._held[p] = 1
         self.handed_out += n
         return out
+
+    def share(self, pages: Iterable[int]) -> None:
+        """One more holder for each of ``pages``, which are held already."""
+        pages = list(pages)
+        for p in pages:
+            if not 1 <= p <= self.num_pages or not self._held[p]:
+                raise CacheError(f"page {p} is held by nobody and cannot be shared")
+        for p in pages:
+            self._held[p] += 1
+
+    def holders(self, page: int) -> int:
+        return self._held[page]
 
     def free(self, pages: Iterable[int]) -> None:
         for p in pages:
@@ -48,21 +60,36 @@ class PagePool:
                 raise CacheError(f"page {p} does not belong to this pool")
             if not self._held[p]:
                 raise CacheError(f"page {p} freed twice")
-            self._held[p] = False
-            self._free.append(p)
+            self._held[p] -= 1
+            if not self._held[p]:
+                self._free.append(p)
+
+    def renumber(self, moved: Dict[int, int]) -> None:
+        """Held pages ``moved`` (from -> to, the targets free) change their numbers; the lowest free page is handed out next."""
+        for a, b in moved.items():
+            if not self._held[a] or self._held[b]:
+                raise CacheError(f"page {a} cannot become page {b}")
+            self._held[b], self._held[a] = self._held[a], 0
+        self._free = [p for p in range(self.num_pages, 0, -1) if not self._held[p]]
 
     def check(self, held_by_requests: Iterable[int]) -> None:
-        """Every page is either free or held by exactly one request."""
+        """Every page is either free or held as often as it has holders.  (``held_by_requests``: pages, once per holder.)"""
         held = list(held_by_requests)
-        if len(set(held)) != len(held):
-            raise CacheError("a page is held twice")
+        times: Dict[int, int] = {}
+        for p in held:
+            times[p] = times.get(p, 0) + 1
+        for p, n in times.items():
+            if n > max(1, self._held[p]):
+                raise CacheError("a page is held twice")
         if len(set(self._free)) != len(self._free):
             raise CacheError("a page is on the free list twice")
-        if set(held) & set(self._free):
+        if set(times) & set(self._free):
             raise CacheError("a page is both held and free")
-        if len(held) + len(self._free) != self.num_pages:
+        if len(times) + len(self._free) != self.num_pages:
             raise CacheError(
-                f"pages lost: {len(held)} held + {len(self._free)} free != {self.num_pages}")
-        for p in held:
+                f"pages lost: {len(times)} held + {len(self._free)} free != {self.num_pages}")
+        for p, n in times.items():
             if not self._held[p]:
                 raise CacheError(f"page {p} is in a block table but marked free")
+            if self._held[p] != n:
+                raise CacheError(f"page {p} is in {n} block tables but has {self._held[p]} holders")

@@ -61,6 +61,8 @@ def cmd_generate(argv: List[str]) -> int:
     p.add_argument("--temperature", type=float, default=0.0)
     p.add_argument("--top-k", type=int, default=-1)
     p.add_argument("--top-p", type=float, default=1.0)
+    p.add_argument("--min-p", type=float, default=0.0, help="leave out tokens of less than this share of the likeliest one's probability")
+    p.add_argument("--n", type=int, default=1, help="continuations per prompt (the prompt is read once)")
     p.add_argument("--ignore-eos", action="store_true")
     a = p.parse_args(argv)
     prompts = [[int(x) for x in s.split(",") if x.strip()] for s in a.prompt_ids]
@@ -80,7 +82,7 @@ def cmd_generate(argv: List[str]) -> int:
     dtype = kw.pop("dtype")
     llm = LLM(a.model_path, dtype=dtype, **kw)
     sp = SamplingParams(temperature=a.temperature, top_k=a.top_k, top_p=a.top_p,
-                        ignore_eos=a.ignore_eos, max_tokens=a.max_tokens, seed=a.seed)
+                        ignore_eos=a.ignore_eos, max_tokens=a.max_tokens, seed=a.seed, min_p=a.min_p, n=a.n)
     for r in llm.generate(prompts, sp):
         print(json.dumps(r))
     return 0

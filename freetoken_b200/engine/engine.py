@@ -162,6 +162,7 @@ class Engine:
                 self._views.append(self.cache.view(owner))
         self._block_views: Dict[int, Any] = {i: self.cache.view(("block", i)) for i, _ in block_needs}
         self.buffers = StepBuffers(self.device, self._metadata_capacity())
+        self.shared_layouts: Dict[Any, Any] = {}  # of steps whose requests share pages (StepBuilder.shared_plan)
         self.graphs: Dict[Any, Any] = {}
         self.graph_logits: Dict[Any, torch.Tensor] = {}
         self.graph_launches: Dict[Any, int] = {}
@@ -217,6 +218,36 @@ class Engine:
 
     def is_open(self, rid: Hashable) -> bool:
         return self.cache.is_open(rid)
+
+    def fork(self, rid: Hashable, copies: Sequence[Hashable]) -> None:
+        """Open ``copies`` as requests that go on from where ``rid`` is: they share its full pages, and the last, partly filled one and
+        recurrent states are copied (on the current stream, behind the steps launched so far).  From then on steps that decode several
+        of them read the shared pages once (:func:`freetoken_b200.kernels.ops.shared_attention`)."""
+        if not copies:
+            return
+        made = self.cache.fork(rid, copies)
+        put = lambda pairs: torch.tensor(pairs, dtype=torch.int32).to(self.device, non_blocking=True)  # noqa: E731
+        for g, pairs in zip(self.cache.paged, made.pages):
+            if pairs:
+                ops.copy_pages(list(g.slabs.values()), put(pairs))
+        states = [t for g in self.cache.state for t in g.tensors.values()]
+        if states:
+            ops.copy_slots(states, put(made.slots))
+        tables = [g.table_dev.unsqueeze(0) for g in self.cache.paged]
+        if tables:
+            ops.copy_slots(tables, put(made.rows))
+        if self.config.check_cache:
+            self.cache.check()
+
+    def compact(self) -> List[int]:
+        """Move the pages in use to the lowest page numbers and return how many that are, per paged group: behind them the slabs hold
+        nothing (what a copy of the cache elsewhere has to take is ``slab[:, :n + 1]``).  Requests notice nothing."""
+        for g, pairs in zip(self.cache.paged, self.cache.compact()):
+            if pairs:
+                ops.copy_pages(list(g.slabs.values()), torch.tensor(pairs, dtype=torch.int32).to(self.device, non_blocking=True))
+        if self.config.check_cache:
+            self.cache.check()
+        return [g.pool.num_pages - g.pool.free_count for g in self.cache.paged]
 
     # ------------------------------------------------------------------ the step
     @torch.inference_mode()
@@ -315,6 +346,8 @@ class Engine:
                 positions[q0:q0 + n] = np.arange(kv - n, kv)
         builder = StepBuilder(self, [(s.q_len, s.kv_len) for s in segments], fixed=graphable,
                               sm_count=self.sm_count)
+        if self.cache.forks and decode_only:
+            builder.requests, builder.table_rows = [e.request_id for e in entries], plan.rows
         builder.add("token_ids", token_ids)
         builder.add("positions", positions)
         builder.add("seg_info", seg_info)

@@ -3,6 +3,10 @@
 ``generate(prompts, sampling_params) -> [{"text", "token_ids"}]``.  Prompts are lists of token
 ids; strings are accepted when the model folder has a ``tokenizer.json`` and the ``tokenizers``
 package is importable.  An EOS token that ends a request is not part of its output (llm.py:94-103).
+
+With ``SamplingParams(n=...)`` the prompt is read once and continued ``n`` times: a result then holds ``samples``, one
+``{"text", "token_ids", "finish_reason", "logprob"}`` per continuation (``logprob``: the sum of its tokens' log-probabilities under the
+model, an EOS among them), and its own keys are the first one's.
 """
 
 from __future__ import annotations
@@ -60,14 +64,22 @@ class LLM:
         sched.run(overlap=self.config.overlap_scheduling and not off)
         self.engine.check_kernels()
         results = []
-        for i in range(len(prompts)):
-            req = sched.done[i]
-            ids = list(req.output)
-            if req.finish_reason == "stop" and ids and ids[-1] in sched.eos:
-                ids = ids[:-1]
-            text = self.tokenizer.decode(ids) if self.tokenizer is not None else ""
-            item = {"text": text, "token_ids": ids, "finish_reason": req.finish_reason}
-            if req.error:
-                item["error"] = req.error
+        for i, sp in enumerate(sampling_params):
+            item = self._result(sched, i)
+            if sp.n > 1 and not sched.done[i].error:
+                others = [self._result(sched, (i, j)) for j in range(1, sp.n)]
+                item["samples"] = [{**r, "logprob": sched.done[rid].logprob}
+                                   for r, rid in zip([dict(item), *others], [i, *((i, j) for j in range(1, sp.n))])]
             results.append(item)
         return results
+
+    def _result(self, sched: Scheduler, rid) -> Dict[str, Any]:
+        req = sched.done[rid]
+        ids = list(req.output)
+        if req.finish_reason == "stop" and ids and ids[-1] in sched.eos:
+            ids = ids[:-1]
+        text = self.tokenizer.decode(ids) if self.tokenizer is not None else ""
+        item = {"text": text, "token_ids": ids, "finish_reason": req.finish_reason}
+        if req.error:
+            item["error"] = req.error
+        return item

@@ -20,6 +20,10 @@ are copied into the next step's token ids there; the host reads them one step la
 What happens when pages run out: they cannot, for admitted requests, because admission reserves
 the pages of the whole request (prompt + max_tokens) in every cache group.  A request that could
 not fit even in an empty cache is finished at once with ``finish_reason="error"``.
+
+A request for several continuations (``SamplingParams.n``) is admitted with request slots and pages for all of them.  Its prompt is
+read once; in the step that ends it the request is forked (:meth:`Engine.fork`), and the continuations' first tokens are drawn from
+the same row of logits.  From then on they are requests like any other, named ``(rid, 1)`` to ``(rid, n - 1)`` beside ``rid``.
 """
 
 from __future__ import annotations
@@ -48,6 +52,8 @@ class Request:
     reserved: List[int] = field(default_factory=list)  # pages reserved per cache group
     in_flight: int = 0  # tokens sampled on the device and not yet read by the host
     source: Optional[Tuple[Any, int]] = None  # (device tensor, index) of the newest such token
+    logprob: Optional[float] = None  # sum over its tokens' log-probabilities, where they are known (SamplingParams.draws)
+    to_fork: int = 0  # continuations beside this one that are still to begin
 
     @property
     def decoding(self) -> bool:
@@ -110,13 +116,36 @@ class Scheduler:
             return self._reject(req, f"prompt of {len(prompt)} tokens does not fit the longest "
                                      f"sequence of {self.max_seq_len}")
         req.max_tokens = min(params.max_tokens, self.max_seq_len - len(prompt))
+        if params.n > self.max_running:
+            return self._reject(req, f"{params.n} continuations, the engine runs {self.max_running} requests at once")
         need = self.engine.cache.pages_to_admit(len(prompt) + req.max_tokens,
                                                   min(self.max_step_tokens, self.max_extend))
+        if params.n > 1:
+            req.to_fork = params.n - 1
+            need = [n + req.to_fork * more for n, more in zip(need, self._fork_needs(req, need))]
         if any(n > p for n, p in zip(need, self.pool_pages)):
             return self._reject(req, f"needs {need} pages, the cache has {self.pool_pages}")
         req.reserved = need
         self.waiting.append(req)
         return rid
+
+    def _fork_needs(self, req: Request, need: Sequence[int]) -> List[int]:
+        """Pages that one continuation more holds at its peak: those behind the prompt's full ones; in a windowed group as many as a
+        request by itself (the pages that both hold may be given back by one long before the other)."""
+        full = len(req.prompt) // self.engine.cache.page_size
+        return [n if g.need.window is not None else n - full for n, g in zip(need, self.engine.cache.paged)]
+
+    def _fork(self, req: Request) -> List[Request]:
+        """The continuations of ``req``, whose prompt's last portion was just launched."""
+        names = [(req.rid, j) for j in range(1, req.to_fork + 1)]
+        self.engine.fork(req.rid, names)
+        base = self.engine.cache.pages_to_admit(len(req.prompt) + req.max_tokens, min(self.max_step_tokens, self.max_extend))
+        more = self._fork_needs(req, base)
+        req.to_fork, req.reserved = 0, base
+        copies = [Request(rid=name, prompt=req.prompt, params=req.params, max_tokens=req.max_tokens, fed=req.fed, reserved=more) for name in names]
+        at = self.running.index(req) + 1
+        self.running[at:at] = copies
+        return copies
 
     def _reject(self, req: Request, why: str) -> Hashable:
         req.finished, req.finish_reason, req.error = True, "error", why
@@ -128,6 +157,8 @@ class Scheduler:
         admitted = []
         while self.waiting and len(self.running) < self.max_running:
             req = self.waiting[0]
+            if len(self.running) + sum(r.to_fork for r in self.running) + 1 + req.to_fork > self.max_running:
+                break  # (slots that continuations will take are not free)
             if any(r + n > p for r, n, p in zip(self.reserved, req.reserved, self.pool_pages)):
                 break  # the first request that does not fit stops the pass
             self.waiting.popleft()
@@ -173,8 +204,17 @@ class Scheduler:
             if not req.decoding:
                 req.fed += len(toks)
         rows = [by_rid[rid] for rid, _ in out.rows]
+        of_row = None
+        if any(r.to_fork for r in rows):
+            of_row = []
+            for i, req in enumerate(list(rows)):  # (a request's continuations take its row, right behind it)
+                copies = self._fork(req) if req.to_fork else []
+                at = len(of_row) + 1
+                rows[at:at] = copies
+                of_row += [i] * (1 + len(copies))
+        more = {} if of_row is None else {"rows": of_row}
         ticket = self.sampler.launch(out.logits, [r.params for r in rows], [r.rid for r in rows],
-                                     [len(r.output) + r.in_flight for r in rows])
+                                     [len(r.output) + r.in_flight for r in rows], **more)
         for i, req in enumerate(rows):
             req.in_flight += 1
             req.source = (ticket.device_tokens, i)
@@ -183,12 +223,15 @@ class Scheduler:
     def _resolve(self, flight: Flight) -> StepReport:
         """Take a launched step's tokens to the host; finish and free what ended."""
         tokens = self.sampler.result(flight.ticket) if flight.ticket is not None else []
+        logprobs = self.sampler.logprobs(flight.ticket) if getattr(flight.ticket, "drawn", None) else [None] * len(tokens)
         sampled, finished = [], []
-        for req, tok in zip(flight.rows, tokens):
+        for req, tok, logprob in zip(flight.rows, tokens, logprobs):
             req.in_flight -= 1
             if req.finished:
                 continue  # ended by an earlier token; this one was computed ahead and is dropped
             req.output.append(tok)
+            if logprob is not None:
+                req.logprob = logprob + (req.logprob or 0.0)
             req.last_token = tok
             sampled.append((req.rid, tok))
             if tok in self.eos and not req.params.ignore_eos:
@@ -248,7 +291,8 @@ class Scheduler:
 
     def abort(self, rid: Hashable) -> bool:
         """Drop a request between steps; its pages and slot are given back.  A token computed
-        ahead for it (overlapped scheduling) is dropped when its step is resolved."""
+        ahead for it (overlapped scheduling) is dropped when its step is resolved.  Continuations that have begun are requests of
+        their own and go on."""
         for req in list(self.waiting):
             if req.rid == rid:
                 self.waiting.remove(req)

@@ -28,6 +28,7 @@ ROWS_TILE = 16    # query rows of a piece on the kernels for few rows
 WIDE_TILE = 256   # on the tcgen05 kernel: two tiles of 128
 WIDE_KEYS = 128   # keys that kernel works on at a time
 MOST_CLUSTER = 8
+MOST_SLOT_BYTES = 64 << 20  # of partial results, where fewer and longer pieces can do with less
 # what a piece costs the tcgen05 kernel: microseconds per key tile with one and with two query tiles, and per piece; and how fast
 # partial results are written and read again
 WIDE_ONE_US, WIDE_TWO_US, WIDE_PIECE_US, JOIN_BYTES_PER_US = 1.35, 2.1, 5.0, 2.5e6
@@ -129,12 +130,42 @@ def piece_lengths(units: np.ndarray, two: np.ndarray, members: np.ndarray, n_kv_
         rounds = -(-costs.shape[0] // g)
         costs = np.concatenate([costs, np.zeros(rounds * g - costs.shape[0])]).reshape(rounds, g)
         costs[1::2] = costs[1::2, ::-1].copy()
-        t = float(costs.sum(axis=0).max()) + float((n * members).sum()) * row_bytes / JOIN_BYTES_PER_US
+        slots = float((n * members).sum())
+        if best_t is not None and slots * row_bytes > 2 * MOST_SLOT_BYTES:
+            break  # (row_bytes: written and read)
+        t = float(costs.sum(axis=0).max()) + slots * row_bytes / JOIN_BYTES_PER_US
         if best_t is None or t < best_t * 0.99:
             best, best_t = most, t
         if most == 1:
             break
     return best
+
+
+@dataclass
+class SharedLayout:
+    """What a work list has that does not depend on the requests' lengths: it stays while the same requests share the same pages."""
+
+    items: np.ndarray
+    members: np.ndarray
+    joins: np.ndarray
+    fixed: np.ndarray  # [n, 8] requests, without their ends
+    n_slots: int
+    wide: bool
+    n_heads: int
+    n_kv_heads: int
+    head_dim: int
+    unit: int          # keys that the kernel for own keys works on at a time
+    blocks: int        # CTAs it has without clusters
+    sm_count: int
+
+    def plan(self, kv_lens: Sequence[int]) -> SharedPlan:
+        requests = self.fixed.copy()
+        requests[:, 3] = kv_lens
+        longest = max(1, int((requests[:, 3] - requests[:, 2]).max(initial=0)))
+        longest = 1 << (longest - 1).bit_length()
+        cluster = own_cluster(longest, self.blocks, self.unit, self.sm_count)
+        return SharedPlan(self.items, self.members, requests, self.joins, self.n_slots, WIDE_TILE if self.wide else ROWS_TILE, cluster,
+                          -(-longest // (cluster * self.unit)), requests.shape[0], self.n_heads, self.n_kv_heads, self.head_dim)
 
 
 def build_shared_plan(kv_lens: Sequence[int], spans: Sequence[Span], n_heads: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype,
@@ -149,7 +180,17 @@ def build_shared_plan(kv_lens: Sequence[int], spans: Sequence[Span], n_heads: in
 
     The tcgen05 kernel takes the shared keys where it takes the sizes, spans begin on multiples of 16 and a set has more query rows than
     the kernel for few rows takes at a time; ``tile_rows`` (16 or 256) asks for one of the two."""
-    n = len(kv_lens)
+    if any(x < 0 for x in kv_lens):
+        raise KernelError("shared_attention: a negative length")
+    for members, start, end in spans:
+        if any(0 <= int(m) < len(kv_lens) and int(end) > kv_lens[int(m)] for m in members):
+            raise KernelError(f"shared_attention: the span [{start}, {end}) does not lie within its members' keys")
+    return shared_layout(len(kv_lens), spans, n_heads, n_kv_heads, head_dim, dtype, page_size, table_rows, sm_count, tile_rows).plan(kv_lens)
+
+
+def shared_layout(n: int, spans: Sequence[Span], n_heads: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype, page_size: int,
+                  table_rows: Optional[Sequence[int]] = None, sm_count: int = 148, tile_rows: Optional[int] = None) -> SharedLayout:
+    """:func:`build_shared_plan` for ``n`` requests up to their lengths, which must reach the spans' ends."""
     if n_heads < 1 or n_kv_heads < 1 or n_heads % n_kv_heads:
         raise KernelError(f"shared_attention: {n_heads} query heads on {n_kv_heads} KV heads")
     rows = list(range(n)) if table_rows is None else [int(r) for r in table_rows]
@@ -157,8 +198,6 @@ def build_shared_plan(kv_lens: Sequence[int], spans: Sequence[Span], n_heads: in
         raise KernelError("shared_attention: one block-table row per request")
     if dtype not in ROWS_KEYS:
         raise KernelError(f"shared_attention: dtype {dtype} is not supported (float32 or bfloat16)")
-    if any(x < 0 for x in kv_lens):
-        raise KernelError("shared_attention: a negative length")
     group = n_heads // n_kv_heads
     taken: List[List[Tuple[int, int]]] = [[] for _ in range(n)]
     sets: List[Tuple[List[int], int, int]] = []
@@ -167,7 +206,7 @@ def build_shared_plan(kv_lens: Sequence[int], spans: Sequence[Span], n_heads: in
         start, end = int(start), int(end)
         if len(set(members)) != len(members) or any(not 0 <= m < n for m in members):
             raise KernelError("shared_attention: a span's members are different requests of the step")
-        if start < 0 or any(end > kv_lens[m] for m in members):
+        if start < 0:
             raise KernelError(f"shared_attention: the span [{start}, {end}) does not lie within its members' keys")
         if end <= start or len(members) < 2:
             continue
@@ -210,7 +249,7 @@ def build_shared_plan(kv_lens: Sequence[int], spans: Sequence[Span], n_heads: in
     items = [it[1:] for it in sorted(items, key=lambda it: it[0])]  # the longest first
 
     # what is a request's own: one range behind its spans
-    requests, joins, longest = [], [], 1
+    requests, joins = [], []
     for i in range(n):
         begin = 0
         for a, b in sorted(taken[i]):
@@ -218,11 +257,8 @@ def build_shared_plan(kv_lens: Sequence[int], spans: Sequence[Span], n_heads: in
                 raise KernelError(f"shared_attention: the spans of request {i} leave out positions {begin} to {a}")
             begin = b
         own = [s for _, s in sorted(slots[i])]
-        requests.append((i, rows[i], begin, int(kv_lens[i]), len(joins), len(own), 0, 0))
+        requests.append((i, rows[i], begin, begin, len(joins), len(own), 0, 0))
         joins += own
-        longest = max(longest, int(kv_lens[i]) - begin)
-    longest = 1 << (longest - 1).bit_length()
-    cluster = own_cluster(longest, max(1, n * n_kv_heads * chunks), ROWS_KEYS[dtype], sm_count)
     as_int = lambda x, w: np.asarray(x, dtype=np.int32).reshape(-1, w) if w else np.asarray(x, dtype=np.int32)  # noqa: E731
-    return SharedPlan(as_int(items, ITEM_INTS), as_int(member_rows, 0), as_int(requests, REQUEST_INTS), as_int(joins, 0), n_slots,
-                      WIDE_TILE if wide else ROWS_TILE, cluster, -(-longest // (cluster * ROWS_KEYS[dtype])), n, n_heads, n_kv_heads, head_dim)
+    return SharedLayout(as_int(items, ITEM_INTS), as_int(member_rows, 0), as_int(joins, 0), as_int(requests, REQUEST_INTS), n_slots, wide,
+                        n_heads, n_kv_heads, head_dim, ROWS_KEYS[dtype], max(1, n * n_kv_heads * chunks), sm_count)

@@ -22,6 +22,7 @@ import numpy as np
 import torch
 
 from .attention_plan import TC_ONE_TILE_COSTS, TC_TWO_TILE_COSTS, AttentionPlan, build_plan, wave_splits
+from .shared_plan import SharedPlan, shared_layout
 
 ALIGN = 4  # int32 elements = 16 bytes
 MOST_LAYOUTS = 64  # layouts of steps whose views are kept
@@ -138,7 +139,10 @@ class StepBuilder:
         self.sm_count = sm_count
         self.sections: List[Tuple[str, np.ndarray]] = []
         self.decode_only = all(q == 1 for q, _ in self.seg_lens)
-        self.plans: Dict[Any, AttentionPlan] = {}
+        self.plans: Dict[Any, Any] = {}  # AttentionPlan or SharedPlan
+        self.requests: List[Any] = []    # of a step that decodes requests which may share pages, and their block-table rows
+        self.table_rows: List[int] = []
+        self._shared: Dict[Any, Any] = {}  # what mixers asked shared_plan for
         self._drafts: Dict[Any, AttentionPlan] = {}  # work lists made to compare kernel forms, not (yet) part of the step
         self.plan_dims: Dict[Any, Tuple[int, int, int]] = {}
 
@@ -215,10 +219,46 @@ class StepBuilder:
             self.add(f"plan.{len(self.plans) - 1}", plan.items)
         return key
 
+    def shared_plan(self, need, n_heads: int, n_kv_heads: int, head_dim: int, dtype, worth) -> Any:
+        """Key of the work list over shared keys for mixers whose cache is ``need``'s, or None where the step's requests share nothing that
+        is ``worth(saved keys)`` it.  What of it does not depend on the requests' lengths is kept while they share the same pages."""
+        if len(self.requests) < 2:
+            return None
+        cache = self.engine.cache
+        group = next((g for g in cache.paged if g.need.group_key() == need.group_key()), None)
+        if group is None:
+            return None
+        what = (group.index, n_heads, n_kv_heads, head_dim)
+        if what in self._shared:
+            return self._shared[what]
+        self._shared[what] = None
+        spans = cache.shared_spans(group, self.requests)
+        if not spans or not worth(sum((len(m) - 1) * (end - start) for m, start, end in spans)):
+            return None
+        known = self.engine.shared_layouts.get(what)
+        if known is None or known[0] is not spans:  # (the same spans as long as nobody forks, ends or moves)
+            known = (spans, shared_layout(len(self.requests), spans, n_heads, n_kv_heads, head_dim, dtype, cache.page_size,
+                                          self.table_rows, self.sm_count))
+            self.engine.shared_layouts[what] = known
+        plan = known[1].plan(self._segments[:, 1])
+        key = self._shared[what] = ("shared_attention", *what, *plan.key())
+        self.plans[key] = plan
+        for name, arr in plan.sections():
+            self.add(f"plan.{len(self.plans) - 1}.{name}", arr)
+        return key
+
     def finish(self, buffers: StepBuffers, workspace) -> Tuple[Dict[str, torch.Tensor], Dict[Any, DevicePlan]]:
         tensors = buffers.upload(self.sections)
         plans: Dict[Any, DevicePlan] = {}
         for i, (key, plan) in enumerate(self.plans.items()):
+            if isinstance(plan, SharedPlan):
+                part_o = part_ml = None
+                if plan.n_slots:
+                    room = 1 << (plan.n_slots - 1).bit_length()  # (a buffer that a recorded graph points to is never replaced: few sizes)
+                    part_o = workspace.get(f"shared.part.{i}.{room}.o", (room, plan.n_heads, plan.head_dim), torch.float32)[:plan.n_slots]
+                    part_ml = workspace.get(f"shared.part.{i}.{room}.ml", (room, plan.n_heads, 2), torch.float32)[:plan.n_slots]
+                plans[key] = plan.bind({name: tensors[f"plan.{i}.{name}"] for name, _ in plan.sections()}, part_o, part_ml)
+                continue
             n_kv, rows, dim = self.plan_dims[key]
             part_o = part_ml = None
             if plan.n_slots:

@@ -43,6 +43,7 @@ TC_PAIR_MIN_TOKENS = 1024  # from this many tokens on, a step goes to the kernel
 TC_PAIR_MIN_TOKENS_LONG = 256  # ... and from this many on when its longest request has TC_PAIR_MIN_SPAN keys and more
 TC_PAIR_MIN_SPAN = 16384       # (rounded up to 2^n): such tiles are cut along the keys into enough pieces for every SM
 AHEAD_MOST_BYTES = 40_000_000  # largest weight that a single token's attention brings into L2 (see GQAttention._weight_ahead)
+SHARED_MIN_KEYS = 1024   # keys that sharing has to save a decode step
 TC_MIN_DECODE_SPAN = 0   # decode steps go there from this length of the longest request (rounded up to 2^n) on
 
 
@@ -113,6 +114,12 @@ def attention_tile_rows(dtype: torch.dtype, decode_only: bool = False, group: in
                         longest_span: int = 0) -> int:
     """Query rows (tokens x group heads) one attention CTA handles (see :func:`attention_kernel_form`)."""
     return attention_kernel_form(dtype, decode_only, group, n_tokens, head_dim, page_size, window, longest_span)[0]
+
+
+def sharing_pays(saved: int) -> bool:
+    """Whether a decode step whose requests would read ``saved`` keys again that another of them reads is taken by
+    ``ops.shared_attention``."""
+    return saved >= SHARED_MIN_KEYS
 
 
 @MIXERS.register("gqa_attention")
@@ -188,6 +195,7 @@ class GQAttention(Mixer):
                           or self.learned_sink or self.proj_bias or self.log_dist_bias or self.neighbours
                           or self.keep_first)
         self._o_weight: Optional[torch.Tensor] = None
+        self._step_shared: Any = None  # the step's work list over shared keys, where its requests share enough
 
     # ------------------------------------------------------------------ tensors
     def param_specs(self) -> Dict[str, ParamSpec]:
@@ -276,6 +284,12 @@ class GQAttention(Mixer):
         page_size = builder.engine.config.page_size if builder.engine is not None else 0
         # forward() of the same step runs the kernel this work list was made for
         self._step_span = builder.longest_span()
+        self._step_shared = None
+        if builder.decode_only and self.own_kv and not self.log_dist_bias and self.window is None and getattr(builder, "requests", None):
+            self._step_shared = builder.shared_plan(self.cache_need(), self.n_heads, self.n_kv_heads, self.pad_dim, self.env.dtype,
+                                                    sharing_pays)
+            if self._step_shared is not None:
+                return
         rows, few_rows = self.kernel_form(builder.decode_only, n_tokens, page_size, self._step_span)
         if rows >= 128 and not few_rows and not builder.decode_only and n_tokens >= TC_PAIR_MIN_TOKENS_LONG \
                 and self.sink is None and not self.learned_sink and not self.log_dist_bias and self.window is None \
@@ -308,14 +322,20 @@ class GQAttention(Mixer):
                                  slab=cache.slabs["v"], slot_map=cache.slot_map))
         ops.norm_rope_store(qkv, self.head_dim, self.rotary_dim, step.positions,
                             self.position.table(), self.eps, self.gemma, sections)
-        plan = step.attention_plans[self._step_plan]
         o = ws.get("attn.o", (T, self.n_heads, self.head_dim), dt, (cap, self.n_heads, self.head_dim))
+        if self._step_shared is not None:
+            ops.shared_attention(q, cache.slabs["k"], cache.slabs["v"], cache.block_table, step.attention_plans[self._step_shared], o, self.scale)
+            return self._projected(o.view(T, self.q_dim), self.params["o_proj.weight"])
+        plan = step.attention_plans[self._step_plan]
         ops.paged_attention(q, cache.slabs["k"], cache.slabs["v"], cache.block_table, step.seg_info,
                             len(step.segments), plan.items_dev, plan.n_items, plan.part_o, plan.part_ml,
                             o, self._step_plan[2], self.scale, self.window, few_rows=self._step_plan[6],
                             **self._weight_ahead(T, self.params["o_proj.weight"]))
-        out = ws.get("attn.out", (T, self.hidden), dt, (cap, self.hidden))
-        ops.linear(o.view(T, self.q_dim), self.params["o_proj.weight"], out)
+        return self._projected(o.view(T, self.q_dim), self.params["o_proj.weight"])
+
+    def _projected(self, o: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+        out = self.env.workspace.get("attn.out", (o.shape[0], self.hidden), self.env.dtype, (self.env.max_step_tokens, self.hidden))
+        ops.linear(o, weight, out)
         return out
 
     def _weight_ahead(self, n_tokens: int, weight: torch.Tensor) -> Dict[str, torch.Tensor]:
@@ -360,15 +380,17 @@ class GQAttention(Mixer):
             ops.norm_rope_store(proj[:, self.v_row: self.g_row], Dv, 0, step.positions, None, self.eps, self.gemma,
                                 [dict(first_head=0, n_heads=G, norm_weight=None, rotate=False, slab=cache.slabs["v"],
                                       slot_map=cache.slot_map, dst_head_dim=Dp, bias=self.params.get("v_bias"))])
-        plan = step.attention_plans[self._step_plan]
         o = ws.get("attn.o", (T, H, Dp), dt, (cap, H, Dp))
-        ops.paged_attention(q, cache.slabs["k"], cache.slabs["v"], cache.block_table, step.seg_info,
-                            len(step.segments), plan.items_dev, plan.n_items, plan.part_o, plan.part_ml,
-                            o, self._step_plan[2], self.scale, self.window, few_rows=self._step_plan[6],
-                            kv_split=self.kv_split, sink=self.params["sink"] if self.learned_sink else self.sink,
-                            dist_bias=self.dist_table(), keep_first=self.keep_first)
+        sink = self.params["sink"] if self.learned_sink else self.sink
+        if self._step_shared is not None:
+            ops.shared_attention(q, cache.slabs["k"], cache.slabs["v"], cache.block_table, step.attention_plans[self._step_shared], o,
+                                 self.scale, sink=sink)
+        else:
+            plan = step.attention_plans[self._step_plan]
+            ops.paged_attention(q, cache.slabs["k"], cache.slabs["v"], cache.block_table, step.seg_info,
+                                len(step.segments), plan.items_dev, plan.n_items, plan.part_o, plan.part_ml,
+                                o, self._step_plan[2], self.scale, self.window, few_rows=self._step_plan[6],
+                                kv_split=self.kv_split, sink=sink, dist_bias=self.dist_table(), keep_first=self.keep_first)
         if self.out_gate:
             ops.gated_heads(o, proj[:, self.g_row:], o, Dv, self.out_gate)
-        out = ws.get("attn.out", (T, self.hidden), dt, (cap, self.hidden))
-        ops.linear(o.view(T, H * Dp), self._o_weight, out)
-        return out
+        return self._projected(o.view(T, H * Dp), self._o_weight)
