@@ -14,6 +14,7 @@ its sizes while the requests grow.  The reference reads shared pages once per re
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import Dict, List, Optional, Sequence, Tuple
 
@@ -103,9 +104,35 @@ def own_cluster(longest: int, blocks: int, tile: int, sm_count: int) -> int:
     return cluster
 
 
+def rows_length(units: Sequence[int], heads: int, dtype: torch.dtype, sm_count: int) -> int:
+    """The most tiles of keys a piece of the kernels for few rows may have.  A CTA goes through its piece tile by tile, and every piece's
+    result is joined behind it, so both grow with the root of a span; and pieces beyond one wave of CTAs (four, once there are
+    that many) only queue.  Measured, pieces of 1, 2 and 4 tiles: two requests of 48 heads on 8 over 256 keys 8.7, 9.5, 11.5 us, over 1,024
+    11.3, 10.5, 11.8, over 4,096 29.7, 18.7, 14.6; 16 over 256 15.4, 11.0, 12.0; in 32 bits (16 heads on 4 of 64) two over 256 9.0,
+    11.8, 18.2, over 4,096 24.3, 19.7, 21.8."""
+    if not units:
+        return 1
+    total = sum(units) * heads
+    root = math.ceil(math.sqrt(max(units)) / (2 if dtype == torch.bfloat16 else 4))
+    return max(root, -(-total // (sm_count if total <= 4 * sm_count else 4 * sm_count)))
+
+
 def takes_wide(dtype: torch.dtype, head_dim: int, page_size: int, group: int) -> bool:
     """Whether the tcgen05 kernel takes these sizes (``csrc/shared_attention_tc.cuh: shared_tc_fits``)."""
     return dtype == torch.bfloat16 and head_dim in (64, 128) and page_size % 16 == 0 and page_size >= 16 and group <= WIDE_TILE // 2
+
+
+def wide_pays(sets: Sequence[Span], group: int, n_kv_heads: int, head_dim: int) -> bool:
+    """Whether the tcgen05 kernel is faster than the one for few rows.  That one reads a set's keys once for every 16 query rows, the
+    other has some 5 us more around its pieces: it takes over from 45,000 keys on, counted once per tile of 16 rows and KV head, where those
+    tiles are 24 and more, from 100,000 where they are fewer (and hold up each other less), twice as many for heads of 64.  A layer of 48
+    heads on 8 of 128, few rows against tcgen05: 3 requests over 4,096 keys 17.7 and 19.7 us, over 8,192 32.0 and 22.0; 5 over 1,024 12.8 and
+    13.1, over 2,048 15.4 and 14.8; 48 over 256 20.0 and 14.6.  16 on 4 of 128: 8 over 8,192 20.5 and 22.5, over 16,384 25.9 and 24.8; 48 over
+    256 10.3 and 14.3, over 1,024 18.4 and 15.1; of 64: 48 over 1,024 12.3 and 12.5, over 2,048 16.9 and 13.3; 16 over 8,192 16.1 and
+    19.2, over 16,384 28.7 and 21.3."""
+    tiles = [-(-len(members) // max(1, ROWS_TILE // group)) * max(1, -(-group // ROWS_TILE)) * n_kv_heads for members, _, _ in sets]
+    keys = sum(t * (end - start) for t, (_, start, end) in zip(tiles, sets))
+    return keys * head_dim >= 128 * (45000 if sum(tiles) >= 24 else 100000)
 
 
 def piece_lengths(units: np.ndarray, two: np.ndarray, members: np.ndarray, n_kv_heads: int, row_bytes: int, ctas: int) -> int:
@@ -178,8 +205,8 @@ def build_shared_plan(kv_lens: Sequence[int], spans: Sequence[Span], n_heads: in
     for these positions (the first member's row is read).  ``end`` may lie inside a page.  The spans of one request must not
     overlap and leave no positions out in front of them; a span of a single member is that request's own.
 
-    The tcgen05 kernel takes the shared keys where it takes the sizes, spans begin on multiples of 16 and a set has more query rows than
-    the kernel for few rows takes at a time; ``tile_rows`` (16 or 256) asks for one of the two."""
+    The tcgen05 kernel takes the shared keys where it takes the sizes, spans begin on multiples of 16 and it is faster
+    (:func:`wide_pays`); ``tile_rows`` (16 or 256) asks for one of the two."""
     if any(x < 0 for x in kv_lens):
         raise KernelError("shared_attention: a negative length")
     for members, start, end in spans:
@@ -217,7 +244,7 @@ def shared_layout(n: int, spans: Sequence[Span], n_heads: int, n_kv_heads: int, 
         sets.append((members, start, end))
 
     wide = takes_wide(dtype, head_dim, page_size, group) and all(start % 16 == 0 for _, start, _ in sets) \
-        and any(len(members) * group > ROWS_TILE for members, _, _ in sets)
+        and wide_pays(sets, group, n_kv_heads, head_dim)
     if tile_rows is not None:
         if tile_rows not in (ROWS_TILE, WIDE_TILE) or (tile_rows == WIDE_TILE and (not takes_wide(dtype, head_dim, page_size, group) or any(
                 start % 16 for _, start, _ in sets))):
@@ -231,8 +258,8 @@ def shared_layout(n: int, spans: Sequence[Span], n_heads: int, n_kv_heads: int, 
     if wide and tiles:
         length = piece_lengths(np.array(units), np.array([2 * len(m) > most for m, _, _ in tiles]), np.array([len(m) for m, _, _ in tiles]),
                                n_kv_heads, 8 * n_heads * head_dim, sm_count)
-    else:  # pieces of about as many units for every CTA that fits
-        length = max(4, -(-sum(units) * n_kv_heads * chunks // (4 * sm_count)))
+    else:
+        length = rows_length(units, n_kv_heads * chunks, dtype, sm_count)
     items, member_rows, slots = [], [], [[] for _ in range(n)]
     n_slots = 0
     for (members, start, end), u in zip(tiles, units):

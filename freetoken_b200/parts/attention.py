@@ -43,7 +43,8 @@ TC_PAIR_MIN_TOKENS = 1024  # from this many tokens on, a step goes to the kernel
 TC_PAIR_MIN_TOKENS_LONG = 256  # ... and from this many on when its longest request has TC_PAIR_MIN_SPAN keys and more
 TC_PAIR_MIN_SPAN = 16384       # (rounded up to 2^n): such tiles are cut along the keys into enough pieces for every SM
 AHEAD_MOST_BYTES = 40_000_000  # largest weight that a single token's attention brings into L2 (see GQAttention._weight_ahead)
-SHARED_MIN_KEYS = 1024   # keys that sharing has to save a decode step
+SHARED_MIN_KEYS = 512    # keys that sharing has to save a decode step, in all
+SHARED_MIN_KEYS_EACH = 100  # and for each of its requests
 TC_MIN_DECODE_SPAN = 0   # decode steps go there from this length of the longest request (rounded up to 2^n) on
 
 
@@ -116,10 +117,13 @@ def attention_tile_rows(dtype: torch.dtype, decode_only: bool = False, group: in
     return attention_kernel_form(dtype, decode_only, group, n_tokens, head_dim, page_size, window, longest_span)[0]
 
 
-def sharing_pays(saved: int) -> bool:
-    """Whether a decode step whose requests would read ``saved`` keys again that another of them reads is taken by
-    ``ops.shared_attention``."""
-    return saved >= SHARED_MIN_KEYS
+def sharing_pays(saved: int, requests: int) -> bool:
+    """Whether a decode step of ``requests`` that would read ``saved`` keys again that another of them reads is taken by
+    ``ops.shared_attention``: from a hundred keys a request on.  A layer's attention, ``ops.paged_attention`` against it, 48 heads on 8 of
+    128: 16 requests over 64 shared keys 8.2 and 10.0 us, over 256 11.0 and 11.1, over 1,024 17.9 and 14.1, over 16,384 156 and 38; 48 over 64
+    14.9 and 16.4, over 256 22.0 and 14.6, over 16,384 422 and 52; 3 over 256 10.3 and 9.0, over 4,096 16.4 and 17.7, over 16,384 36.1 and
+    27.9; 16 on 4 of 64, 48 over 256 16.9 and 7.9, in 32 bits 19.2 and 17.1."""
+    return saved >= SHARED_MIN_KEYS and saved >= SHARED_MIN_KEYS_EACH * requests
 
 
 @MIXERS.register("gqa_attention")

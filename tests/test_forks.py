@@ -206,6 +206,7 @@ def test_forked_requests_give_the_plain_models_logits(name, cpu, monkeypatch, tm
     shared pages through the shared list (block-sparse layers do not)."""
     calls = []
     monkeypatch.setattr("freetoken_b200.parts.attention.SHARED_MIN_KEYS", 1)
+    monkeypatch.setattr("freetoken_b200.parts.attention.SHARED_MIN_KEYS_EACH", 0)
     monkeypatch.setattr(ops, "shared_attention", lambda *a, **k: (calls.append(1), fork_refs.shared_attention(*a, **k))[1])
     folder = model_folder(tmp_path_factory.getbasetemp(), name, ALL[name])
     plain = PlainM3(folder)

@@ -26,6 +26,7 @@ OTHERS = {f"{m}-{n}": raw for m, every in (("gizulorn", GIZULORN), ("kekopel", K
 def sharing(monkeypatch):
     """Every decode step whose requests share a page takes the shared list; how often that was."""
     monkeypatch.setattr("freetoken_b200.parts.attention.SHARED_MIN_KEYS", 1)
+    monkeypatch.setattr("freetoken_b200.parts.attention.SHARED_MIN_KEYS_EACH", 0)
     ops.variant_counts(reset=True)
     return lambda: {k: v for k, v in ops.variant_counts().items() if k.startswith("shared attention")}
 

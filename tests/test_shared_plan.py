@@ -92,19 +92,24 @@ def test_refusals(lens, spans, what):
         build_shared_plan(lens, spans, 8, 2, 64, torch.float32, 16)
 
 
-def test_the_wide_form_is_taken_where_it_fits():
-    rows = lambda members, heads=16, kv=4, dim=64, dtype=torch.bfloat16, page=16, **kw: build_shared_plan(  # noqa: E731
-        [200] * 40, [(list(range(members)), 0, 160)], heads, kv, dim, dtype, page, **kw).tile_rows
-    assert rows(20) == 256 and rows(20, dim=128) == 256
-    assert rows(4) == 16  # 16 query rows
-    assert rows(20, dtype=torch.float32) == rows(20, dim=48) == rows(20, page=8) == rows(20, heads=516) == 16
-    assert rows(20, tile_rows=16) == 16 and rows(4, tile_rows=256) == 256
-    assert build_shared_plan([200] * 9, [(list(range(9)), 0, 30), (list(range(9)), 30, 160)], 16, 4, 64, torch.bfloat16, 16).tile_rows == 16
-    for kw in (dict(dim=48), dict(dtype=torch.float32), dict(page=8)):
+def test_the_wide_form_is_taken_where_it_fits_and_pays():
+    def rows(members, keys, heads=16, kv=4, dim=64, dtype=torch.bfloat16, page=16, start=0, **kw):
+        spans = ([(list(range(members)), 0, start)] if start else []) + [(list(range(members)), start, keys)]
+        return build_shared_plan([keys + 40] * 48, spans, heads, kv, dim, dtype, page, **kw).tile_rows
+
+    # the figures beside the rule: who is faster there
+    assert [rows(n, k, 48, 8, 128) for n, k in ((3, 4096), (3, 8192), (5, 1024), (5, 2048), (48, 256), (16, 256), (16, 1024))] == [16, 256, 16, 256, 256, 16, 256]
+    assert [rows(n, k, 16, 4, 128) for n, k in ((8, 8192), (8, 16384), (48, 256), (48, 1024), (2, 16384))] == [16, 256, 16, 256, 16]
+    assert [rows(n, k) for n, k in ((48, 1024), (48, 2048), (16, 8192), (16, 16384))] == [16, 256, 16, 256]
+    # sizes that it does not take
+    assert rows(48, 4096) == 256
+    assert rows(48, 4096, dtype=torch.float32) == rows(48, 4096, dim=48) == rows(48, 4096, page=8) == rows(48, 4096, heads=516) == rows(48, 4096, start=30) == 16
+    assert rows(48, 4096, tile_rows=16) == 16 and rows(2, 64, tile_rows=256) == 256
+    for kw in (dict(dim=48), dict(dtype=torch.float32), dict(page=8), dict(start=30)):
         with pytest.raises(KernelError):
-            rows(20, tile_rows=256, **kw)
+            rows(20, 4096, tile_rows=256, **kw)
     with pytest.raises(KernelError):
-        rows(20, tile_rows=64)
+        rows(20, 4096, tile_rows=64)
     with pytest.raises(KernelError):
         build_shared_plan([1], [], 8, 2, 64, torch.float16, 16)
     assert build_shared_plan([5], [], 8, 2, 64, torch.bfloat16, 16, tile_rows=256).items.shape == (0, 8)
