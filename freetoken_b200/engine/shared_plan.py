@@ -30,6 +30,7 @@ WIDE_TILE = 256   # on the tcgen05 kernel: two tiles of 128
 WIDE_KEYS = 128   # keys that kernel works on at a time
 MOST_CLUSTER = 8
 MOST_SLOT_BYTES = 64 << 20  # of partial results, where fewer and longer pieces can do with less
+OWN_CTAS_PER_SM, OWN_BEHIND_US = 4, 9.0  # of the kernel for own keys; what it takes more where it has to wait for the other to end
 # what a piece costs the tcgen05 kernel: microseconds per key tile with one and with two query tiles, and per piece; and how fast
 # partial results are written and read again
 WIDE_ONE_US, WIDE_TWO_US, WIDE_PIECE_US, JOIN_BYTES_PER_US = 1.35, 2.1, 5.0, 2.5e6
@@ -97,9 +98,11 @@ def tile_members(n: int, most: int) -> List[Tuple[int, int]]:
 
 
 def own_cluster(longest: int, blocks: int, tile: int, sm_count: int) -> int:
-    """CTAs that share one request's own keys: as many as fill the GPU twice, none with less than a tile of keys."""
+    """CTAs that share one request's own keys: no more than fill the GPU once, none with less than two tiles of keys.  (Clusters that queue
+    for SMs wait for several to be free at once.  48 heads on 8 of 128, clusters of 1, 2, 4 and 8: 20 requests of 600 own keys 26.4, 35.6,
+    46.9, 77.8 us; 8 of 300 24.8, 22.5, 22.0, 26.6; 4 of 1,500 of 16 heads on 4 34.6, 22.3, 16.4, 17.4; 2 of 500 15.1, 11.5, 10.0, 10.2.)"""
     cluster = 1
-    while cluster < MOST_CLUSTER and blocks * cluster < 2 * sm_count and longest > cluster * tile:
+    while cluster < MOST_CLUSTER and 2 * blocks * cluster <= sm_count and longest > 2 * cluster * tile:
         cluster *= 2
     return cluster
 
@@ -135,9 +138,11 @@ def wide_pays(sets: Sequence[Span], group: int, n_kv_heads: int, head_dim: int) 
     return keys * head_dim >= 128 * (45000 if sum(tiles) >= 24 else 100000)
 
 
-def piece_lengths(units: np.ndarray, two: np.ndarray, members: np.ndarray, n_kv_heads: int, row_bytes: int, ctas: int) -> int:
+def piece_lengths(units: np.ndarray, two: np.ndarray, members: np.ndarray, n_kv_heads: int, row_bytes: int, ctas: int, own_ctas: int) -> int:
     """The most key tiles a piece of the tcgen05 kernel may have, by the estimated time of the launches: the kernel deals the sorted
-    list out to and fro over its CTAs, the busiest of them decides; partial results are written and read once per piece."""
+    list out to and fro over its CTAs, the busiest of them decides; partial results are written and read once per piece; and the kernel
+    for own keys runs under it where SMs are left that have room for all of its CTAs.  (12 requests of 48 heads on 8 over 4,096 keys, 128 pieces 28.2
+    us, 64 pieces 18.9; 16 over 16,384 37.1 and 31.2 with 104.)"""
     best, best_t = 1, None
     longest = int(units.max())
     seen = set()
@@ -161,6 +166,8 @@ def piece_lengths(units: np.ndarray, two: np.ndarray, members: np.ndarray, n_kv_
         if best_t is not None and slots * row_bytes > 2 * MOST_SLOT_BYTES:
             break  # (row_bytes: written and read)
         t = float(costs.sum(axis=0).max()) + slots * row_bytes / JOIN_BYTES_PER_US
+        if own_ctas > OWN_CTAS_PER_SM * (ctas - g):
+            t += OWN_BEHIND_US
         if best_t is None or t < best_t * 0.99:
             best, best_t = most, t
         if most == 1:
@@ -255,9 +262,10 @@ def shared_layout(n: int, spans: Sequence[Span], n_heads: int, n_kv_heads: int, 
     unit = WIDE_KEYS if wide else ROWS_KEYS[dtype]
     tiles = [(members[a:a + k], start, end) for members, start, end in sets for a, k in tile_members(len(members), most)]
     units = [-(-(end - start) // unit) for _, start, end in tiles]
+    own_ctas = max(1, n * n_kv_heads * chunks)
     if wide and tiles:
         length = piece_lengths(np.array(units), np.array([2 * len(m) > most for m, _, _ in tiles]), np.array([len(m) for m, _, _ in tiles]),
-                               n_kv_heads, 8 * n_heads * head_dim, sm_count)
+                               n_kv_heads, 8 * n_heads * head_dim, sm_count, max(own_ctas, min(2 * own_ctas, sm_count)))  # (clusters of two, often)
     else:
         length = rows_length(units, n_kv_heads * chunks, dtype, sm_count)
     items, member_rows, slots = [], [], [[] for _ in range(n)]
@@ -288,4 +296,4 @@ def shared_layout(n: int, spans: Sequence[Span], n_heads: int, n_kv_heads: int, 
         joins += own
     as_int = lambda x, w: np.asarray(x, dtype=np.int32).reshape(-1, w) if w else np.asarray(x, dtype=np.int32)  # noqa: E731
     return SharedLayout(as_int(items, ITEM_INTS), as_int(member_rows, 0), as_int(joins, 0), as_int(requests, REQUEST_INTS), n_slots, wide,
-                        n_heads, n_kv_heads, head_dim, ROWS_KEYS[dtype], max(1, n * n_kv_heads * chunks), sm_count)
+                        n_heads, n_kv_heads, head_dim, ROWS_KEYS[dtype], own_ctas, sm_count)

@@ -73,9 +73,10 @@ def test_members_are_dealt_to_tiles_evenly():
 
 def test_own_keys_are_split_while_the_gpu_is_not_full():
     assert own_cluster(2048, 8, 64, 148) == 8
-    assert own_cluster(64, 8, 64, 148) == 1      # a tile of keys each at least
+    assert own_cluster(128, 8, 64, 148) == 1     # two tiles of keys each at least
+    assert own_cluster(512, 8, 64, 148) == 4
     assert own_cluster(2048, 512, 64, 148) == 1  # enough requests
-    assert own_cluster(256, 200, 64, 148) == 2
+    assert own_cluster(512, 64, 64, 148) == 2
 
 
 @pytest.mark.parametrize("lens,spans,what", [
