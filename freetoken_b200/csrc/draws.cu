@@ -51,32 +51,73 @@ __device__ __forceinline__ float of_key(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// 2^(j / 32)
-__device__ const double kPowers[32] = {
-    1.00000000000000000e+00, 1.02189714865411663e+00, 1.04427378242741375e+00, 1.06714040067682370e+00,
-    1.09050773266525769e+00, 1.11438674259589243e+00, 1.13878863475669156e+00, 1.16372485877757748e+00,
-    1.18920711500272103e+00, 1.21524735998046896e+00, 1.24185781207348400e+00, 1.26905095719173322e+00,
-    1.29683955465100964e+00, 1.32523664315974132e+00, 1.35425554693689265e+00, 1.38390988196383202e+00,
-    1.41421356237309515e+00, 1.44518080697704665e+00, 1.47682614593949935e+00, 1.50916442759342284e+00,
-    1.54221082540794074e+00, 1.57598084510788650e+00, 1.61049033194925428e+00, 1.64575547815396495e+00,
-    1.68179283050742900e+00, 1.71861929812247793e+00, 1.75625216037329945e+00, 1.79470907500310717e+00,
-    1.83400808640934243e+00, 1.87416763411029996e+00, 1.91520656139714740e+00, 1.95714412417540018e+00,
+// 2^(j / 256)
+__device__ const double kPowers[256] = {
+    1.00000000000000000e+00, 1.00271127505020252e+00, 1.00542990111280273e+00, 1.00815589811841755e+00, 1.01088928605170048e+00,
+    1.01363008495148943e+00, 1.01637831491095310e+00, 1.01913399607773791e+00, 1.02189714865411663e+00, 1.02466779289713572e+00,
+    1.02744594911876375e+00, 1.03023163768604098e+00, 1.03302487902122841e+00, 1.03582569360195720e+00, 1.03863410196137873e+00,
+    1.04145012468831610e+00, 1.04427378242741375e+00, 1.04710509587928979e+00, 1.04994408580068721e+00, 1.05279077300462642e+00,
+    1.05564517836055716e+00, 1.05850732279451276e+00, 1.06137722728926209e+00, 1.06425491288446450e+00, 1.06714040067682370e+00,
+    1.07003371182024187e+00, 1.07293486752597556e+00, 1.07584388906279105e+00, 1.07876079775711986e+00, 1.08168561499321525e+00,
+    1.08461836221330921e+00, 1.08755906091776966e+00, 1.09050773266525769e+00, 1.09346439907288584e+00, 1.09642908181637688e+00,
+    1.09940180263022191e+00, 1.10238258330784089e+00, 1.10537144570174117e+00, 1.10836841172367873e+00, 1.11137350334481755e+00,
+    1.11438674259589243e+00, 1.11740815156736928e+00, 1.12043775240960675e+00, 1.12347556733301990e+00, 1.12652161860824185e+00,
+    1.12957592856628808e+00, 1.13263851959871920e+00, 1.13570941415780546e+00, 1.13878863475669156e+00, 1.14187620396956158e+00,
+    1.14497214443180417e+00, 1.14807647884017894e+00, 1.15118922995298267e+00, 1.15431042059021594e+00, 1.15744007363375112e+00,
+    1.16057821202749878e+00, 1.16372485877757748e+00, 1.16688003695248166e+00, 1.17004376968325019e+00, 1.17321608016363732e+00,
+    1.17639699165028122e+00, 1.17958652746287584e+00, 1.18278471098434101e+00, 1.18599156566099384e+00, 1.18920711500272103e+00,
+    1.19243138258315118e+00, 1.19566439203982733e+00, 1.19890616707438058e+00, 1.20215673145270308e+00, 1.20541610900512386e+00,
+    1.20868432362658162e+00, 1.21196139927680124e+00, 1.21524735998046896e+00, 1.21854222982740845e+00, 1.22184603297275762e+00,
+    1.22515879363714553e+00, 1.22848053610687002e+00, 1.23181128473407586e+00, 1.23515106393693341e+00, 1.23849989819981654e+00,
+    1.24185781207348400e+00, 1.24522483017525798e+00, 1.24860097718920482e+00, 1.25198627786631622e+00, 1.25538075702469110e+00,
+    1.25878443954971653e+00, 1.26219735039425074e+00, 1.26561951457880628e+00, 1.26905095719173322e+00, 1.27249170338940276e+00,
+    1.27594177839639200e+00, 1.27940120750566932e+00, 1.28287001607877826e+00, 1.28634822954602557e+00, 1.28983587340666572e+00,
+    1.29333297322908947e+00, 1.29683955465100964e+00, 1.30035564337965059e+00, 1.30388126519193581e+00, 1.30741644593467732e+00,
+    1.31096121152476441e+00, 1.31451558794935464e+00, 1.31807960126606405e+00, 1.32165327760315754e+00, 1.32523664315974132e+00,
+    1.32882972420595435e+00, 1.33243254708316150e+00, 1.33604513820414583e+00, 1.33966752405330292e+00, 1.34329973118683532e+00,
+    1.34694178623294580e+00, 1.35059371589203447e+00, 1.35425554693689265e+00, 1.35792730621290114e+00, 1.36160902063822475e+00,
+    1.36530071720401192e+00, 1.36900242297459052e+00, 1.37271416508766841e+00, 1.37643597075453017e+00, 1.38016786726023799e+00,
+    1.38390988196383202e+00, 1.38766204229852907e+00, 1.39142437577192624e+00, 1.39519690996620027e+00, 1.39897967253831124e+00,
+    1.40277269122020476e+00, 1.40657599381901544e+00, 1.41038960821727066e+00, 1.41421356237309515e+00, 1.41804788432041518e+00,
+    1.42189260216916558e+00, 1.42574774410549421e+00, 1.42961333839197002e+00, 1.43348941336778890e+00, 1.43737599744898237e+00,
+    1.44127311912862566e+00, 1.44518080697704665e+00, 1.44909908964203504e+00, 1.45302799584905262e+00, 1.45696755440144377e+00,
+    1.46091779418064704e+00, 1.46487874414640573e+00, 1.46885043333698184e+00, 1.47283289086936753e+00, 1.47682614593949935e+00,
+    1.48083022782247187e+00, 1.48484516587275239e+00, 1.48887098952439700e+00, 1.49290772829126484e+00, 1.49695541176723546e+00,
+    1.50101406962642558e+00, 1.50508373162340647e+00, 1.50916442759342284e+00, 1.51325618745260981e+00, 1.51735904119821474e+00,
+    1.52147301890881459e+00, 1.52559815074453842e+00, 1.52973446694728699e+00, 1.53388199784095591e+00, 1.53804077383165683e+00,
+    1.54221082540794074e+00, 1.54639218314102145e+00, 1.55058487768499997e+00, 1.55478893977708865e+00, 1.55900440023783693e+00,
+    1.56323128997135763e+00, 1.56746963996555300e+00, 1.57171948129234140e+00, 1.57598084510788650e+00, 1.58025376265282458e+00,
+    1.58453826525249375e+00, 1.58883438431716395e+00, 1.59314215134226700e+00, 1.59746159790862707e+00, 1.60179275568269341e+00,
+    1.60613565641677103e+00, 1.61049033194925428e+00, 1.61485681420486071e+00, 1.61923513519486373e+00, 1.62362532701732887e+00,
+    1.62802742185734783e+00, 1.63244145198727497e+00, 1.63686744976696441e+00, 1.64130544764400632e+00, 1.64575547815396495e+00,
+    1.65021757392061774e+00, 1.65469176765619430e+00, 1.65917809216161616e+00, 1.66367658032673638e+00, 1.66818726513058246e+00,
+    1.67271017964159663e+00, 1.67724535701787847e+00, 1.68179283050742900e+00, 1.68635263344839337e+00, 1.69092479926930528e+00,
+    1.69550936148933262e+00, 1.70010635371852348e+00, 1.70471580965805125e+00, 1.70933776310046293e+00, 1.71397224792992597e+00,
+    1.71861929812247793e+00, 1.72327894774627399e+00, 1.72795123096183767e+00, 1.73263618202231107e+00, 1.73733383527370622e+00,
+    1.74204422515515644e+00, 1.74676738619916905e+00, 1.75150335303187821e+00, 1.75625216037329945e+00, 1.76101384303758390e+00,
+    1.76578843593327273e+00, 1.77057597406355471e+00, 1.77537649252652119e+00, 1.78019002651542446e+00, 1.78501661131893496e+00,
+    1.78985628232140104e+00, 1.79470907500310717e+00, 1.79957502494053512e+00, 1.80445416780662393e+00, 1.80934653937103196e+00,
+    1.81425217550039886e+00, 1.81917111215860849e+00, 1.82410338540705341e+00, 1.82904903140489727e+00, 1.83400808640934243e+00,
+    1.83898058677589371e+00, 1.84396656895862598e+00, 1.84896606951045084e+00, 1.85397912508338547e+00, 1.85900577242882048e+00,
+    1.86404604839778898e+00, 1.86909998994123860e+00, 1.87416763411029996e+00, 1.87924901805656019e+00, 1.88434417903233453e+00,
+    1.88945315439093919e+00, 1.89457598158696561e+00, 1.89971269817655530e+00, 1.90486334181767414e+00, 1.91002795027038985e+00,
+    1.91520656139714740e+00, 1.92039921316304740e+00, 1.92560594363612503e+00, 1.93082679098762711e+00, 1.93606179349229435e+00,
+    1.94131098952864045e+00, 1.94657441757923322e+00, 1.95185211623097832e+00, 1.95714412417540018e+00, 1.96245048020892732e+00,
+    1.96777122323317588e+00, 1.97310639225523432e+00, 1.97845602638795093e+00, 1.98382016485021939e+00, 1.98919884696726634e+00,
+    1.99459211217094023e+00,
 };
-// e^x for x <= 0: x = k ln 2 / 32 + r with k = 32 n + j the nearest, e^x = 2^n 2^(j / 32) e^r, |r| <= ln 2 / 64, where the series up to r^5 is
-// within 2.3e-15; ln 2 / 32 in two parts, of which k times the first (36 bits) is exact.  Below e^-700: zero.
-__device__ __forceinline__ double exp_down(double x, const double* powers) {
-  if (!(x > -700.0)) return x != x ? x : 0.0;
-  double k = fma(x, 4.61662413084468283841e+01, 6755399441055744.0);
+// 2^y for y <= 0: with k = 256 n + j the integer nearest to 256 y and r = y - k / 256 (exact, |r| <= 2^-9), 2^y = 2^n 2^(j / 256) 2^r, where the
+// series up to r^3 is within 2.3e-15.  Below 2^-1000: zero.  (Nine operations in 64 bits, at 5 to 6 cycles a warp what such a pass
+// is made of; powers of 1/32 and the series up to r^5 took thirteen.)
+__device__ __forceinline__ double exp2_down(double y, const double* powers) {
+  double k = fma(y, 256.0, 6755399441055744.0);
   const int n = __double2loint(k);
   k -= 6755399441055744.0;
-  double r = fma(k, -2.16608493924468348268e-02, x);
-  r = fma(k, -5.14560924465533821524e-14, r);
-  double q = fma(r, 1.0 / 120.0, 1.0 / 24.0);
-  q = fma(q, r, 1.0 / 6.0);
-  q = fma(q, r, 0.5);
-  q = fma(q * r, r, r);
-  const double t = powers[n & 31], y = fma(t, q, t);
-  return __hiloint2double(__double2hiint(y) + ((n >> 5) << 20), __double2loint(y));
+  const double r = fma(k, -1.0 / 256.0, y);
+  double q = fma(r, 5.55041086648215831e-02, 2.40226506959100722e-01);
+  q = fma(q, r, 6.93147180559945286e-01);
+  const double t = powers[n & 255], v = fma(t, q * r, t);
+  return y > -1000.0 ? __hiloint2double(__double2hiint(v) + ((n >> 8) << 20), __double2loint(v)) : y != y ? y : 0.0;
 }
 
 __device__ __forceinline__ uint32_t draw_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -104,26 +145,24 @@ __device__ __forceinline__ double warp_sum64(double v) {
   return v;
 }
 
-constexpr int kSums = 8;
 struct DrawShared {
-  double powers[32];
-  double parts[kDrawWarps][kSums];  // the warps' sums
-  double sums[2][kSums];            // the CTA's, for the cluster: in turns, so that one barrier a pass is enough
+  double powers[256];
+  double parts[kDrawWarps][4];  // the warps' sums
+  int counts[kDrawWarps][4];
+  double sums[2][8];            // the CTA's, for the cluster: in turns, so that one barrier a pass is enough
   double listed_mass[kListed];
   uint32_t listed[kListed];
-  double result[kSums];             // the cluster's
-  uint32_t own_key[2];              // the CTA's largest and smallest key
+  double result[8];             // the cluster's
+  uint32_t own_key[2];          // the CTA's largest and smallest key
   int own_index[2];
   uint32_t keys[kDrawWarps], low_keys[kDrawWarps];
-  int found, first;
+  int found, first, crossing;
 };
 
 template <int N>
 struct SumCount {
   static constexpr int value = N;
 };
-using Sums1 = SumCount<1>;
-using Sums8 = SumCount<8>;
 
 template <bool STAGED>
 __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_constant__ DrawParams p) {
@@ -142,10 +181,11 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
   }
   const int chunk = p.run * kDrawThreads, c0 = min(V, rank * chunk), n_here = min(V - c0, chunk);  // (rank * chunk < 2^31: the host checks)
   const float* x = p.logits + (size_t)row * p.stride + c0;
-  if (tid < 32) sh.powers[tid] = kPowers[tid];
+  if (tid < 256) sh.powers[tid] = kPowers[tid];
   if (tid == 0) {
     sh.found = 0x7fffffff;
     sh.first = 0x7fffffff;
+    sh.crossing = 0x7fffffff;
   }
   // ---- the chunk comes in; its largest logit
   uint32_t top_key = 0u, low_key = 0xffffffffu;  // the largest logit, and the smallest above -infinity
@@ -159,15 +199,15 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
     if ((((uintptr_t)x) & 15) == 0) {
       const float4* x4 = reinterpret_cast<const float4*>(x);
       const int n4 = n_here >> 2;
-      for (int i0 = 0; i0 < n4; i0 += 4 * kDrawThreads) {
-        float4 v[4];
+      for (int i0 = 0; i0 < n4; i0 += 7 * kDrawThreads) {
+        float4 v[7];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 7; ++e) {
           const int i = i0 + e * kDrawThreads + tid;
           if (i < n4) v[e] = __ldg(x4 + i);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 7; ++e) {
           const int i = i0 + e * kDrawThreads + tid;
           if (i < n4) {
             if (STAGED) *reinterpret_cast<uint4*>(staged + 4 * i) = make_uint4(note(v[e].x), note(v[e].y), note(v[e].z), note(v[e].w));
@@ -220,39 +260,59 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
   const float top = of_key(top_key), t = p.temperature[draw];
   const int i0 = min(n_here, tid * p.run), i1 = min(n_here, i0 + p.run);
   auto at = [&](int i) -> uint32_t { return STAGED ? staged[i] : order_key(clean(__ldg(x + i))); };
-  int turn = 0;
-  // N sums over the cluster, the same in every thread
-  auto cluster_sums = [&](auto nc, double (&v)[kSums]) {
-    constexpr int N = decltype(nc)::value;
+  // four keys of the run at a time (0 behind its end), so that four exponentials are under way at once
+  auto four = [&](int i, uint32_t (&k)[4]) {
 #pragma unroll
-    for (int s = 0; s < N; ++s) {
-      v[s] = warp_sum64(v[s]);
-      if (lane == 0) sh.parts[warp][s] = v[s];
+    for (int e = 0; e < 4; ++e) k[e] = i + e < i1 ? at(i + e) : 0u;
+  };
+  int turn = 0;
+  // Sums over the cluster, the same in every thread: NM of 64-bit numbers and NC of integers.
+  auto cluster_sums = [&](auto masses, auto counts, double (&m)[4], int (&n)[4]) {
+    constexpr int NM = decltype(masses)::value, NC = decltype(counts)::value;
+#pragma unroll
+    for (int s = 0; s < NM; ++s) {
+      const double v = warp_sum64(m[s]);
+      if (lane == 0) sh.parts[warp][s] = v;
+    }
+#pragma unroll
+    for (int s = 0; s < NC; ++s) {
+      const int v = __reduce_add_sync(0xffffffffu, n[s]);
+      if (lane == 0) sh.counts[warp][s] = v;
     }
     __syncthreads();
-    if (tid < N) {
-      double sum = 0.0;
+    if (warp == 0) {
+      if (lane < NM) {
+        double sum = 0.0;
 #pragma unroll
-      for (int w = 0; w < kDrawWarps; ++w) sum += sh.parts[w][tid];
-      sh.sums[turn][tid] = sum;
+        for (int w = 0; w < kDrawWarps; ++w) sum += sh.parts[w][lane];
+        sh.sums[turn][lane] = sum;
+      } else if (lane >= 4 && lane < 4 + NC) {
+        int sum = 0;
+#pragma unroll
+        for (int w = 0; w < kDrawWarps; ++w) sum += sh.counts[w][lane - 4];
+        sh.sums[turn][lane] = sum;
+      }
     }
-    if (C > 1) draw_barrier(); else __syncthreads();
     if (C > 1) {
+      draw_barrier();
       if (warp == 0) {  // lane 8 c + s: sums s of CTAs c and c + 4
         const int s = lane & 7, c = lane >> 3;
         double sum = 0.0;
-        if (s < N) {
+        if (s < NM || (s >= 4 && s < 4 + NC)) {
           if (c < C) sum = remote_f64(draw_remote(&sh.sums[turn][s], c));
           if (c + 4 < C) sum += remote_f64(draw_remote(&sh.sums[turn][s], c + 4));
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 8);
         sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-        if (lane < N) sh.result[lane] = sum;
+        if (lane < 8) sh.result[lane] = sum;
       }
-      __syncthreads();
     }
+    __syncthreads();
+    const double* from = C > 1 ? sh.result : sh.sums[turn];
 #pragma unroll
-    for (int s = 0; s < N; ++s) v[s] = C > 1 ? sh.result[s] : sh.sums[turn][s];
+    for (int s = 0; s < NM; ++s) m[s] = from[s];
+#pragma unroll
+    for (int s = 0; s < NC; ++s) n[s] = (int)from[4 + s];
     turn ^= 1;
   };
   int token = 0;
@@ -274,15 +334,18 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
         token = sh.first;
       }
     } else {
-      const double inv_t = 1.0 / (double)t;
-      auto mass_of = [&](uint32_t k) -> double { return k == top_key ? 1.0 : exp_down(((double)of_key(k) - (double)top) * inv_t, sh.powers); };
+      const double inv_t = 1.0 / (double)t, per_bit = inv_t * 1.4426950408889634074;  // z / ln 2 of a logit's distance
+      auto mass_of = [&](uint32_t k) -> double {
+        const double m = exp2_down(((double)of_key(k) - (double)top) * per_bit, sh.powers);
+        return k == top_key ? 1.0 : m;
+      };
       double whole = -1.0;  // the mass of the whole row at this temperature, where it was summed up
       // The largest key from `lo` on at which the number (by_mass: the mass) of the logits that reach it is `need` (by_mass: `need` of what
       // reaches `lo`) or more; `lo` where not even that has as many.
       auto search = [&](bool by_mass, uint32_t lo, double need) -> uint32_t {
         uint32_t hi = top_key;
         double above = 0.0;    // of the logits above `hi`
-        double inside = 1e30;  // logits between
+        int inside = V, mine = 0;  // logits between, and this thread's of them
         bool by_key = false;
         for (int pass = 0; (lo < hi && inside > kListed) || pass == 0; ++pass) {
           // Three candidates between: by value, as logits spread like their values do (close below the largest where some lie far away, masked
@@ -300,32 +363,39 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
           q1 = min(max(q1, lo + 1u), max(hi, lo + 1u));
           q2 = min(max(q2, q1), max(hi, lo + 1u));
           q3 = min(max(q3, q2), max(hi, lo + 1u));
-          double v[kSums] = {};
-          int n0 = 0, n1 = 0, n2 = 0, n3 = 0;  // logits that reach lo, q1, q2, q3, and no more than hi
-          if (by_mass) {
-            for (int i = i0; i < i1; ++i) {
-              const uint32_t k = at(i);
-              if (k < lo || k > hi) continue;
-              const double e = mass_of(k);
-              ++n0;
-              v[0] += e;
-              if (k >= q1) { ++n1; v[1] += e; }
-              if (k >= q2) { ++n2; v[2] += e; }
-              if (k >= q3) { ++n3; v[3] += e; }
+          double v[4] = {0.0, 0.0, 0.0, 0.0};  // mass (or number) and number of the logits that reach lo, q1, q2, q3, and no more than hi
+          int n[4] = {0, 0, 0, 0};
+          for (int i = i0; i < i1; i += 4) {
+            uint32_t k[4];
+            four(i, k);
+            bool some = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (k[e] > hi) k[e] = 0u;
+              n[0] += k[e] >= lo;
+              n[1] += k[e] >= q1;
+              n[2] += k[e] >= q2;
+              n[3] += k[e] >= q3;
+              some |= k[e] >= lo;
             }
-          } else {
-#pragma unroll 4
-            for (int i = i0; i < i1; ++i) {
-              const uint32_t k = at(i) <= hi ? at(i) : 0u;
-              n0 += k >= lo;
-              n1 += k >= q1;
-              n2 += k >= q2;
-              n3 += k >= q3;
+            if (by_mass && some) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const double m = mass_of(k[e]);
+                v[0] += k[e] >= lo ? m : 0.0;
+                v[1] += k[e] >= q1 ? m : 0.0;
+                v[2] += k[e] >= q2 ? m : 0.0;
+                v[3] += k[e] >= q3 ? m : 0.0;
+              }
             }
-            v[0] = n0; v[1] = n1; v[2] = n2; v[3] = n3;
           }
-          v[4] = n0; v[5] = n1; v[6] = n2; v[7] = n3;
-          cluster_sums(Sums8(), v);
+          const int own0 = n[0], own1 = n[1], own2 = n[2], own3 = n[3];  // this thread's
+          if (by_mass) {
+            cluster_sums(SumCount<4>(), SumCount<4>(), v, n);
+          } else {
+            cluster_sums(SumCount<0>(), SumCount<4>(), v, n);
+            v[0] = n[0]; v[1] = n[1]; v[2] = n[2]; v[3] = n[3];
+          }
           if (pass == 0) {
             if (by_mass) {
               if (lo == low_key) whole = v[0];
@@ -337,18 +407,13 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
             if (lo >= hi) return lo;
           }
           by_key = false;
-          if (above + v[3] >= need) { lo = q3; inside = v[7]; }
-          else if (above + v[2] >= need) { above += v[3]; lo = q2; hi = q3 - 1u; inside = v[6] - v[7]; }
-          else if (above + v[1] >= need) { above += v[2]; lo = q1; hi = q2 - 1u; inside = v[5] - v[6]; }
-          else { above += v[1]; hi = q1 - 1u; inside = v[4] - v[5]; by_key = wide; }
+          if (above + v[3] >= need) { lo = q3; inside = n[3]; mine = own3; }
+          else if (above + v[2] >= need) { above += v[3]; lo = q2; hi = q3 - 1u; inside = n[2] - n[3]; mine = own2 - own3; }
+          else if (above + v[1] >= need) { above += v[2]; lo = q1; hi = q2 - 1u; inside = n[1] - n[2]; mine = own1 - own2; }
+          else { above += v[1]; hi = q1 - 1u; inside = n[0] - n[1]; by_key = wide; mine = own0 - own1; }
         }
         if (lo >= hi) return lo;
         // the few between, in the order of their indices, by every CTA
-        int mine = 0;
-        for (int i = i0; i < i1; ++i) {
-          const uint32_t k = at(i);
-          mine += k >= lo && k <= hi;
-        }
         int before = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -363,12 +428,16 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
           all += sh.keys[w];
         }
         int to = base + before - mine;
-        for (int i = i0; i < i1 && mine > 0; ++i) {
-          const uint32_t k = at(i);
-          if (k < lo || k > hi) continue;
-          sh.listed[to] = k;
-          sh.listed_mass[to] = by_mass ? mass_of(k) : 1.0;
-          ++to;
+        const int full = base + before;
+        for (int i = i0; to < full; i += 4) {
+          uint32_t k[4];
+          four(i, k);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (k[e] >= lo && k[e] <= hi) {
+              sh.listed[to] = k[e];
+              sh.listed_mass[to++] = by_mass ? mass_of(k[e]) : 1.0;
+            }
         }
         if (tid == 0) sh.own_index[0] = all;
         if (C > 1) draw_barrier(); else __syncthreads();
@@ -417,19 +486,23 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
         if (near > 4u) quick = max(quick, near - 4u);
       }
       auto kept = [&](uint32_t k) -> double {
-        if (k < quick) return 0.0;
-        if (k == top_key) return 1.0;
-        const double z = ((double)of_key(k) - (double)top) * inv_t;
-        return z >= least ? exp_down(z, sh.powers) : 0.0;
+        const double d = (double)of_key(k) - (double)top, m = exp2_down(d * per_bit, sh.powers);
+        return k == top_key ? 1.0 : k >= quick && d * inv_t >= least ? m : 0.0;
       };
       // the thread's run, then the running mass behind every thread's run
       double c = 0.0;
       int newest = -1;
-      for (int i = i0; i < i1; ++i) {
-        const double e = kept(at(i));
-        if (e > 0.0) {
-          c += e;
-          newest = i;
+      for (int i = i0; i < i1; i += 4) {
+        uint32_t k[4];
+        four(i, k);
+        if (max(max(k[0], k[1]), max(k[2], k[3])) < quick) continue;
+        double m[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m[e] = kept(k[e]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          c += m[e];
+          if (m[e] > 0.0) newest = i + e;
         }
       }
       double behind = c;
@@ -454,37 +527,64 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
         sh.own_index[1] = newest < 0 ? -1 : c0 + newest;
       }
       if (C > 1) draw_barrier(); else __syncthreads();
-      double total = 0.0, here = 0.0;
-      int last = -1;
-      for (int r = 0; r < C; ++r) {
-        if (r == rank) here = total;
-        total += C > 1 ? remote_f64(draw_remote(&sh.sums[turn][0], r)) : all;
-        last = max(last, C > 1 ? (int)remote_u32(draw_remote(&sh.own_index[1], r)) : newest);
+      if (warp == 0) {
+        double theirs = 0.0;
+        int newest_there = -1;
+        if (lane < C) {
+          theirs = C > 1 ? remote_f64(draw_remote(&sh.sums[turn][0], lane)) : all;
+          newest_there = C > 1 ? (int)remote_u32(draw_remote(&sh.own_index[1], lane)) : newest < 0 ? -1 : c0 + newest;
+        }
+        double total = 0.0, here = 0.0;
+        for (int r = 0; r < C; ++r) {
+          if (r == rank) here = total;
+          total += __shfl_sync(0xffffffffu, theirs, r);
+        }
+        newest_there = __reduce_max_sync(0xffffffffu, newest_there);
+        if (lane == 0) {
+          sh.result[0] = total;
+          sh.result[1] = here;
+          sh.result[2] = newest_there;
+        }
       }
+      __syncthreads();
+      const double total = sh.result[0], here = sh.result[1];
+      const int last = (int)sh.result[2];
       turn ^= 1;
       if (quick == low_key && !(mp > 0.f)) whole = total;
       whole = t == 1.f ? whole : -1.0;
       whole_row = whole;
       const double target = (double)p.u[draw] * total;
-      const double start = here + front + (behind - c);
-      // (the first thread whose run's end passes the target; what rounding leaves between a run's end and the next one's start goes to the next)
-      if (c > 0.0 && here + front + behind > target) {
-        double run = start;
-        for (int i = i0; i < i1; ++i) {
-          const double e = kept(at(i));
-          run += e;
-          if (e > 0.0 && run > target) {
-            atomicMin(&sh.found, c0 + i);
+      // the first thread whose run's end passes the target; its warp takes the run, a lane a logit
+      if (c > 0.0 && here + front + behind > target) atomicMin(&sh.crossing, tid);
+      __syncthreads();
+      const int crossing = sh.crossing;
+      if (crossing >> 5 == warp) {
+        double run = __shfl_sync(0xffffffffu, here + front + (behind - c), crossing & 31);
+        const int end = min(n_here, (crossing + 1) * p.run);
+        int token_here = -1;
+        for (int j0 = min(n_here, crossing * p.run); j0 < end; j0 += 32) {
+          const int i = j0 + lane;
+          const double m = i < end ? kept(at(i)) : 0.0;
+          double sum = m;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const double other = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += other;
+          }
+          const unsigned past = __ballot_sync(0xffffffffu, m > 0.0 && run + sum > target), some = __ballot_sync(0xffffffffu, m > 0.0);
+          if (past) {
+            token_here = j0 + __ffs((int)past) - 1;
             break;
           }
+          if (some) token_here = j0 + 31 - __clz((int)some);  // (its last kept one, should rounding have it)
+          run += __shfl_sync(0xffffffffu, sum, 31);
         }
+        if (lane == 0) sh.found = c0 + token_here;
       }
       __syncthreads();
       if (C > 1) {
-        draw_barrier();
-        int lowest = 0x7fffffff;
-        for (int r = 0; r < C; ++r) lowest = min(lowest, (int)remote_u32(draw_remote(&sh.found, r)));
-        token = lowest;
+        draw_barrier();  // (the first warp of the first CTA writes the answer)
+        token = (int)__reduce_min_sync(0xffffffffu, warp == 0 && rank == 0 && lane < C ? remote_u32(draw_remote(&sh.found, lane)) : 0x7fffffffu);
       } else {
         token = sh.found;
       }
@@ -492,21 +592,22 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
     }
   }
   if (p.logprobs) {
-    // likely logits in 64 bits, the many others (below e^-8 of the largest) in 32: their errors are random and small against the sum
-    double v[kSums] = {};
+    // In 32 bits: an exponential is within 2^-22.5 (and its argument's rounding), the errors of many are random.
+    double v[4] = {whole_row, 0.0, 0.0, 0.0};
     if (top_key != 0u && whole_row < 0.0) {
-      float rest = 0.f;
-      for (int i = i0; i < i1; ++i) {
-        const uint32_t k = at(i);
-        const float xi = of_key(k), d = xi - top;
-        if (k == top_key) v[0] += 1.0;
-        else if (d > -8.f) v[0] += exp_down((double)xi - (double)top, sh.powers);
-        else rest += __expf(d);
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int i = i0; i < i1; i += 4) {
+        uint32_t k[4];
+        four(i, k);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float d = k[e] == top_key ? 0.f : of_key(k[e]) - top;
+          sum[e] += __expf(d);
+        }
       }
-      v[0] += (double)rest;
-      cluster_sums(Sums1(), v);
-    } else {
-      v[0] = whole_row;
+      int n[4];
+      v[0] = (double)(sum[0] + sum[1]) + (double)(sum[2] + sum[3]);
+      cluster_sums(SumCount<1>(), SumCount<0>(), v, n);
     }
     if (rank == 0 && tid == 0) {
       const float xt = clean(p.logits[(size_t)row * p.stride + token]);
