@@ -11,7 +11,7 @@
 // Masses are sums of 64-bit numbers: with 200,000 tokens of like probability the borders between tokens lie 5e-6 of the mass apart and
 // sums in 32 bits are 1e-6 off, so that every few draws would name a neighbour.  Sums are taken in a fixed order.
 //
-// A cluster of up to eight CTAs takes a draw: a thread has a run of neighbouring logits, kept in shared memory from the one pass over
+// A cluster of up to sixteen CTAs takes a draw: a thread has a run of neighbouring logits, kept in shared memory from the one pass over
 // memory.  A threshold is searched for by the number or the mass of the logits above it, with three candidates a pass; a logit's
 // exponential is taken only where it lies between the last candidates, and when at most kListed logits do, each of them is tried.
 // What bounds it: for one draw the passes one after the other (a barrier of the cluster and a trip through its shared memory each, about
@@ -120,6 +120,11 @@ __device__ __forceinline__ double exp2_down(double y, const double* powers) {
   return y > -1000.0 ? __hiloint2double(__double2hiint(v) + ((n >> 8) << 20), __double2loint(v)) : y != y ? y : 0.0;
 }
 
+__device__ __forceinline__ float exp2f_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ uint32_t draw_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ uint32_t draw_remote(const void* p, int rank) {
   uint32_t r;
@@ -295,13 +300,11 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
     }
     if (C > 1) {
       draw_barrier();
-      if (warp == 0) {  // lane 8 c + s: sums s of CTAs c and c + 4
-        const int s = lane & 7, c = lane >> 3;
+      if (warp == 0) {  // lane 8 c + s: sums s of CTAs c, c + 4, ...
+        const int s = lane & 7;
         double sum = 0.0;
-        if (s < NM || (s >= 4 && s < 4 + NC)) {
-          if (c < C) sum = remote_f64(draw_remote(&sh.sums[turn][s], c));
-          if (c + 4 < C) sum += remote_f64(draw_remote(&sh.sums[turn][s], c + 4));
-        }
+        if (s < NM || (s >= 4 && s < 4 + NC))
+          for (int c = lane >> 3; c < C; c += 4) sum += remote_f64(draw_remote(&sh.sums[turn][s], c));
         sum += __shfl_xor_sync(0xffffffffu, sum, 8);
         sum += __shfl_xor_sync(0xffffffffu, sum, 16);
         if (lane < 8) sh.result[lane] = sum;
@@ -339,30 +342,138 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
         const double m = exp2_down(((double)of_key(k) - (double)top) * per_bit, sh.powers);
         return k == top_key ? 1.0 : m;
       };
+      int held_by_k = V;  // logits that top-k left
       double whole = -1.0;  // the mass of the whole row at this temperature, where it was summed up
+      // Three candidates between: by value, as logits spread like their values do: close below the largest where some lie far away (masked
+      // ones, say: true is returned then), in quarters, or, in a narrow range, around the place that `part` of what it holds lies above; or by
+      // key, which ends whatever they are.
+      auto candidates = [&](uint32_t lo, uint32_t hi, bool by_key, double part, uint32_t& q1, uint32_t& q2, uint32_t& q3) -> bool {
+        const uint32_t gap = hi - lo;
+        const float a = of_key(lo), b = of_key(hi);
+        q1 = lo + gap / 4u + (gap < 4u), q2 = lo + gap / 2u + (gap & 1u), q3 = hi - gap / 4u;
+        const bool wide = !(b - a <= 64.f * t);
+        if (!by_key && b < INFINITY) {
+          q1 = order_key(clean(wide ? b - 30.f * t : a + 0.25f * (b - a)));
+          q2 = order_key(clean(wide ? b - 10.f * t : a + 0.5f * (b - a)));
+          q3 = order_key(clean(wide ? b - 4.f * t : a + 0.75f * (b - a)));
+          if (!wide && part >= 0.0 && b - a <= 8.f * t) {
+            const float guess = b - (float)part * (b - a), off = 0.06f * (b - a);
+            q1 = order_key(clean(guess - off));
+            q2 = order_key(clean(guess));
+            q3 = order_key(clean(guess + off));
+          }
+        }
+        q1 = min(max(q1, lo + 1u), max(hi, lo + 1u));
+        q2 = min(max(q2, q1), max(hi, lo + 1u));
+        q3 = min(max(q3, q2), max(hi, lo + 1u));
+        return wide;
+      };
       // The largest key from `lo` on at which the number (by_mass: the mass) of the logits that reach it is `need` (by_mass: `need` of what
       // reaches `lo`) or more; `lo` where not even that has as many.
       auto search = [&](bool by_mass, uint32_t lo, double need) -> uint32_t {
         uint32_t hi = top_key;
         double above = 0.0;    // of the logits above `hi`
-        int inside = V, mine = 0;  // logits between, and this thread's of them
+        int inside = held_by_k, mine = 0;  // logits between, and this thread's of them
         bool by_key = false;
-        for (int pass = 0; (lo < hi && inside > kListed) || pass == 0; ++pass) {
-          // Three candidates between: by value, as logits spread like their values do (close below the largest where some lie far away, masked
-          // ones say); by key, which ends whatever they are, where the part far away was the one, and every third time.
-          uint32_t q1, q2, q3;
-          const uint32_t gap = hi - lo;
-          const float a = of_key(lo), b = of_key(hi);
-          q1 = lo + gap / 4u + (gap < 4u), q2 = lo + gap / 2u + (gap & 1u), q3 = hi - gap / 4u;
-          const bool wide = !(b - a <= 64.f * t);
-          if (!by_key && pass % 3 != 2 && b < INFINITY) {
-            q1 = order_key(clean(wide ? b - 30.f * t : a + 0.25f * (b - a)));
-            q2 = order_key(clean(wide ? b - 10.f * t : a + 0.5f * (b - a)));
-            q3 = order_key(clean(wide ? b - 4.f * t : a + 0.75f * (b - a)));
+        double part = -1.0;  // of what is between, how much lies above the place that is searched for, about
+        int pass = 0;
+        if (by_mass) {
+          // In 32 bits first, down to where the sums' roundings (2^-16 of them is more than those make) leave it open; then one pass in 64 bits
+          // over everything, which finds the mass and confirms the place.  (Each pass over everything in 64 bits is 12 us, in 32 bits 3.)
+          const uint32_t limit = lo;
+          const float per_bit32 = (float)per_bit;
+          double reach = 0.0, need32 = 0.0, held = 0.0;  // mass of all, what is wanted of it, mass between
+          for (int p32 = 0; p32 < 12 && lo < hi && inside > kListed / 2; ++p32) {
+            uint32_t q1, q2, q3;
+            const bool wide = candidates(lo, hi, by_key || p32 % 4 == 3, part, q1, q2, q3);
+            float f[4] = {0.f, 0.f, 0.f, 0.f};
+            int n[4] = {0, 0, 0, 0};
+            for (int i = i0; i < i1; i += 4) {
+              uint32_t k[4];
+              four(i, k);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if (k[e] > hi) k[e] = 0u;
+                const float m = k[e] == top_key ? 1.f : exp2f_fast((of_key(k[e]) - top) * per_bit32);
+                if (p32 == 0) f[0] += k[e] >= lo ? m : 0.f;
+                if (k[e] >= q1) { ++n[1]; f[1] += m; }
+                if (k[e] >= q2) { ++n[2]; f[2] += m; }
+                if (k[e] >= q3) { ++n[3]; f[3] += m; }
+              }
+            }
+            double v[4] = {f[0], f[1], f[2], f[3]};
+            cluster_sums(SumCount<4>(), SumCount<4>(), v, n);
+            if (p32 == 0) {
+              reach = v[0];
+              need32 = need * reach;
+            } else {
+              v[0] = held;
+            }
+            n[0] = inside;
+            const uint32_t q[4] = {lo, q1, q2, q3};
+            const double open = reach * (1.0 / 65536.0);
+            int a = 0, b = 4;  // the last candidate that is reached for sure, the first that is not
+#pragma unroll
+            for (int s = 1; s < 4; ++s)
+              if (above + v[s] >= need32 + open) a = s;
+#pragma unroll
+            for (int s = 3; s > 0; --s)
+              if (above + v[s] <= need32 - open) b = s;
+            if (a == 0 && b == 4) break;
+            by_key = a == 0 && wide;
+            int below = n[0], beyond = 0;
+#pragma unroll
+            for (int s = 1; s < 4; ++s) {
+              if (s == a) { lo = q[s]; below = n[s]; }
+              if (s == b) { hi = q[s] - 1u; beyond = n[s]; }
+            }
+            inside = below - beyond;
+            double more = 0.0;
+            held = v[0];
+#pragma unroll
+            for (int s = 1; s < 4; ++s) {
+              if (s == a) held = v[s];
+              if (s == b) more = v[s];
+            }
+            above += more;
+            held -= more;
+            part = (need32 - above) / fmax(held, 1e-300);
           }
-          q1 = min(max(q1, lo + 1u), max(hi, lo + 1u));
-          q2 = min(max(q2, q1), max(hi, lo + 1u));
-          q3 = min(max(q3, q2), max(hi, lo + 1u));
+          double v[4] = {0.0, 0.0, 0.0, 0.0};  // what reaches `limit`, `lo`, and what is above `hi`
+          int n[4] = {0, 0, 0, 0};
+          for (int i = i0; i < i1; i += 4) {
+            uint32_t k[4];
+            four(i, k);
+            if (max(max(k[0], k[1]), max(k[2], k[3])) < limit) continue;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const double m = k[e] >= limit ? mass_of(k[e]) : 0.0;
+              v[0] += m;
+              v[1] += k[e] >= lo ? m : 0.0;
+              v[2] += k[e] > hi ? m : 0.0;
+              n[0] += k[e] >= lo && k[e] <= hi;
+            }
+          }
+          mine = n[0];
+          cluster_sums(SumCount<3>(), SumCount<1>(), v, n);
+          if (limit == low_key) whole = v[0];
+          need *= v[0];
+          if (!(need > 0.0)) return top_key;
+          above = v[2];
+          inside = n[0];
+          if (!(v[1] >= need && v[2] < need)) {  // (not the place after all)
+            lo = limit;
+            hi = top_key;
+            above = 0.0;
+            inside = V;
+          }
+          by_key = false;
+          part = -1.0;
+          pass = 1;
+        }
+        for (; (lo < hi && inside > kListed) || pass == 0; ++pass) {
+          uint32_t q1, q2, q3;
+          const bool wide = candidates(lo, hi, by_key || pass % 3 == 2, part, q1, q2, q3);
           double v[4] = {0.0, 0.0, 0.0, 0.0};  // mass (or number) and number of the logits that reach lo, q1, q2, q3, and no more than hi
           int n[4] = {0, 0, 0, 0};
           for (int i = i0; i < i1; i += 4) {
@@ -397,20 +508,16 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
             v[0] = n[0]; v[1] = n[1]; v[2] = n[2]; v[3] = n[3];
           }
           if (pass == 0) {
-            if (by_mass) {
-              if (lo == low_key) whole = v[0];
-              need *= v[0];
-              if (!(need > 0.0)) return top_key;
-            } else if (v[0] < need) {
-              return lo;
-            }
+            if (v[0] < need) return lo;
             if (lo >= hi) return lo;
           }
           by_key = false;
-          if (above + v[3] >= need) { lo = q3; inside = n[3]; mine = own3; }
-          else if (above + v[2] >= need) { above += v[3]; lo = q2; hi = q3 - 1u; inside = n[2] - n[3]; mine = own2 - own3; }
-          else if (above + v[1] >= need) { above += v[2]; lo = q1; hi = q2 - 1u; inside = n[1] - n[2]; mine = own1 - own2; }
+          double held = v[0] - v[1];
+          if (above + v[3] >= need) { lo = q3; inside = n[3]; mine = own3; held = v[3]; }
+          else if (above + v[2] >= need) { above += v[3]; lo = q2; hi = q3 - 1u; inside = n[2] - n[3]; mine = own2 - own3; held = v[2] - v[3]; }
+          else if (above + v[1] >= need) { above += v[2]; lo = q1; hi = q2 - 1u; inside = n[1] - n[2]; mine = own1 - own2; held = v[1] - v[2]; }
           else { above += v[1]; hi = q1 - 1u; inside = n[0] - n[1]; by_key = wide; mine = own0 - own1; }
+          if (by_mass) part = (need - above) / fmax(held, 1e-300);  // (a tail's numbers fall off too fast for that)
         }
         if (lo >= hi) return lo;
         // the few between, in the order of their indices, by every CTA
@@ -475,7 +582,10 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
       };
       uint32_t limit = low_key;  // (key 0 is never drawn)
       const int k = p.top_k[draw];
-      if (k > 0 && k < V) limit = search(false, limit, (double)k);
+      if (k > 0 && k < V) {
+        limit = search(false, limit, (double)k);
+        held_by_k = k;  // (about: ties stay)
+      }
       const float tp = p.top_p[draw];
       if (tp < 1.f) limit = search(true, limit, fmax((double)tp, 0.0));
       const float mp = p.min_p[draw];
@@ -631,13 +741,15 @@ extern "C" int ftk_sample_draws(const float* logits, long long row_stride, int n
   FTK_REQUIRE(rows || n_draws <= n_rows, "sample_draws: %d draws from %d rows", n_draws, n_rows);
   FTK_REQUIRE(n_draws <= (1 << 24), "sample_draws: %d draws", n_draws);
   DrawParams p{logits, row_stride, n_rows, vocab, rows, temperature, top_k, top_p, min_p, u, out, logprobs, 1, 1};
-  // a CTA for every 4,096 logits, eight at most
-  while (p.cluster < 8 && vocab > p.cluster * 4096) p.cluster *= 2;
+  // a CTA for every 4,096 logits, eight at most; sixteen where that leaves SMs idle
+  while (p.cluster < (n_draws <= 8 ? 16 : 8) && vocab > p.cluster * 4096) p.cluster *= 2;
   p.run = ((vocab + p.cluster * kDrawThreads - 1) / (p.cluster * kDrawThreads)) | 1;
   const bool held = p.run <= kMostRun;  // (430,000 logits; longer rows are read again in every pass)
   const size_t smem = held ? (size_t)p.run * kDrawThreads * sizeof(float) : 0;
   auto kern = held ? draw_kernel<true> : draw_kernel<false>;
-  FTK_REQUIRE(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess, "sample_draws: cannot set up the kernel");
+  FTK_REQUIRE(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess &&
+                  (p.cluster <= 8 || cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess),
+              "sample_draws: cannot set up the kernel");
   note_variant(held ? "draws: rows in shared memory" : "draws: rows read again in every pass");
   const dim3 grid((unsigned)(n_draws * p.cluster));
   if (p.cluster > 1) launch_kernel_clusters(kern, p.cluster, grid, dim3(kDrawThreads), smem, (cudaStream_t)stream, p);
