@@ -15,7 +15,7 @@ its sizes while the requests grow.  The reference reads shared pages once per re
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -40,6 +40,12 @@ ROWS_KEYS = {torch.bfloat16: 64, torch.float32: 32}  # keys the kernels for few 
 Span = Tuple[Sequence[int], int, int]  # members (indices of requests), first position, one past the last
 
 
+def _rounded(n: int) -> int:
+    """``n`` up to a power of two or three halves of one."""
+    top = 1 << (n - 1).bit_length() if n else 0
+    return top // 4 * 3 if top >= 4 and n <= top // 4 * 3 else top
+
+
 @dataclass
 class SharedPlan:
     """int32 arrays of one step's shared and own keys, and what the launch needs beside them."""
@@ -60,6 +66,16 @@ class SharedPlan:
     def key(self) -> Tuple[int, ...]:
         """What a recorded step's launches depend on."""
         return (self.items.shape[0], self.members.shape[0], self.requests.shape[0], self.joins.shape[0], self.n_slots, self.tile_rows, self.cluster, self.own_tiles)
+
+    def rounded(self) -> "SharedPlan":
+        """The same work in lists of few sizes (two to an octave), so that few launches have to be recorded: items behind the last have no
+        members, which makes them no pieces, and nobody points to other entries behind the last."""
+        def room(arr: np.ndarray) -> np.ndarray:
+            out = np.zeros((_rounded(arr.shape[0]), *arr.shape[1:]), dtype=arr.dtype)
+            out[:arr.shape[0]] = arr
+            return out
+
+        return replace(self, items=room(self.items), members=room(self.members), joins=room(self.joins), n_slots=_rounded(self.n_slots))
 
     def sections(self) -> List[Tuple[str, np.ndarray]]:
         return [("items", self.items), ("members", self.members), ("requests", self.requests), ("joins", self.joins)]

@@ -241,6 +241,8 @@ class StepBuilder:
                                           self.table_rows, self.sm_count))
             self.engine.shared_layouts[what] = known
         plan = known[1].plan(self._segments[:, 1])
+        if self.fixed:
+            plan = plan.rounded()
         key = self._shared[what] = ("shared_attention", *what, *plan.key())
         self.plans[key] = plan
         for name, arr in plan.sections():
@@ -254,9 +256,10 @@ class StepBuilder:
             if isinstance(plan, SharedPlan):
                 part_o = part_ml = None
                 if plan.n_slots:
-                    room = 1 << (plan.n_slots - 1).bit_length()  # (a buffer that a recorded graph points to is never replaced: few sizes)
-                    part_o = workspace.get(f"shared.part.{i}.{room}.o", (room, plan.n_heads, plan.head_dim), torch.float32)[:plan.n_slots]
-                    part_ml = workspace.get(f"shared.part.{i}.{room}.ml", (room, plan.n_heads, 2), torch.float32)[:plan.n_slots]
+                    # (a buffer that a recorded step points to is never replaced)
+                    tag = f"shared.part.{i}.{plan.n_slots}" if self.fixed else f"shared.part.{i}"
+                    part_o = workspace.get(tag + ".o", (plan.n_slots, plan.n_heads, plan.head_dim), torch.float32)
+                    part_ml = workspace.get(tag + ".ml", (plan.n_slots, plan.n_heads, 2), torch.float32)
                 plans[key] = plan.bind({name: tensors[f"plan.{i}.{name}"] for name, _ in plan.sections()}, part_o, part_ml)
                 continue
             n_kv, rows, dim = self.plan_dims[key]

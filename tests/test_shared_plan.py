@@ -2,6 +2,7 @@
 
 import random
 
+import numpy as np
 import pytest
 import torch
 
@@ -121,3 +122,23 @@ def test_refuses_heads_that_do_not_divide():
         build_shared_plan([1], [], 7, 2, 64, torch.float32, 16)
     with pytest.raises(KernelError):
         build_shared_plan([1, 1], [], 8, 2, 64, torch.float32, 16, table_rows=[0])
+
+
+def test_recorded_steps_have_lists_of_few_sizes():
+    """Prompts of every length under every number of continuations: as many launches to record as there are numbers, times a few."""
+    keys = {}
+    for members in (2, 7, 8):
+        for length in range(640, 4096, 48):
+            plan = build_shared_plan([length + 10] * members, [(list(range(members)), 0, length)], 48, 8, 128, torch.bfloat16, 16).rounded()
+            keys.setdefault(members, set()).add(plan.key())
+    assert max(len(k) for k in keys.values()) <= 14
+    rng = random.Random(3)
+    for n in (3, 9, 20):
+        lens = [rng.randrange(900, 1300) for _ in range(n)]
+        spans = [(list(range(n)), 0, 512), (list(range(n // 2)), 512, 864)]
+        plan = build_shared_plan(lens, spans, 16, 4, 64, torch.bfloat16, 16)
+        round_ = plan.rounded()
+        for name in ("items", "members", "joins"):
+            a, b = getattr(plan, name), getattr(round_, name)
+            assert np.array_equal(b[:len(a)], a) and not b[len(a):].any() and len(a) <= len(b) <= 1.5 * len(a)
+        assert plan.n_slots <= round_.n_slots and np.array_equal(plan.requests, round_.requests) and round_.rounded().key() == round_.key()
