@@ -837,14 +837,14 @@ static int moe_gemm_tc_set_status(int code) { return set_status(g_status, code);
 }  // namespace ftk
 
 // Writes a code into a status word from the host, as a kernel whose wait ran out would: unit 0 = the
-// grouped GEMM's word, 1 = the attention kernel's, 2 = the delta rule's, 3 = linear attention's, 4 = the 32-bit products', 5 = attention's over shared keys.  It exists
-// so that the path from a status word to the caller's error can be exercised without making any wait on the device run out.
+// grouped GEMM's word, 1 = the attention kernel's, 2 = the delta rule's, 3 = linear attention's, 4 = the 32-bit products',
+// 6 = attention's over shared keys (5 is nobody's).  It exists so that the path from a status word to the caller's error can be exercised without making any wait on the device run out.
 extern "C" int ftk_debug_set_status(int unit, int code) {
   int (*const set[])(int) = {ftk::moe_gemm_tc_set_status, ftk::attention_tc_set_status, ftk::delta_chunk_set_status, ftk::gla_chunks_set_status,
-                             ftk::moe_gemm_split_set_status, ftk::shared_attention_set_status};
+                             ftk::moe_gemm_split_set_status, nullptr, ftk::shared_attention_set_status};
   constexpr int n = sizeof(set) / sizeof(set[0]);
-  if (unit < 0 || unit >= n) {
-    set_error("debug_set_status: unit must be 0 to %d, got %d", n - 1, unit);
+  if (unit < 0 || unit >= n || !set[unit]) {
+    set_error("debug_set_status: unit must be 0 to 4 or 6, got %d", unit);
     return 1;
   }
   if (set[unit](code) != 0) {

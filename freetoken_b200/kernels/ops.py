@@ -311,8 +311,8 @@ def variant_counts(reset: bool = False) -> dict:
 
 def debug_set_status(unit: int, code: int) -> None:
     """Write ``code`` into a status word from the host (``unit`` 0: grouped GEMM, 1: attention, 2: the delta rule's chunks, 3: gated
-    linear attention's, 4: 32-bit products, 5: attention over shared keys), as a kernel whose bounded wait ran out would have.  For tests of the error path;
-    nothing waits."""
+    linear attention's, 4: 32-bit products, 6: attention over shared keys; 5 is nobody's), as a kernel whose bounded wait ran out would
+    have.  For tests of the error path; nothing waits."""
     _check(_lib().ftk_debug_set_status(int(unit), int(code)), "debug_set_status", 0)
 
 
@@ -725,7 +725,8 @@ def shared_attention(q: torch.Tensor, k_slab: torch.Tensor, v_slab: torch.Tensor
     ``q, out [T, Hq, D]``; slabs ``[pages, Hkv, page_size, D]``; ``block_table [rows, width]`` page ids; ``plan`` from
     :func:`freetoken_b200.engine.shared_plan.build_shared_plan`, on the device with its scratch.  Request ``i`` of the plan is row
     ``i`` of ``q``; it reads all of its keys (its own token's lies among them).  Rows of ``out`` that are no request's stay as they are,
-    a request without keys gets zeros.  float32 and bfloat16, heads of 16 to 256 in steps of 16, any page size and group.  Results do
+    a request without keys gets zeros.  float32 and bfloat16, heads of 16 to 256 in steps of 16, any page size and group; pieces of 256
+    query rows want a positive ``scale``.  The table's pages of shared keys must exist; own keys whose page does not are left out.  Results do
     not depend on the order in which blocks run, but on the plan (the order of a request's sums is that of its pieces).
 
     ``sink``: a logit, a float32 tensor ``[Hq]`` of one per query head, or None, as in :func:`paged_attention`.
@@ -734,6 +735,8 @@ def shared_attention(q: torch.Tensor, k_slab: torch.Tensor, v_slab: torch.Tensor
     fixed = plan.fixed
     if fixed is None:
         fixed = plan.fixed = _shared_fixed(plan)
+    elif plan.requests.device.index != torch._C._cuda_getDevice():
+        raise KernelError(f"shared_attention: the plan is on '{plan.requests.device}', the current device is 'cuda:{torch._C._cuda_getDevice()}'")
     host = plan.host
     shape, slab = q.shape, k_slab.shape
     if len(shape) != 3 or len(slab) != 4:

@@ -304,3 +304,26 @@ def test_refusals():
     slab = torch.empty((4, 2, 16, 24), dtype=BF16, device=DEV)
     with pytest.raises(KernelError, match="head_dim"):
         ops.shared_attention(wide, slab, slab, table, build_shared_plan(lens, [], 8, 2, 24, BF16, 16).to(DEV), torch.empty_like(wide), 0.125)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tile_rows", [16, 256])
+def test_rounded_lists_give_the_same(tile_rows):
+    lens, spans = [700, 650, 644, 300, 701, 0, 650], [([0, 1, 2, 4, 6], 0, 640), ([3, 5], 0, 0)]
+    q, k, v, table = case(lens, spans, 16, 4, 64, 16, BF16)
+    plan = build_shared_plan(lens, spans, 16, 4, 64, BF16, 16, tile_rows=tile_rows)
+    round_ = plan.rounded()
+    assert round_.key() != plan.key()
+    got = [run(q, k, v, table, p.to(DEV), 0.125) for p in (plan, round_)]
+    assert torch.equal(*got)
+
+
+@pytest.mark.gpu
+def test_a_plan_on_another_device_is_refused(monkeypatch):
+    lens, spans = [50, 49], TWO
+    q, k, v, table = [t.to(DEV) for t in case(lens, spans, 8, 2, 64, 16, BF16)]
+    plan, out = build_shared_plan(lens, spans, 8, 2, 64, BF16, 16).to(DEV), torch.empty_like(q)
+    ops.shared_attention(q, k, v, table, plan, out, 0.125)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 1)  # (of two, the second is current)
+    with pytest.raises(KernelError, match="the plan is on"):
+        ops.shared_attention(q, k, v, table, plan, out, 0.125)
