@@ -461,15 +461,16 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
           if (!(need > 0.0)) return top_key;
           above = v[2];
           inside = n[0];
-          if (!(v[1] >= need && v[2] < need)) {  // (not the place after all)
+          pass = 1;
+          if (!(v[1] >= need && v[2] < need)) {  // (not the place after all: from the start)
             lo = limit;
             hi = top_key;
             above = 0.0;
             inside = V;
+            pass = 0;
           }
           by_key = false;
           part = -1.0;
-          pass = 1;
         }
         for (; (lo < hi && inside > kListed) || pass == 0; ++pass) {
           uint32_t q1, q2, q3;
