@@ -15,14 +15,17 @@
 // memory.  A threshold is searched for by the number or the mass of the logits above it, with three candidates a pass; a logit's
 // exponential is taken only where it lies between the last candidates, and when at most kListed logits do, each of them is tried.
 // What bounds it: for one draw the passes one after the other (a barrier of the cluster and a trip through its shared memory each, about
-// a microsecond); for many the exponentials in 64 bits (13 operations each at 64 an SM and cycle).
+// a microsecond); for many the instructions of the passes (0.7 of the issue slots taken, the 64-bit pipe 0.12): so logits lie in shared
+// memory as numbers, four to a load, and are compared as such.  Rows of 200,000, from L2: one draw without filters 21 us, min-p 18,
+// top-k 50, top-p and min-p 35, top-p alone 43; 96 draws from 24 rows 80, 122 and (top-p) 204 us (with ordered integers, one to a load, 107,
+// 145 and 268); 256 rows with min-p 132.
 #include "common.cuh"
 
 namespace ftk {
 
 constexpr int kDrawThreads = 512, kDrawWarps = kDrawThreads / 32;
 constexpr int kListed = 256;      // logits that are tried one by one
-constexpr int kMostRun = 105;     // logits of a thread's run that shared memory has room for
+constexpr int kMostRun = 108;     // logits of a thread's run that shared memory has room for
 
 struct DrawParams {
   const float* logits;
@@ -36,11 +39,11 @@ struct DrawParams {
   const float* u;
   int32_t* out;
   float* logprobs;
-  int cluster, run;  // CTAs a draw; logits of a thread's run (odd: neighbouring threads' runs begin in different banks)
+  int cluster, run;  // CTAs a draw; logits of a thread's run (four times an odd number: eight threads' quarters then lie in different banks)
 };
 
 // Logits in an order-preserving integer form: key 0 stands for NaN and -infinity.
-__device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x + 0.f; }  // (-0 is 0)
+__device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY) + 0.f; }  // (of a NaN and a number fmaxf gives the number; -0 is 0)
 __device__ __forceinline__ uint32_t order_key(float x) {
   if (x == -INFINITY) return 0u;
   const uint32_t b = __float_as_uint(x);
@@ -117,7 +120,7 @@ __device__ __forceinline__ double exp2_down(double y, const double* powers) {
   double q = fma(r, 5.55041086648215831e-02, 2.40226506959100722e-01);
   q = fma(q, r, 6.93147180559945286e-01);
   const double t = powers[n & 255], v = fma(t, q * r, t);
-  return y > -1000.0 ? __hiloint2double(__double2hiint(v) + ((n >> 8) << 20), __double2loint(v)) : y != y ? y : 0.0;
+  return y > -1000.0 ? __hiloint2double(__double2hiint(v) + ((n >> 8) << 20), __double2loint(v)) : 0.0;
 }
 
 __device__ __forceinline__ float exp2f_fast(float x) {
@@ -173,7 +176,7 @@ template <bool STAGED>
 __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_constant__ DrawParams p) {
   pdl_wait();
   pdl_trigger();
-  extern __shared__ __align__(16) uint32_t staged[];  // the chunk's logits as keys
+  extern __shared__ __align__(16) float staged[];  // the chunk's logits, -infinity behind the row's end
   __shared__ DrawShared sh;
   const int C = p.cluster, rank = blockIdx.x % C, draw = blockIdx.x / C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, V = p.vocab;
   const int row = p.rows ? p.rows[draw] : draw;
@@ -193,13 +196,14 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
     sh.crossing = 0x7fffffff;
   }
   // ---- the chunk comes in; its largest logit
-  uint32_t top_key = 0u, low_key = 0xffffffffu;  // the largest logit, and the smallest above -infinity
+  uint32_t top_key, low_key;  // the largest logit, and the smallest above -infinity
   {
-    auto note = [&](float v) -> uint32_t {
-      const uint32_t k = order_key(clean(v));
-      top_key = max(top_key, k);
-      low_key = min(low_key, k - 1u);  // (0 wraps)
-      return k;
+    float most = -INFINITY, least = INFINITY;
+    auto note = [&](float v) -> float {
+      v = clean(v);
+      most = fmaxf(most, v);
+      least = fminf(least, v == -INFINITY ? INFINITY : v);
+      return v;
     };
     if ((((uintptr_t)x) & 15) == 0) {
       const float4* x4 = reinterpret_cast<const float4*>(x);
@@ -215,14 +219,14 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
         for (int e = 0; e < 7; ++e) {
           const int i = i0 + e * kDrawThreads + tid;
           if (i < n4) {
-            if (STAGED) *reinterpret_cast<uint4*>(staged + 4 * i) = make_uint4(note(v[e].x), note(v[e].y), note(v[e].z), note(v[e].w));
-            else note(v[e].x), note(v[e].y), note(v[e].z), note(v[e].w);
+            const float4 c = make_float4(note(v[e].x), note(v[e].y), note(v[e].z), note(v[e].w));
+            if (STAGED) *reinterpret_cast<float4*>(staged + 4 * i) = c;
           }
         }
       }
       for (int i = 4 * n4 + tid; i < n_here; i += kDrawThreads) {
-        const uint32_t k = note(x[i]);
-        if (STAGED) staged[i] = k;
+        const float c = note(x[i]);
+        if (STAGED) staged[i] = c;
       }
     } else {
       for (int i0 = 0; i0 < n_here; i0 += 8 * kDrawThreads) {
@@ -236,12 +240,16 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
         for (int e = 0; e < 8; ++e) {
           const int i = i0 + e * kDrawThreads + tid;
           if (i < n_here) {
-            const uint32_t k = note(v[e]);
-            if (STAGED) staged[i] = k;
+            const float c = note(v[e]);
+            if (STAGED) staged[i] = c;
           }
         }
       }
     }
+    if (STAGED)
+      for (int i = n_here + tid; i < chunk && i < ((n_here + 3) & ~3); i += kDrawThreads) staged[i] = -INFINITY;
+    top_key = order_key(most);
+    low_key = least == INFINITY && most < INFINITY ? 0xffffffffu : order_key(least) - 1u;
     top_key = __reduce_max_sync(0xffffffffu, top_key);
     low_key = __reduce_min_sync(0xffffffffu, low_key);
   }
@@ -262,14 +270,34 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
     low_key = __reduce_min_sync(0xffffffffu, lane < C ? remote_u32(draw_remote(&sh.own_key[1], lane)) : 0xffffffffu);
   }
   low_key += 1u;
-  const float top = of_key(top_key), t = p.temperature[draw];
+  const float t = p.temperature[draw];
   const int i0 = min(n_here, tid * p.run), i1 = min(n_here, i0 + p.run);
-  auto at = [&](int i) -> uint32_t { return STAGED ? staged[i] : order_key(clean(__ldg(x + i))); };
-  // four keys of the run at a time (0 behind its end), so that four exponentials are under way at once
-  auto four = [&](int i, uint32_t (&k)[4]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) k[e] = i + e < i1 ? at(i + e) : 0u;
+  // Where the largest logit is infinite, its like have all of the mass: they count as 0, the others as -infinity.
+  const bool endless = top_key == order_key(INFINITY);
+  if (endless) {
+    if (STAGED) {
+      for (int i = i0; i < i1; ++i) staged[i] = staged[i] == INFINITY ? 0.f : -INFINITY;
+      __syncthreads();
+    }
+    top_key = low_key = order_key(0.f);
+  }
+  const float top = of_key(top_key);
+  auto seen = [&](float v) -> float {
+    v = clean(v);
+    return !endless ? v : v == INFINITY ? 0.f : -INFINITY;
   };
+  auto at = [&](int i) -> float { return STAGED ? staged[i] : seen(__ldg(x + i)); };
+  // four of the run at a time (-infinity behind its end), so that four exponentials are under way at once
+  auto four = [&](int i, float (&v)[4]) {
+    if (STAGED) {
+      const float4 f = *reinterpret_cast<const float4*>(staged + i);
+      v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = i + e < i1 ? at(i + e) : -INFINITY;
+    }
+  };
+  auto most_of = [](const float (&v)[4]) { return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])); };
   int turn = 0;
   // Sums over the cluster, the same in every thread: NM of 64-bit numbers and NC of integers.
   auto cluster_sums = [&](auto masses, auto counts, double (&m)[4], int (&n)[4]) {
@@ -323,7 +351,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
   if (top_key != 0u) {
     if (!(t > 0.f)) {  // the lowest index of the largest logit
       for (int i = i0; i < i1; ++i)
-        if (at(i) == top_key) {
+        if (at(i) == top) {
           atomicMin(&sh.first, c0 + i);
           break;
         }
@@ -338,10 +366,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
       }
     } else {
       const double inv_t = 1.0 / (double)t, per_bit = inv_t * 1.4426950408889634074;  // z / ln 2 of a logit's distance
-      auto mass_of = [&](uint32_t k) -> double {
-        const double m = exp2_down(((double)of_key(k) - (double)top) * per_bit, sh.powers);
-        return k == top_key ? 1.0 : m;
-      };
+      auto mass_of = [&](float v) -> double { return exp2_down(((double)v - (double)top) * per_bit, sh.powers); };
       int held_by_k = V;  // logits that top-k left
       double whole = -1.0;  // the mass of the whole row at this temperature, where it was summed up
       // Three candidates between: by value, as logits spread like their values do: close below the largest where some lie far away (masked
@@ -352,7 +377,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
         const float a = of_key(lo), b = of_key(hi);
         q1 = lo + gap / 4u + (gap < 4u), q2 = lo + gap / 2u + (gap & 1u), q3 = hi - gap / 4u;
         const bool wide = !(b - a <= 64.f * t);
-        if (!by_key && b < INFINITY) {
+        if (!by_key) {
           q1 = order_key(clean(wide ? b - 30.f * t : a + 0.25f * (b - a)));
           q2 = order_key(clean(wide ? b - 10.f * t : a + 0.5f * (b - a)));
           q3 = order_key(clean(wide ? b - 4.f * t : a + 0.75f * (b - a)));
@@ -369,36 +394,39 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
         return wide;
       };
       // The largest key from `lo` on at which the number (by_mass: the mass) of the logits that reach it is `need` (by_mass: `need` of what
-      // reaches `lo`) or more; `lo` where not even that has as many.
+      // reaches `lo`) or more; `lo` where not even that has as many.  (Logits are compared as numbers: what lies above key `hi` reaches the
+      // number of key hi + 1.)
       auto search = [&](bool by_mass, uint32_t lo, double need) -> uint32_t {
         uint32_t hi = top_key;
         double above = 0.0;    // of the logits above `hi`
         int inside = held_by_k, mine = 0;  // logits between, and this thread's of them
-        bool by_key = false;
+        bool by_key = false, sure = false;
         double part = -1.0;  // of what is between, how much lies above the place that is searched for, about
-        int pass = 0;
         if (by_mass) {
           // In 32 bits first, down to where the sums' roundings (2^-16 of them is more than those make) leave it open; then one pass in 64 bits
-          // over everything, which finds the mass and confirms the place.  (Each pass over everything in 64 bits is 12 us, in 32 bits 3.)
+          // over everything, which finds the mass and confirms the place.
           const uint32_t limit = lo;
-          const float per_bit32 = (float)per_bit;
+          const float limit_x = of_key(limit), per_bit32 = fminf((float)per_bit, 3e38f);
           double reach = 0.0, need32 = 0.0, held = 0.0;  // mass of all, what is wanted of it, mass between
+          int over = 0;                                  // logits above `hi`
           for (int p32 = 0; p32 < 12 && lo < hi && inside > kListed / 2; ++p32) {
-            uint32_t q1, q2, q3;
-            const bool wide = candidates(lo, hi, by_key || p32 % 4 == 3, part, q1, q2, q3);
+            uint32_t q[4];
+            const bool wide = candidates(lo, hi, by_key || p32 % 4 == 3, part, q[1], q[2], q[3]);
+            q[0] = lo;
+            const float lo_x = of_key(lo), q1 = of_key(q[1]), q2 = of_key(q[2]), q3 = of_key(q[3]);
             float f[4] = {0.f, 0.f, 0.f, 0.f};
             int n[4] = {0, 0, 0, 0};
             for (int i = i0; i < i1; i += 4) {
-              uint32_t k[4];
-              four(i, k);
+              float v[4];
+              four(i, v);
+              if (most_of(v) < lo_x) continue;
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                if (k[e] > hi) k[e] = 0u;
-                const float m = k[e] == top_key ? 1.f : exp2f_fast((of_key(k[e]) - top) * per_bit32);
-                if (p32 == 0) f[0] += k[e] >= lo ? m : 0.f;
-                if (k[e] >= q1) { ++n[1]; f[1] += m; }
-                if (k[e] >= q2) { ++n[2]; f[2] += m; }
-                if (k[e] >= q3) { ++n[3]; f[3] += m; }
+                const float m = exp2f_fast((v[e] - top) * per_bit32);
+                f[0] += v[e] >= limit_x ? m : 0.f;
+                if (v[e] >= q1) { ++n[1]; f[1] += m; }
+                if (v[e] >= q2) { ++n[2]; f[2] += m; }
+                if (v[e] >= q3) { ++n[3]; f[3] += m; }
               }
             }
             double v[4] = {f[0], f[1], f[2], f[3]};
@@ -407,51 +435,45 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
               reach = v[0];
               need32 = need * reach;
             } else {
-              v[0] = held;
+              v[0] = above + held;
             }
-            n[0] = inside;
-            const uint32_t q[4] = {lo, q1, q2, q3};
+            n[0] = over + inside;
             const double open = reach * (1.0 / 65536.0);
             int a = 0, b = 4;  // the last candidate that is reached for sure, the first that is not
 #pragma unroll
             for (int s = 1; s < 4; ++s)
-              if (above + v[s] >= need32 + open) a = s;
+              if (v[s] >= need32 + open) a = s;
 #pragma unroll
             for (int s = 3; s > 0; --s)
-              if (above + v[s] <= need32 - open) b = s;
+              if (v[s] <= need32 - open) b = s;
             if (a == 0 && b == 4) break;
             by_key = a == 0 && wide;
-            int below = n[0], beyond = 0;
+            int below = n[0], beyond = over;
+            double mass_below = v[0], mass_beyond = above;
 #pragma unroll
             for (int s = 1; s < 4; ++s) {
-              if (s == a) { lo = q[s]; below = n[s]; }
-              if (s == b) { hi = q[s] - 1u; beyond = n[s]; }
+              if (s == a) { lo = q[s]; below = n[s]; mass_below = v[s]; }
+              if (s == b) { hi = q[s] - 1u; beyond = n[s]; mass_beyond = v[s]; }
             }
+            over = beyond;
             inside = below - beyond;
-            double more = 0.0;
-            held = v[0];
-#pragma unroll
-            for (int s = 1; s < 4; ++s) {
-              if (s == a) held = v[s];
-              if (s == b) more = v[s];
-            }
-            above += more;
-            held -= more;
+            above = mass_beyond;
+            held = mass_below - mass_beyond;
             part = (need32 - above) / fmax(held, 1e-300);
           }
+          const float lo_x = of_key(lo), over_x = of_key(hi + 1u);
           double v[4] = {0.0, 0.0, 0.0, 0.0};  // what reaches `limit`, `lo`, and what is above `hi`
           int n[4] = {0, 0, 0, 0};
           for (int i = i0; i < i1; i += 4) {
-            uint32_t k[4];
-            four(i, k);
-            if (max(max(k[0], k[1]), max(k[2], k[3])) < limit) continue;
+            float x4[4];
+            four(i, x4);
+            if (most_of(x4) < limit_x) continue;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const double m = k[e] >= limit ? mass_of(k[e]) : 0.0;
-              v[0] += m;
-              v[1] += k[e] >= lo ? m : 0.0;
-              v[2] += k[e] > hi ? m : 0.0;
-              n[0] += k[e] >= lo && k[e] <= hi;
+              const double m = mass_of(x4[e]);
+              if (x4[e] >= limit_x) v[0] += m;
+              if (x4[e] >= lo_x) { v[1] += m; ++n[0]; }
+              if (x4[e] >= over_x) { v[2] += m; --n[0]; }
             }
           }
           mine = n[0];
@@ -461,45 +483,51 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
           if (!(need > 0.0)) return top_key;
           above = v[2];
           inside = n[0];
-          pass = 1;
-          if (!(v[1] >= need && v[2] < need)) {  // (not the place after all: from the start)
+          sure = v[1] >= need && v[2] < need;
+          if (!sure) {  // (not the place after all: from the start)
             lo = limit;
             hi = top_key;
             above = 0.0;
-            inside = V;
-            pass = 0;
           }
           by_key = false;
           part = -1.0;
         }
-        for (; (lo < hi && inside > kListed) || pass == 0; ++pass) {
-          uint32_t q1, q2, q3;
-          const bool wide = candidates(lo, hi, by_key || pass % 3 == 2, part, q1, q2, q3);
+        for (int pass = 0; !sure || (lo < hi && inside > kListed); ++pass) {
+          uint32_t k1, k2, k3;
+          const bool wide = candidates(lo, hi, by_key || pass % 3 == 2, part, k1, k2, k3);
+          const float lo_x = of_key(lo), over_x = of_key(hi + 1u), q1 = of_key(k1), q2 = of_key(k2), q3 = of_key(k3);
           double v[4] = {0.0, 0.0, 0.0, 0.0};  // mass (or number) and number of the logits that reach lo, q1, q2, q3, and no more than hi
-          int n[4] = {0, 0, 0, 0};
-          for (int i = i0; i < i1; i += 4) {
-            uint32_t k[4];
-            four(i, k);
-            bool some = false;
+          int n[4] = {0, 0, 0, 0}, own_over = 0;
+          if (by_mass) {
+            for (int i = i0; i < i1; i += 4) {
+              float x4[4];
+              four(i, x4);
+              if (most_of(x4) < lo_x) continue;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if (k[e] > hi) k[e] = 0u;
-              n[0] += k[e] >= lo;
-              n[1] += k[e] >= q1;
-              n[2] += k[e] >= q2;
-              n[3] += k[e] >= q3;
-              some |= k[e] >= lo;
+              for (int e = 0; e < 4; ++e)
+                if (x4[e] >= lo_x && !(x4[e] >= over_x)) {
+                  const double m = mass_of(x4[e]);
+                  ++n[0], v[0] += m;
+                  if (x4[e] >= q1) { ++n[1]; v[1] += m; }
+                  if (x4[e] >= q2) { ++n[2]; v[2] += m; }
+                  if (x4[e] >= q3) { ++n[3]; v[3] += m; }
+                }
             }
-            if (by_mass && some) {
+          } else {
+            for (int i = i0; i < i1; i += 4) {
+              float x4[4];
+              four(i, x4);
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const double m = mass_of(k[e]);
-                v[0] += k[e] >= lo ? m : 0.0;
-                v[1] += k[e] >= q1 ? m : 0.0;
-                v[2] += k[e] >= q2 ? m : 0.0;
-                v[3] += k[e] >= q3 ? m : 0.0;
+                n[0] += x4[e] >= lo_x;
+                n[1] += x4[e] >= q1;
+                n[2] += x4[e] >= q2;
+                n[3] += x4[e] >= q3;
+                own_over += x4[e] >= over_x;
               }
             }
+#pragma unroll
+            for (int s = 0; s < 4; ++s) n[s] -= own_over;
           }
           const int own0 = n[0], own1 = n[1], own2 = n[2], own3 = n[3];  // this thread's
           if (by_mass) {
@@ -508,16 +536,17 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
             cluster_sums(SumCount<0>(), SumCount<4>(), v, n);
             v[0] = n[0]; v[1] = n[1]; v[2] = n[2]; v[3] = n[3];
           }
-          if (pass == 0) {
+          if (!sure) {
             if (v[0] < need) return lo;
             if (lo >= hi) return lo;
+            sure = true;
           }
           by_key = false;
           double held = v[0] - v[1];
-          if (above + v[3] >= need) { lo = q3; inside = n[3]; mine = own3; held = v[3]; }
-          else if (above + v[2] >= need) { above += v[3]; lo = q2; hi = q3 - 1u; inside = n[2] - n[3]; mine = own2 - own3; held = v[2] - v[3]; }
-          else if (above + v[1] >= need) { above += v[2]; lo = q1; hi = q2 - 1u; inside = n[1] - n[2]; mine = own1 - own2; held = v[1] - v[2]; }
-          else { above += v[1]; hi = q1 - 1u; inside = n[0] - n[1]; by_key = wide; mine = own0 - own1; }
+          if (above + v[3] >= need) { lo = k3; inside = n[3]; mine = own3; held = v[3]; }
+          else if (above + v[2] >= need) { above += v[3]; lo = k2; hi = k3 - 1u; inside = n[2] - n[3]; mine = own2 - own3; held = v[2] - v[3]; }
+          else if (above + v[1] >= need) { above += v[2]; lo = k1; hi = k2 - 1u; inside = n[1] - n[2]; mine = own1 - own2; held = v[1] - v[2]; }
+          else { above += v[1]; hi = k1 - 1u; inside = n[0] - n[1]; by_key = wide; mine = own0 - own1; }
           if (by_mass) part = (need - above) / fmax(held, 1e-300);  // (a tail's numbers fall off too fast for that)
         }
         if (lo >= hi) return lo;
@@ -537,14 +566,15 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
         }
         int to = base + before - mine;
         const int full = base + before;
+        const float lo_x = of_key(lo), over_x = of_key(hi + 1u);
         for (int i = i0; to < full; i += 4) {
-          uint32_t k[4];
-          four(i, k);
+          float v[4];
+          four(i, v);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (k[e] >= lo && k[e] <= hi) {
-              sh.listed[to] = k[e];
-              sh.listed_mass[to++] = by_mass ? mass_of(k[e]) : 1.0;
+            if (v[e] >= lo_x && !(v[e] >= over_x)) {
+              sh.listed[to] = order_key(v[e]);
+              sh.listed_mass[to++] = by_mass ? mass_of(v[e]) : 1.0;
             }
         }
         if (tid == 0) sh.own_index[0] = all;
@@ -592,24 +622,25 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
       const float mp = p.min_p[draw];
       const double least = mp > 0.f ? fmin(log((double)mp), 0.0) : -INFINITY;
       uint32_t quick = limit;  // most of what min-p leaves out is told by its key (which is rounded, so four steps are left for the exact question)
-      if (mp > 0.f && top < INFINITY) {
+      if (mp > 0.f) {
         const uint32_t near = order_key(clean((float)((double)top + least * (double)t)));
         if (near > 4u) quick = max(quick, near - 4u);
       }
-      auto kept = [&](uint32_t k) -> double {
-        const double d = (double)of_key(k) - (double)top, m = exp2_down(d * per_bit, sh.powers);
-        return k == top_key ? 1.0 : k >= quick && d * inv_t >= least ? m : 0.0;
+      const float quick_x = of_key(quick);
+      auto kept = [&](float v) -> double {
+        const double d = (double)v - (double)top, m = exp2_down(d * per_bit, sh.powers);
+        return v >= quick_x && d * inv_t >= least ? m : 0.0;
       };
       // the thread's run, then the running mass behind every thread's run
       double c = 0.0;
       int newest = -1;
       for (int i = i0; i < i1; i += 4) {
-        uint32_t k[4];
-        four(i, k);
-        if (max(max(k[0], k[1]), max(k[2], k[3])) < quick) continue;
+        float v[4];
+        four(i, v);
+        if (most_of(v) < quick_x) continue;
         double m[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) m[e] = kept(k[e]);
+        for (int e = 0; e < 4; ++e) m[e] = kept(v[e]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           c += m[e];
@@ -708,20 +739,17 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
     if (top_key != 0u && whole_row < 0.0) {
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
       for (int i = i0; i < i1; i += 4) {
-        uint32_t k[4];
-        four(i, k);
+        float v4[4];
+        four(i, v4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float d = k[e] == top_key ? 0.f : of_key(k[e]) - top;
-          sum[e] += __expf(d);
-        }
+        for (int e = 0; e < 4; ++e) sum[e] += __expf(v4[e] - top);
       }
       int n[4];
       v[0] = (double)(sum[0] + sum[1]) + (double)(sum[2] + sum[3]);
       cluster_sums(SumCount<1>(), SumCount<0>(), v, n);
     }
     if (rank == 0 && tid == 0) {
-      const float xt = clean(p.logits[(size_t)row * p.stride + token]);
+      const float xt = seen(p.logits[(size_t)row * p.stride + token]);
       p.logprobs[draw] = top_key == 0u ? -INFINITY : (float)((xt == top ? 0.0 : (double)xt - (double)top) - log(v[0]));
     }
   }
@@ -744,8 +772,8 @@ extern "C" int ftk_sample_draws(const float* logits, long long row_stride, int n
   DrawParams p{logits, row_stride, n_rows, vocab, rows, temperature, top_k, top_p, min_p, u, out, logprobs, 1, 1};
   // a CTA for every 4,096 logits, eight at most; sixteen where that leaves SMs idle
   while (p.cluster < (n_draws <= 8 ? 16 : 8) && vocab > p.cluster * 4096) p.cluster *= 2;
-  p.run = ((vocab + p.cluster * kDrawThreads - 1) / (p.cluster * kDrawThreads)) | 1;
-  const bool held = p.run <= kMostRun;  // (430,000 logits; longer rows are read again in every pass)
+  p.run = 4 * (((vocab + 4 * p.cluster * kDrawThreads - 1) / (4 * p.cluster * kDrawThreads)) | 1);
+  const bool held = p.run <= kMostRun;  // (442,000 logits; longer rows are read again in every pass)
   const size_t smem = held ? (size_t)p.run * kDrawThreads * sizeof(float) : 0;
   auto kern = held ? draw_kernel<true> : draw_kernel<false>;
   FTK_REQUIRE(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess &&
