@@ -113,14 +113,28 @@ def tile_members(n: int, most: int) -> List[Tuple[int, int]]:
     return [(a, b - a) for a, b in zip(edges, edges[1:])]
 
 
-def own_cluster(longest: int, blocks: int, tile: int, sm_count: int) -> int:
-    """CTAs that share one request's own keys: no more than fill the GPU once, none with less than two tiles of keys.  (Clusters that queue
-    for SMs wait for several to be free at once.  48 heads on 8 of 128, clusters of 1, 2, 4 and 8: 20 requests of 600 own keys 26.4, 35.6,
-    46.9, 77.8 us; 8 of 300 24.8, 22.5, 22.0, 26.6; 4 of 1,500 of 16 heads on 4 34.6, 22.3, 16.4, 17.4; 2 of 500 15.1, 11.5, 10.0, 10.2.)"""
-    cluster = 1
-    while cluster < MOST_CLUSTER and 2 * blocks * cluster <= sm_count and longest > 2 * cluster * tile:
+def own_slots(dtype: torch.dtype, head_dim: int) -> int:
+    """CTAs of the kernel for own keys on an SM: by registers, and by shared memory with all of its places for tiles."""
+    if dtype == torch.bfloat16:
+        smem = (ROWS_TILE + 6 * ROWS_KEYS[dtype]) * (head_dim + 8) * 2
+    else:
+        smem = (ROWS_TILE * head_dim + 4 * ROWS_KEYS[dtype] * (head_dim + 4)) * 4
+    return max(1, min(OWN_CTAS_PER_SM if head_dim <= 128 else 2, 228 * 1024 // (smem + 5 * 1024)))
+
+
+def own_cluster(longest: int, blocks: int, dtype: torch.dtype, slots: int) -> int:
+    """CTAs that share one request's own keys, none with less than two tiles of them.  A CTA takes as long to come and go as for some of its
+    tiles (and for one more with every two others it joins with), and clusters beyond the ``slots`` of the GPU (a seventh of them stays
+    empty) wait for several at once.  Clusters of 1, 2, 4 and 8, us, own keys of one length: 48 heads on 8 of 128, 20 requests of 600 26,
+    35, 47, 78; 8 of 4,000 84, 52, 35, 45; 32 of 1,500 46, 54, 68, 102; 16 on 4 of 64 in 32 bits, 6 of 1,000 91, 50, 29, 20."""
+    tile, lost = ROWS_KEYS[dtype], 9.0 if dtype == torch.bfloat16 else 4.0
+    best, best_t, cluster = 1, None, 1
+    while cluster <= MOST_CLUSTER and (cluster == 1 or longest > cluster * tile):
+        t = max(1.0, blocks * cluster / (0.85 * slots)) * (lost + 0.75 * longest / (cluster * tile) + cluster // 2)  # (lengths vary: three quarters)
+        if best_t is None or t < 0.95 * best_t:
+            best, best_t = cluster, t
         cluster *= 2
-    return cluster
+    return best
 
 
 def rows_length(units: Sequence[int], heads: int, dtype: torch.dtype, sm_count: int) -> int:
@@ -204,18 +218,20 @@ class SharedLayout:
     n_heads: int
     n_kv_heads: int
     head_dim: int
-    unit: int          # keys that the kernel for own keys works on at a time
+    dtype: torch.dtype
     blocks: int        # CTAs it has without clusters
-    sm_count: int
+    slots: int         # CTAs of it that the GPU takes at once
 
     def plan(self, kv_lens: Sequence[int]) -> SharedPlan:
         requests = self.fixed.copy()
         requests[:, 3] = kv_lens
         longest = max(1, int((requests[:, 3] - requests[:, 2]).max(initial=0)))
         longest = 1 << (longest - 1).bit_length()
-        cluster = own_cluster(longest, self.blocks, self.unit, self.sm_count)
+        cluster = own_cluster(longest, self.blocks, self.dtype, self.slots)
+        # the longest first: 48 requests of up to 1,500 own keys 66 -> 46 us, 32 of up to 700 beside 32,000 shared ones 66.0 -> 63.5
+        requests = requests[np.argsort(requests[:, 2] - requests[:, 3], kind="stable")]
         return SharedPlan(self.items, self.members, requests, self.joins, self.n_slots, WIDE_TILE if self.wide else ROWS_TILE, cluster,
-                          -(-longest // (cluster * self.unit)), requests.shape[0], self.n_heads, self.n_kv_heads, self.head_dim)
+                          -(-longest // (cluster * ROWS_KEYS[self.dtype])), requests.shape[0], self.n_heads, self.n_kv_heads, self.head_dim)
 
 
 def build_shared_plan(kv_lens: Sequence[int], spans: Sequence[Span], n_heads: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype,
@@ -312,4 +328,4 @@ def shared_layout(n: int, spans: Sequence[Span], n_heads: int, n_kv_heads: int, 
         joins += own
     as_int = lambda x, w: np.asarray(x, dtype=np.int32).reshape(-1, w) if w else np.asarray(x, dtype=np.int32)  # noqa: E731
     return SharedLayout(as_int(items, ITEM_INTS), as_int(member_rows, 0), as_int(joins, 0), as_int(requests, REQUEST_INTS), n_slots, wide,
-                        n_heads, n_kv_heads, head_dim, ROWS_KEYS[dtype], own_ctas, sm_count)
+                        n_heads, n_kv_heads, head_dim, dtype, own_ctas, sm_count * own_slots(dtype, head_dim))

@@ -22,12 +22,14 @@ def covered(plan, n, rows):
             assert slot0 + i not in of_slot and slot0 + i < plan.n_slots
             of_slot[slot0 + i] = (m, kb, ke) if i < k else (m, ke, ke)
     assert sorted(of_slot) == list(range(plan.n_slots))
-    out = []
-    for i, (q, row, lo, hi, j0, k, *_) in enumerate(plan.requests.tolist()):
-        assert q == i and row == rows[i]
+    out = [None] * n
+    own = (plan.requests[:, 3] - plan.requests[:, 2]).tolist()
+    assert own == sorted(own, reverse=True) and sorted(plan.requests[:, 0].tolist()) == list(range(n))  # (the longest first)
+    for i, row, lo, hi, j0, k, *_ in plan.requests.tolist():
+        assert row == rows[i]
         pieces = [of_slot[s] for s in plan.joins[j0:j0 + k].tolist()]
         assert all(m == i for m, _, _ in pieces)
-        out.append([(a, b) for _, a, b in pieces] + [(lo, hi)])
+        out[i] = [(a, b) for _, a, b in pieces] + [(lo, hi)]
     return out
 
 
@@ -73,11 +75,12 @@ def test_members_are_dealt_to_tiles_evenly():
 
 
 def test_own_keys_are_split_while_the_gpu_is_not_full():
-    assert own_cluster(2048, 8, 64, 148) == 8
-    assert own_cluster(128, 8, 64, 148) == 1     # two tiles of keys each at least
-    assert own_cluster(512, 8, 64, 148) == 4
-    assert own_cluster(2048, 512, 64, 148) == 1  # enough requests
-    assert own_cluster(512, 64, 64, 148) == 2
+    bf16, slots = torch.bfloat16, 296
+    assert own_cluster(2048, 8, bf16, slots) == 8
+    assert own_cluster(128, 8, bf16, slots) <= 2     # two tiles of keys each at least
+    assert own_cluster(2048, 512, bf16, slots) == 1  # enough requests
+    assert [own_cluster(1 << (x - 1).bit_length(), 8 * n, bf16, slots) for n, x in ((20, 600), (8, 4000), (32, 1500), (16, 2000), (18, 400))] == [1, 4, 1, 2, 1]
+    assert own_cluster(1024, 24, torch.float32, 592) == 8
 
 
 @pytest.mark.parametrize("lens,spans,what", [
