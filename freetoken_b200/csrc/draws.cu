@@ -147,7 +147,8 @@ __device__ __forceinline__ uint32_t remote_u32(uint32_t at) {
 __device__ __forceinline__ void draw_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ double warp_sum64(double v) {
+template <typename T>
+__device__ __forceinline__ T warp_sum_of(T v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
@@ -299,12 +300,12 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
   };
   auto most_of = [](const float (&v)[4]) { return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])); };
   int turn = 0;
-  // Sums over the cluster, the same in every thread: NM of 64-bit numbers and NC of integers.
-  auto cluster_sums = [&](auto masses, auto counts, double (&m)[4], int (&n)[4]) {
+  // Sums over the cluster, the same in every thread: NM of masses (a warp's in their own type, the others in 64 bits) and NC of integers.
+  auto cluster_sums = [&](auto masses, auto counts, const auto& part, double (&m)[4], int (&n)[4]) {
     constexpr int NM = decltype(masses)::value, NC = decltype(counts)::value;
 #pragma unroll
     for (int s = 0; s < NM; ++s) {
-      const double v = warp_sum64(m[s]);
+      const double v = warp_sum_of(part[s]);
       if (lane == 0) sh.parts[warp][s] = v;
     }
 #pragma unroll
@@ -313,17 +314,22 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
       if (lane == 0) sh.counts[warp][s] = v;
     }
     __syncthreads();
-    if (warp == 0) {
-      if (lane < NM) {
-        double sum = 0.0;
+    if (warp == 0) {  // lane 16 h + w: sums 2 h and 2 h + 1 of warp w
+      const int w = lane & 15, h = lane >> 4 << 1;
+      double a = h < NM ? sh.parts[w][h] : 0.0, b = h + 1 < NM ? sh.parts[w][h + 1] : 0.0;
+      int c = h < NC ? sh.counts[w][h] : 0, d = h + 1 < NC ? sh.counts[w][h + 1] : 0;
 #pragma unroll
-        for (int w = 0; w < kDrawWarps; ++w) sum += sh.parts[w][lane];
-        sh.sums[turn][lane] = sum;
-      } else if (lane >= 4 && lane < 4 + NC) {
-        int sum = 0;
-#pragma unroll
-        for (int w = 0; w < kDrawWarps; ++w) sum += sh.counts[w][lane - 4];
-        sh.sums[turn][lane] = sum;
+      for (int o = 8; o > 0; o >>= 1) {
+        if (NM > 0) a += __shfl_xor_sync(0xffffffffu, a, o);
+        if (NM > 1) b += __shfl_xor_sync(0xffffffffu, b, o);
+        if (NC > 0) c += __shfl_xor_sync(0xffffffffu, c, o);
+        if (NC > 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+      }
+      if (w == 0) {
+        sh.sums[turn][h] = a;
+        sh.sums[turn][h + 1] = b;
+        sh.sums[turn][4 + h] = c;
+        sh.sums[turn][5 + h] = d;
       }
     }
     if (C > 1) {
@@ -331,8 +337,15 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
       if (warp == 0) {  // lane 8 c + s: sums s of CTAs c, c + 4, ...
         const int s = lane & 7;
         double sum = 0.0;
-        if (s < NM || (s >= 4 && s < 4 + NC))
-          for (int c = lane >> 3; c < C; c += 4) sum += remote_f64(draw_remote(&sh.sums[turn][s], c));
+        if (s < NM || (s >= 4 && s < 4 + NC)) {
+          double v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int c = (lane >> 3) + 4 * e;
+            v[e] = c < C ? remote_f64(draw_remote(&sh.sums[turn][s], c)) : 0.0;
+          }
+          sum = (v[0] + v[1]) + (v[2] + v[3]);
+        }
         sum += __shfl_xor_sync(0xffffffffu, sum, 8);
         sum += __shfl_xor_sync(0xffffffffu, sum, 16);
         if (lane < 8) sh.result[lane] = sum;
@@ -429,8 +442,8 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
                 if (v[e] >= q3) { ++n[3]; f[3] += m; }
               }
             }
-            double v[4] = {f[0], f[1], f[2], f[3]};
-            cluster_sums(SumCount<4>(), SumCount<4>(), v, n);
+            double v[4];
+            cluster_sums(SumCount<4>(), SumCount<4>(), f, v, n);
             if (p32 == 0) {
               reach = v[0];
               need32 = need * reach;
@@ -477,7 +490,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
             }
           }
           mine = n[0];
-          cluster_sums(SumCount<3>(), SumCount<1>(), v, n);
+          cluster_sums(SumCount<3>(), SumCount<1>(), v, v, n);
           if (limit == low_key) whole = v[0];
           need *= v[0];
           if (!(need > 0.0)) return top_key;
@@ -531,9 +544,9 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
           }
           const int own0 = n[0], own1 = n[1], own2 = n[2], own3 = n[3];  // this thread's
           if (by_mass) {
-            cluster_sums(SumCount<4>(), SumCount<4>(), v, n);
+            cluster_sums(SumCount<4>(), SumCount<4>(), v, v, n);
           } else {
-            cluster_sums(SumCount<0>(), SumCount<4>(), v, n);
+            cluster_sums(SumCount<0>(), SumCount<4>(), v, v, n);
             v[0] = n[0]; v[1] = n[1]; v[2] = n[2]; v[3] = n[3];
           }
           if (!sure) {
@@ -746,7 +759,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
       }
       int n[4];
       v[0] = (double)(sum[0] + sum[1]) + (double)(sum[2] + sum[3]);
-      cluster_sums(SumCount<1>(), SumCount<0>(), v, n);
+      cluster_sums(SumCount<1>(), SumCount<0>(), v, v, n);
     }
     if (rank == 0 && tid == 0) {
       const float xt = seen(p.logits[(size_t)row * p.stride + token]);
