@@ -156,7 +156,7 @@ __device__ __forceinline__ T warp_sum_of(T v) {
 
 struct DrawShared {
   double powers[256];
-  double parts[kDrawWarps][4];  // the warps' sums
+  double parts[kDrawWarps][8];  // the warps' sums
   int counts[kDrawWarps][4];
   double sums[2][8];            // the CTA's, for the cluster: in turns, so that one barrier a pass is enough
   double listed_mass[kListed];
@@ -300,8 +300,9 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
   };
   auto most_of = [](const float (&v)[4]) { return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])); };
   int turn = 0;
-  // Sums over the cluster, the same in every thread: NM of masses (a warp's in their own type, the others in 64 bits) and NC of integers.
-  auto cluster_sums = [&](auto masses, auto counts, const auto& part, double (&m)[4], int (&n)[4]) {
+  // Sums over the cluster, the same in every thread: NM of masses (a warp's in their own type, the others in 64 bits) and NC of integers
+  // (four of them at most, and then four masses).
+  auto cluster_sums = [&](auto masses, auto counts, const auto& part, auto& m, int (&n)[4]) {
     constexpr int NM = decltype(masses)::value, NC = decltype(counts)::value;
 #pragma unroll
     for (int s = 0; s < NM; ++s) {
@@ -314,22 +315,28 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
       if (lane == 0) sh.counts[warp][s] = v;
     }
     __syncthreads();
-    if (warp == 0) {  // lane 16 h + w: sums 2 h and 2 h + 1 of warp w
-      const int w = lane & 15, h = lane >> 4 << 1;
-      double a = h < NM ? sh.parts[w][h] : 0.0, b = h + 1 < NM ? sh.parts[w][h + 1] : 0.0;
-      int c = h < NC ? sh.counts[w][h] : 0, d = h + 1 < NC ? sh.counts[w][h + 1] : 0;
+    if (warp == 0) {  // lane 16 h + w: every second sum from h on, of warp w
+      const int w = lane & 15, h = lane >> 4;
+      double a[(NM + 1) / 2 + 1];
+      int c[(NC + 1) / 2 + 1];
+#pragma unroll
+      for (int e = 0; 2 * e < NM; ++e) a[e] = 2 * e + h < NM ? sh.parts[w][2 * e + h] : 0.0;
+#pragma unroll
+      for (int e = 0; 2 * e < NC; ++e) c[e] = 2 * e + h < NC ? sh.counts[w][2 * e + h] : 0;
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) {
-        if (NM > 0) a += __shfl_xor_sync(0xffffffffu, a, o);
-        if (NM > 1) b += __shfl_xor_sync(0xffffffffu, b, o);
-        if (NC > 0) c += __shfl_xor_sync(0xffffffffu, c, o);
-        if (NC > 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+#pragma unroll
+        for (int e = 0; 2 * e < NM; ++e) a[e] += __shfl_xor_sync(0xffffffffu, a[e], o);
+#pragma unroll
+        for (int e = 0; 2 * e < NC; ++e) c[e] += __shfl_xor_sync(0xffffffffu, c[e], o);
       }
       if (w == 0) {
-        sh.sums[turn][h] = a;
-        sh.sums[turn][h + 1] = b;
-        sh.sums[turn][4 + h] = c;
-        sh.sums[turn][5 + h] = d;
+#pragma unroll
+        for (int e = 0; 2 * e < NM; ++e)
+          if (2 * e + h < NM) sh.sums[turn][2 * e + h] = a[e];
+#pragma unroll
+        for (int e = 0; 2 * e < NC; ++e)
+          if (2 * e + h < NC) sh.sums[turn][4 + 2 * e + h] = c[e];
       }
     }
     if (C > 1) {
@@ -381,6 +388,8 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
       const double inv_t = 1.0 / (double)t, per_bit = inv_t * 1.4426950408889634074;  // z / ln 2 of a logit's distance
       auto mass_of = [&](float v) -> double { return exp2_down(((double)v - (double)top) * per_bit, sh.powers); };
       int held_by_k = V;  // logits that top-k left
+      double over_mine = 0.0;           // of this thread's logits: the mass of those that reach key `over_key`, where that was summed up
+      uint32_t over_key = 0xffffffffu;
       double whole = -1.0;  // the mass of the whole row at this temperature, where it was summed up
       // Three candidates between: by value, as logits spread like their values do: close below the largest where some lie far away (masked
       // ones, say: true is returned then), in quarters, or, in a narrow range, around the place that `part` of what it holds lies above; or by
@@ -420,15 +429,31 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
           // over everything, which finds the mass and confirms the place.
           const uint32_t limit = lo;
           const float limit_x = of_key(limit), per_bit32 = fminf((float)per_bit, 3e38f);
-          double reach = 0.0, need32 = 0.0, held = 0.0;  // mass of all, what is wanted of it, mass between
-          int over = 0;                                  // logits above `hi`
-          for (int p32 = 0; p32 < 12 && lo < hi && inside > kListed / 2; ++p32) {
-            uint32_t q[4];
-            const bool wide = candidates(lo, hi, by_key || p32 % 4 == 3, part, q[1], q[2], q[3]);
+          double reach = 0.0, held = 0.0;  // mass of all, mass between
+          bool few = inside <= kListed / 2;
+          for (int p32 = 0; p32 < 12 && lo < hi && !few; ++p32) {
+            // Seven candidates: in eighths by value or, where a few times T is between, around the place that a mass spread evenly over it
+            // would put there; now and then by key, which ends whatever the logits are.
+            uint32_t q[8];
+            const float a = of_key(lo), b = of_key(hi), width = b - a;
+            const bool wide = !(width <= 64.f * t), near = part >= 0.0 && width <= 8.f * t;
+            const bool keys = by_key || p32 % 4 == 3;
+            const float guess = b - (float)part * width;
             q[0] = lo;
-            const float lo_x = of_key(lo), q1 = of_key(q[1]), q2 = of_key(q[2]), q3 = of_key(q[3]);
-            float f[4] = {0.f, 0.f, 0.f, 0.f};
-            int n[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int s = 1; s < 8; ++s) {
+              const float off[8] = {0.f, -0.25f, -0.08f, -0.02f, 0.f, 0.02f, 0.08f, 0.25f}, down[8] = {0.f, 60.f, 30.f, 20.f, 14.f, 9.f, 5.f, 2.f};
+              const float x = wide ? b - down[s] * t : near ? guess + off[s] * width : a + 0.125f * s * width;
+              uint32_t k = keys ? lo + (uint32_t)(((unsigned long long)(hi - lo) * s + 7) >> 3) : order_key(clean(x));
+              q[s] = max(min(max(k, lo + 1u), hi), q[s - 1]);
+            }
+            const float lo_x = of_key(lo);
+            float qx[8], f[8];
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+              qx[s] = s ? of_key(q[s]) : limit_x;
+              f[s] = 0.f;
+            }
             for (int i = i0; i < i1; i += 4) {
               float v[4];
               four(i, v);
@@ -436,43 +461,31 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const float m = exp2f_fast((v[e] - top) * per_bit32);
-                f[0] += v[e] >= limit_x ? m : 0.f;
-                if (v[e] >= q1) { ++n[1]; f[1] += m; }
-                if (v[e] >= q2) { ++n[2]; f[2] += m; }
-                if (v[e] >= q3) { ++n[3]; f[3] += m; }
+#pragma unroll
+                for (int s = 0; s < 8; ++s)
+                  if (v[e] >= qx[s]) f[s] += m;
               }
             }
-            double v[4];
-            cluster_sums(SumCount<4>(), SumCount<4>(), f, v, n);
-            if (p32 == 0) {
-              reach = v[0];
-              need32 = need * reach;
-            } else {
-              v[0] = above + held;
-            }
-            n[0] = over + inside;
-            const double open = reach * (1.0 / 65536.0);
-            int a = 0, b = 4;  // the last candidate that is reached for sure, the first that is not
-#pragma unroll
-            for (int s = 1; s < 4; ++s)
-              if (v[s] >= need32 + open) a = s;
-#pragma unroll
-            for (int s = 3; s > 0; --s)
-              if (v[s] <= need32 - open) b = s;
-            if (a == 0 && b == 4) break;
-            by_key = a == 0 && wide;
-            int below = n[0], beyond = over;
+            double v[8];
+            int none[4];
+            cluster_sums(SumCount<8>(), SumCount<0>(), f, v, none);
+            if (p32 == 0) reach = v[0];
+            else v[0] = above + held;
+            const double need32 = need * reach, open = reach * (1.0 / 65536.0);
+            int sure_s = 0, not_s = 8;  // the last candidate that is reached for sure, the first that is not
             double mass_below = v[0], mass_beyond = above;
 #pragma unroll
-            for (int s = 1; s < 4; ++s) {
-              if (s == a) { lo = q[s]; below = n[s]; mass_below = v[s]; }
-              if (s == b) { hi = q[s] - 1u; beyond = n[s]; mass_beyond = v[s]; }
-            }
-            over = beyond;
-            inside = below - beyond;
+            for (int s = 1; s < 8; ++s)
+              if (v[s] >= need32 + open) { sure_s = s; lo = q[s]; mass_below = v[s]; }
+#pragma unroll
+            for (int s = 7; s > 0; --s)
+              if (v[s] <= need32 - open) { not_s = s; hi = q[s] - 1u; mass_beyond = v[s]; }
+            if (sure_s == 0 && not_s == 8) break;
+            by_key = sure_s == 0 && wide;
             above = mass_beyond;
             held = mass_below - mass_beyond;
             part = (need32 - above) / fmax(held, 1e-300);
+            few = (float)held <= (kListed / 2) * exp2f_fast((of_key(lo) - top) * per_bit32);  // (each has as much as the lowest at least)
           }
           const float lo_x = of_key(lo), over_x = of_key(hi + 1u);
           double v[4] = {0.0, 0.0, 0.0, 0.0};  // what reaches `limit`, `lo`, and what is above `hi`
@@ -490,6 +503,8 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
             }
           }
           mine = n[0];
+          over_mine = v[2];
+          over_key = hi + 1u;
           cluster_sums(SumCount<3>(), SumCount<1>(), v, v, n);
           if (limit == low_key) whole = v[0];
           need *= v[0];
@@ -498,6 +513,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
           inside = n[0];
           sure = v[1] >= need && v[2] < need;
           if (!sure) {  // (not the place after all: from the start)
+            over_key = 0xffffffffu;
             lo = limit;
             hi = top_key;
             above = 0.0;
@@ -560,6 +576,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
           else if (above + v[2] >= need) { above += v[3]; lo = k2; hi = k3 - 1u; inside = n[2] - n[3]; mine = own2 - own3; held = v[2] - v[3]; }
           else if (above + v[1] >= need) { above += v[2]; lo = k1; hi = k2 - 1u; inside = n[1] - n[2]; mine = own1 - own2; held = v[1] - v[2]; }
           else { above += v[1]; hi = k1 - 1u; inside = n[0] - n[1]; by_key = wide; mine = own0 - own1; }
+          over_key = 0xffffffffu;
           if (by_mass) part = (need - above) / fmax(held, 1e-300);  // (a tail's numbers fall off too fast for that)
         }
         if (lo >= hi) return lo;
@@ -594,15 +611,23 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
         if (C > 1) draw_barrier(); else __syncthreads();
         // each of them is tried by a thread of rank 0's numbering: what reaches it
         uint32_t best = lo;
-        int n_all = 0, from_rank = -1, from = 0;
-        for (int c = 0; c < C; ++c) {
-          const int n = C > 1 ? (int)remote_u32(draw_remote(&sh.own_index[0], c)) : all;
-          if (tid >= n_all && tid < n_all + n) {
-            from_rank = c;
-            from = tid - n_all;
-          }
-          n_all += n;
+        const int theirs = lane < C ? (C > 1 ? (int)remote_u32(draw_remote(&sh.own_index[0], lane)) : all) : 0;
+        int n_all = theirs;  // the lists' lengths, added up
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int other = __shfl_up_sync(0xffffffffu, n_all, o);
+          if (lane >= o) n_all += other;
         }
+        int from_rank = -1, from = 0;
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          const int end = __shfl_sync(0xffffffffu, n_all, c), n = __shfl_sync(0xffffffffu, theirs, c);
+          if (tid < end && tid >= end - n) {
+            from_rank = c;
+            from = tid - (end - n);
+          }
+        }
+        n_all = __shfl_sync(0xffffffffu, n_all, 31);
         const uint32_t key = from_rank >= 0 ? (C > 1 ? remote_u32(draw_remote(&sh.listed[from], from_rank)) : sh.listed[from]) : 0u;
         const double weight = from_rank >= 0 ? (C > 1 ? remote_f64(draw_remote(&sh.listed_mass[from], from_rank)) : sh.listed_mass[from]) : 0.0;
         if (C > 1) draw_barrier(); else __syncthreads();  // (everyone has what it needs of the others' lists)
@@ -612,9 +637,12 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
         }
         __syncthreads();
         if (from_rank >= 0) {
-          double sum = above;
-          for (int j = 0; j < n_all; ++j) sum += sh.listed[j] >= key ? sh.listed_mass[j] : 0.0;
-          if (sum >= need) best = key;
+          double sum[4] = {above, 0.0, 0.0, 0.0};
+          for (int j = 0; j < n_all; j += 4)  // (what is behind the last is key 0)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (sh.listed[j + e] >= key) sum[e] += sh.listed_mass[j + e];
+          if ((sum[0] + sum[1]) + (sum[2] + sum[3]) >= need) best = key;
         }
         best = __reduce_max_sync(0xffffffffu, best);
         __syncthreads();
@@ -647,17 +675,33 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
       // the thread's run, then the running mass behind every thread's run
       double c = 0.0;
       int newest = -1;
-      for (int i = i0; i < i1; i += 4) {
-        float v[4];
-        four(i, v);
-        if (most_of(v) < quick_x) continue;
-        double m[4];
+      if (over_key != 0xffffffffu && !(mp > 0.f)) {  // top-p's search left the mass above its last bracket
+        const float over_x = of_key(over_key);
+        c = over_mine;
+        for (int i = i0; i < i1; i += 4) {
+          float v[4];
+          four(i, v);
+          if (most_of(v) < quick_x) continue;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) m[e] = kept(v[e]);
+          for (int e = 0; e < 4; ++e)
+            if (v[e] >= quick_x) {
+              newest = i + e;
+              if (!(v[e] >= over_x)) c += mass_of(v[e]);
+            }
+        }
+      } else {
+        for (int i = i0; i < i1; i += 4) {
+          float v[4];
+          four(i, v);
+          if (most_of(v) < quick_x) continue;
+          double m[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          c += m[e];
-          if (m[e] > 0.0) newest = i + e;
+          for (int e = 0; e < 4; ++e) m[e] = kept(v[e]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            c += m[e];
+            if (m[e] > 0.0) newest = i + e;
+          }
         }
       }
       double behind = c;
