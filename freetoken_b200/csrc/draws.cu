@@ -14,16 +14,18 @@
 // A cluster of up to sixteen CTAs takes a draw: a thread has a run of neighbouring logits, kept in shared memory from the one pass over
 // memory.  A threshold is searched for by the number or the mass of the logits above it, with three candidates a pass; a logit's
 // exponential is taken only where it lies between the last candidates, and when at most kListed logits do, each of them is tried.
-// What bounds it: for one draw the passes one after the other (a barrier of the cluster and a trip through its shared memory each, about
-// a microsecond); for many the instructions of the passes (0.7 of the issue slots taken, the 64-bit pipe 0.12): so logits lie in shared
-// memory as numbers, four to a load, and are compared as such.  Rows of 200,000, from L2: one draw without filters 21 us, min-p 18,
-// top-k 50, top-p and min-p 35, top-p alone 43; 96 draws from 24 rows 80, 122 and (top-p) 204 us (with ordered integers, one to a load, 107,
-// 145 and 268); 256 rows with min-p 132.
+// What a CTA has to tell the others it writes into their shared memory in front of the cluster's barrier: reading it there behind
+// the barrier would be one trip more a pass.
+// What bounds it: for one draw the passes one after the other (a barrier of the cluster each, a microsecond or so with the wait for the
+// slowest CTA); for many the instructions of the passes (0.7 of the issue slots taken, the 64-bit pipe 0.12): so logits lie in shared
+// memory as numbers, four to a load, and are compared as such.  Rows of 200,000 logits: one draw without filters 20 us, min-p 17,
+// top-k 50, top-p and min-p 32, top-p alone 38; 96 draws from 24 rows 78, 119 and (top-p) 172 us; 256 rows with min-p 128.
 #include "common.cuh"
 
 namespace ftk {
 
 constexpr int kDrawThreads = 512, kDrawWarps = kDrawThreads / 32;
+constexpr int kMostCluster = 16;
 constexpr int kListed = 256;      // logits that are tried one by one
 constexpr int kMostRun = 108;     // logits of a thread's run that shared memory has room for
 
@@ -134,18 +136,13 @@ __device__ __forceinline__ uint32_t draw_remote(const void* p, int rank) {
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(draw_addr(p)), "r"(rank));
   return r;
 }
-__device__ __forceinline__ double remote_f64(uint32_t at) {
-  double v;
-  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(at));
-  return v;
-}
-__device__ __forceinline__ uint32_t remote_u32(uint32_t at) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at));
-  return v;
-}
+__device__ __forceinline__ void put_f64(uint32_t at, double v) { asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(v) : "memory"); }
+__device__ __forceinline__ void put_u32(uint32_t at, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
+__device__ __forceinline__ void draw_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void draw_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void draw_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  draw_arrive();
+  draw_wait();
 }
 template <typename T>
 __device__ __forceinline__ T warp_sum_of(T v) {
@@ -158,14 +155,11 @@ struct DrawShared {
   double powers[256];
   double parts[kDrawWarps][8];  // the warps' sums
   int counts[kDrawWarps][4];
-  double sums[2][8];            // the CTA's, for the cluster: in turns, so that one barrier a pass is enough
+  double inbox[2][kMostCluster][8];  // what every CTA of the cluster has sent to this one: in turns, so that one barrier a pass is enough
   double listed_mass[kListed];
   uint32_t listed[kListed];
-  double result[8];             // the cluster's
-  uint32_t own_key[2];          // the CTA's largest and smallest key
-  int own_index[2];
   uint32_t keys[kDrawWarps], low_keys[kDrawWarps];
-  int found, first, crossing;
+  int first, crossing;
 };
 
 template <int N>
@@ -188,11 +182,11 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
     }
     return;
   }
+  if (C > 1) draw_arrive();  // (waited for in front of the first word to another CTA)
   const int chunk = p.run * kDrawThreads, c0 = min(V, rank * chunk), n_here = min(V - c0, chunk);  // (rank * chunk < 2^31: the host checks)
   const float* x = p.logits + (size_t)row * p.stride + c0;
   if (tid < 256) sh.powers[tid] = kPowers[tid];
   if (tid == 0) {
-    sh.found = 0x7fffffff;
     sh.first = 0x7fffffff;
     sh.crossing = 0x7fffffff;
   }
@@ -261,15 +255,27 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
   __syncthreads();
   top_key = __reduce_max_sync(0xffffffffu, lane < kDrawWarps ? sh.keys[lane] : 0u);
   low_key = __reduce_min_sync(0xffffffffu, lane < kDrawWarps ? sh.low_keys[lane] : 0xffffffffu);
-  if (C > 1) {
-    if (tid == 0) {
-      sh.own_key[0] = top_key;
-      sh.own_key[1] = low_key;
+  int turn = 0;
+  // A word to slot s of every CTA's inbox; from warp 0, by a lane for each of them.
+  auto send = [&](int s, double v) {
+    if (C == 1) {
+      if (lane == 0) sh.inbox[turn][0][s] = v;
+    } else if (lane < C) {
+      put_f64(draw_remote(&sh.inbox[turn][rank][s], lane), v);
     }
-    draw_barrier();
-    top_key = __reduce_max_sync(0xffffffffu, lane < C ? remote_u32(draw_remote(&sh.own_key[0], lane)) : 0u);
-    low_key = __reduce_min_sync(0xffffffffu, lane < C ? remote_u32(draw_remote(&sh.own_key[1], lane)) : 0xffffffffu);
+  };
+  auto meet = [&]() {
+    if (C > 1) draw_barrier(); else __syncthreads();
+  };
+  if (C > 1) draw_wait();
+  if (warp == 0) {
+    send(0, top_key);
+    send(1, low_key);
   }
+  meet();
+  top_key = __reduce_max_sync(0xffffffffu, lane < C ? (uint32_t)sh.inbox[turn][lane][0] : 0u);
+  low_key = __reduce_min_sync(0xffffffffu, lane < C ? (uint32_t)sh.inbox[turn][lane][1] : 0xffffffffu);
+  turn ^= 1;
   low_key += 1u;
   const float t = p.temperature[draw];
   const int i0 = min(n_here, tid * p.run), i1 = min(n_here, i0 + p.run);
@@ -299,7 +305,6 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
     }
   };
   auto most_of = [](const float (&v)[4]) { return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])); };
-  int turn = 0;
   // Sums over the cluster, the same in every thread: NM of masses (a warp's in their own type, the others in 64 bits) and NC of integers
   // (four of them at most, and then four masses).
   auto cluster_sums = [&](auto masses, auto counts, const auto& part, auto& m, int (&n)[4]) {
@@ -330,40 +335,34 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
 #pragma unroll
         for (int e = 0; 2 * e < NC; ++e) c[e] += __shfl_xor_sync(0xffffffffu, c[e], o);
       }
-      if (w == 0) {
+      // (lane 16 h + w has them for CTA w)
+      if (w < C) {
+        double* mine = &sh.inbox[turn][rank][h];
+        const uint32_t to = C > 1 ? draw_remote(mine, w) : draw_addr(mine);
 #pragma unroll
         for (int e = 0; 2 * e < NM; ++e)
-          if (2 * e + h < NM) sh.sums[turn][2 * e + h] = a[e];
+          if (2 * e + h < NM) put_f64(to + 16 * e, a[e]);
 #pragma unroll
         for (int e = 0; 2 * e < NC; ++e)
-          if (2 * e + h < NC) sh.sums[turn][4 + 2 * e + h] = c[e];
+          if (2 * e + h < NC) put_f64(to + 32 + 16 * e, c[e]);
       }
     }
-    if (C > 1) {
-      draw_barrier();
-      if (warp == 0) {  // lane 8 c + s: sums s of CTAs c, c + 4, ...
-        const int s = lane & 7;
-        double sum = 0.0;
-        if (s < NM || (s >= 4 && s < 4 + NC)) {
-          double v[4];
+    meet();
+    // every warp by itself; lane 8 c + s: sums s of CTAs c, c + 4, ...
+    const int s = lane & 7, c = lane >> 3;
+    double sum = 0.0;
+    if (s < NM || (s >= 4 && s < 4 + NC)) {
+      double v[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int c = (lane >> 3) + 4 * e;
-            v[e] = c < C ? remote_f64(draw_remote(&sh.sums[turn][s], c)) : 0.0;
-          }
-          sum = (v[0] + v[1]) + (v[2] + v[3]);
-        }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-        if (lane < 8) sh.result[lane] = sum;
-      }
+      for (int e = 0; e < 4; ++e) v[e] = c + 4 * e < C ? sh.inbox[turn][c + 4 * e][s] : 0.0;
+      sum = (v[0] + v[1]) + (v[2] + v[3]);
     }
-    __syncthreads();
-    const double* from = C > 1 ? sh.result : sh.sums[turn];
+    sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
 #pragma unroll
-    for (int s = 0; s < NM; ++s) m[s] = from[s];
+    for (int e = 0; e < NM; ++e) m[e] = __shfl_sync(0xffffffffu, sum, e);
 #pragma unroll
-    for (int s = 0; s < NC; ++s) n[s] = (int)from[4 + s];
+    for (int e = 0; e < NC; ++e) n[e] = (int)__shfl_sync(0xffffffffu, sum, 4 + e);
     turn ^= 1;
   };
   int token = 0;
@@ -376,14 +375,10 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
           break;
         }
       __syncthreads();
-      if (C > 1) {
-        draw_barrier();
-        int lowest = 0x7fffffff;
-        for (int c = 0; c < C; ++c) lowest = min(lowest, (int)remote_u32(draw_remote(&sh.first, c)));
-        token = lowest;
-      } else {
-        token = sh.first;
-      }
+      if (warp == 0) send(0, sh.first);
+      meet();
+      token = (int)__reduce_min_sync(0xffffffffu, lane < C ? (uint32_t)sh.inbox[turn][lane][0] : 0x7fffffffu);
+      turn ^= 1;
     } else {
       const double inv_t = 1.0 / (double)t, per_bit = inv_t * 1.4426950408889634074;  // z / ln 2 of a logit's distance
       auto mass_of = [&](float v) -> double { return exp2_down(((double)v - (double)top) * per_bit, sh.powers); };
@@ -423,6 +418,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
         double above = 0.0;    // of the logits above `hi`
         int inside = held_by_k, mine = 0;  // logits between, and this thread's of them
         bool by_key = false, sure = false;
+        int from_s = 0, to_s = -1;  // the counts of the last pass whose difference is what each CTA has between
         double part = -1.0;  // of what is between, how much lies above the place that is searched for, about
         if (by_mass) {
           // In 32 bits first, down to where the sums' roundings (2^-16 of them is more than those make) leave it open; then one pass in 64 bits
@@ -572,15 +568,21 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
           }
           by_key = false;
           double held = v[0] - v[1];
-          if (above + v[3] >= need) { lo = k3; inside = n[3]; mine = own3; held = v[3]; }
-          else if (above + v[2] >= need) { above += v[3]; lo = k2; hi = k3 - 1u; inside = n[2] - n[3]; mine = own2 - own3; held = v[2] - v[3]; }
-          else if (above + v[1] >= need) { above += v[2]; lo = k1; hi = k2 - 1u; inside = n[1] - n[2]; mine = own1 - own2; held = v[1] - v[2]; }
-          else { above += v[1]; hi = k1 - 1u; inside = n[0] - n[1]; by_key = wide; mine = own0 - own1; }
+          if (above + v[3] >= need) { lo = k3; inside = n[3]; mine = own3; held = v[3]; from_s = 3; to_s = -1; }
+          else if (above + v[2] >= need) { above += v[3]; lo = k2; hi = k3 - 1u; inside = n[2] - n[3]; mine = own2 - own3; held = v[2] - v[3]; from_s = 2; to_s = 3; }
+          else if (above + v[1] >= need) { above += v[2]; lo = k1; hi = k2 - 1u; inside = n[1] - n[2]; mine = own1 - own2; held = v[1] - v[2]; from_s = 1; to_s = 2; }
+          else { above += v[1]; hi = k1 - 1u; inside = n[0] - n[1]; by_key = wide; mine = own0 - own1; from_s = 0; to_s = 1; }
           over_key = 0xffffffffu;
           if (by_mass) part = (need - above) / fmax(held, 1e-300);  // (a tail's numbers fall off too fast for that)
         }
         if (lo >= hi) return lo;
-        // the few between, in the order of their indices, by every CTA
+        // the few between go to every CTA, in the order of their indices: behind those of the CTAs in front, as the last pass counted them
+        int there = 0;
+        if (lane < C) {
+          const double* counts = sh.inbox[turn ^ 1][lane] + 4;
+          there = (int)(counts[from_s] - (to_s >= 0 ? counts[to_s] : 0.0));
+        }
+        int base = __reduce_add_sync(0xffffffffu, lane < rank ? there : 0);
         int before = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -589,54 +591,32 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
         }
         if (lane == 31) sh.keys[warp] = before;
         __syncthreads();
-        int base = 0, all = 0;
-        for (int w = 0; w < kDrawWarps; ++w) {
-          if (w < warp) base += sh.keys[w];
-          all += sh.keys[w];
-        }
+        base += __reduce_add_sync(0xffffffffu, lane < warp ? sh.keys[lane] : 0u);
         int to = base + before - mine;
         const int full = base + before;
         const float lo_x = of_key(lo), over_x = of_key(hi + 1u);
-        for (int i = i0; to < full; i += 4) {
+        for (int i = i0; to < full && i < i1; i += 4) {
           float v[4];
           four(i, v);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (v[e] >= lo_x && !(v[e] >= over_x)) {
-              sh.listed[to] = order_key(v[e]);
-              sh.listed_mass[to++] = by_mass ? mass_of(v[e]) : 1.0;
+            if (v[e] >= lo_x && !(v[e] >= over_x) && to < kListed) {
+              const uint32_t key = order_key(v[e]);
+              const double mass = by_mass ? mass_of(v[e]) : 1.0;
+              for (int c = 0; c < C; ++c) {
+                put_u32(C > 1 ? draw_remote(&sh.listed[to], c) : draw_addr(&sh.listed[to]), key);
+                put_f64(C > 1 ? draw_remote(&sh.listed_mass[to], c) : draw_addr(&sh.listed_mass[to]), mass);
+              }
+              ++to;
             }
         }
-        if (tid == 0) sh.own_index[0] = all;
-        if (C > 1) draw_barrier(); else __syncthreads();
-        // each of them is tried by a thread of rank 0's numbering: what reaches it
+        const int n_all = min(inside, kListed);
+        if (tid >= n_all && tid < kListed) sh.listed[tid] = 0u;  // (no logit's)
+        meet();
+        // each of them is tried by a thread: what reaches it
         uint32_t best = lo;
-        const int theirs = lane < C ? (C > 1 ? (int)remote_u32(draw_remote(&sh.own_index[0], lane)) : all) : 0;
-        int n_all = theirs;  // the lists' lengths, added up
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int other = __shfl_up_sync(0xffffffffu, n_all, o);
-          if (lane >= o) n_all += other;
-        }
-        int from_rank = -1, from = 0;
-#pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          const int end = __shfl_sync(0xffffffffu, n_all, c), n = __shfl_sync(0xffffffffu, theirs, c);
-          if (tid < end && tid >= end - n) {
-            from_rank = c;
-            from = tid - (end - n);
-          }
-        }
-        n_all = __shfl_sync(0xffffffffu, n_all, 31);
-        const uint32_t key = from_rank >= 0 ? (C > 1 ? remote_u32(draw_remote(&sh.listed[from], from_rank)) : sh.listed[from]) : 0u;
-        const double weight = from_rank >= 0 ? (C > 1 ? remote_f64(draw_remote(&sh.listed_mass[from], from_rank)) : sh.listed_mass[from]) : 0.0;
-        if (C > 1) draw_barrier(); else __syncthreads();  // (everyone has what it needs of the others' lists)
-        if (tid < kListed) {
-          sh.listed[tid] = key;
-          sh.listed_mass[tid] = weight;
-        }
-        __syncthreads();
-        if (from_rank >= 0) {
+        const uint32_t key = tid < n_all ? sh.listed[tid] : 0u;
+        if (tid < n_all) {
           double sum[4] = {above, 0.0, 0.0, 0.0};
           for (int j = 0; j < n_all; j += 4)  // (what is behind the last is key 0)
 #pragma unroll
@@ -721,33 +701,20 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
         all += sh.parts[w][0];
       }
       newest = (int)__reduce_max_sync(0xffffffffu, lane < kDrawWarps ? sh.keys[lane] : 0u) - 1;
-      if (tid == 0) {
-        sh.sums[turn][0] = all;
-        sh.own_index[1] = newest < 0 ? -1 : c0 + newest;
-      }
-      if (C > 1) draw_barrier(); else __syncthreads();
       if (warp == 0) {
-        double theirs = 0.0;
-        int newest_there = -1;
-        if (lane < C) {
-          theirs = C > 1 ? remote_f64(draw_remote(&sh.sums[turn][0], lane)) : all;
-          newest_there = C > 1 ? (int)remote_u32(draw_remote(&sh.own_index[1], lane)) : newest < 0 ? -1 : c0 + newest;
-        }
-        double total = 0.0, here = 0.0;
-        for (int r = 0; r < C; ++r) {
-          if (r == rank) here = total;
-          total += __shfl_sync(0xffffffffu, theirs, r);
-        }
-        newest_there = __reduce_max_sync(0xffffffffu, newest_there);
-        if (lane == 0) {
-          sh.result[0] = total;
-          sh.result[1] = here;
-          sh.result[2] = newest_there;
-        }
+        send(0, all);
+        send(1, newest < 0 ? -1.0 : (double)(c0 + newest));
       }
-      __syncthreads();
-      const double total = sh.result[0], here = sh.result[1];
-      const int last = (int)sh.result[2];
+      meet();
+      const double theirs = lane < C ? sh.inbox[turn][lane][0] : 0.0;
+      const int last = __reduce_max_sync(0xffffffffu, lane < C ? (int)sh.inbox[turn][lane][1] : -1);
+      double so_far = theirs;
+#pragma unroll
+      for (int o = 1; o < kMostCluster; o <<= 1) {
+        const double other = __shfl_up_sync(0xffffffffu, so_far, o);
+        if (lane >= o) so_far += other;
+      }
+      const double total = __shfl_sync(0xffffffffu, so_far, C - 1), here = rank ? __shfl_sync(0xffffffffu, so_far, rank - 1) : 0.0;
       turn ^= 1;
       if (quick == low_key && !(mp > 0.f)) whole = total;
       whole = t == 1.f ? whole : -1.0;
@@ -757,10 +724,10 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
       if (c > 0.0 && here + front + behind > target) atomicMin(&sh.crossing, tid);
       __syncthreads();
       const int crossing = sh.crossing;
+      int token_here = -1;
       if (crossing >> 5 == warp) {
         double run = __shfl_sync(0xffffffffu, here + front + (behind - c), crossing & 31);
         const int end = min(n_here, (crossing + 1) * p.run);
-        int token_here = -1;
         for (int j0 = min(n_here, crossing * p.run); j0 < end; j0 += 32) {
           const int i = j0 + lane;
           const double m = i < end ? kept(at(i)) : 0.0;
@@ -778,15 +745,13 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
           if (some) token_here = j0 + 31 - __clz((int)some);  // (its last kept one, should rounding have it)
           run += __shfl_sync(0xffffffffu, sum, 31);
         }
-        if (lane == 0) sh.found = c0 + token_here;
+        if (lane == 0 && token_here >= 0) sh.first = c0 + token_here;
       }
       __syncthreads();
-      if (C > 1) {
-        draw_barrier();  // (the first warp of the first CTA writes the answer)
-        token = (int)__reduce_min_sync(0xffffffffu, warp == 0 && rank == 0 && lane < C ? remote_u32(draw_remote(&sh.found, lane)) : 0x7fffffffu);
-      } else {
-        token = sh.found;
-      }
+      if (warp == 0) send(0, sh.first);
+      meet();
+      token = (int)__reduce_min_sync(0xffffffffu, lane < C ? (uint32_t)sh.inbox[turn][lane][0] : 0x7fffffffu);
+      turn ^= 1;
       if (token == 0x7fffffff) token = last;  // (u of one and more, or none of the runs by rounding: the last kept one)
     }
   }
@@ -811,7 +776,6 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
     }
   }
   if (rank == 0 && tid == 0) p.out[draw] = token;
-  if (C > 1) draw_barrier();  // nobody leaves while its shared memory is read
 }
 
 }  // namespace ftk
