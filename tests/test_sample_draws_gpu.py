@@ -68,7 +68,7 @@ def check(x, rows, t, k, p, mp, u):
         # sums of up to 2^18 terms in 64 bits are off by 2^-34 of the mass at the very most
         assert got[r] == token or near < 2.0 ** -34, (r, got[r], token, near, kept, [b(a)[r] for a in (t, k, p, mp, u)])
         if got[r] == token:
-            assert lp[r] == logp or abs(lp[r] - logp) <= 2.0 ** -23 * max(1.0, abs(logp)), (r, lp[r], logp)
+            assert lp[r] == float(torch.tensor(logp, dtype=torch.float64).float()) or abs(lp[r] - logp) <= 2.0 ** -23 * max(1.0, abs(logp)), (r, lp[r], logp)
 
 
 def rows_of(kind, n, vocab, rng):
@@ -122,6 +122,40 @@ def test_a_large_vocabulary(kind):
     u = rng.random(R)
     check(x, rng.integers(0, 3, R), rng.choice([0.5, 1.0, 1.4], R), rng.choice([0, 0, 40, 5000], R), rng.choice([1.0, 0.9, 0.999], R),
           rng.choice([0.0, 0.05], R), u)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["normal", "masked", "infinite"])
+def test_rows_beyond_shared_memory(kind):
+    """Longer than a cluster's CTAs hold: read again in every pass."""
+    rng = np.random.default_rng(77)
+    vocab, R = 460001, 12
+    x = rows_of("masked" if kind == "masked" else "normal", 2, vocab, rng)
+    if kind == "infinite":
+        x[0, [5, 123456, 460000]] = np.inf
+        x[1, ::3] = np.inf
+        u = rng.random(R).astype(np.float32)
+        rows = np.arange(R) % 2
+        got, lp = draws(torch.from_numpy(x).to(DEV), rows, 0.7, rng.choice([0, 1, 40], R), rng.choice([1.0, 0.5], R), rng.choice([0.0, 0.1], R), u)
+        for r in range(R):  # of equals all stay
+            at = np.flatnonzero(x[rows[r]] == np.inf)
+            assert got[r] == at[min(int(np.float64(u[r]) * len(at)), len(at) - 1)] and np.isclose(lp[r], -np.log(len(at)), rtol=2e-7, atol=0)
+        return
+    check(x, rng.integers(0, 2, R), rng.choice([0.5, 1.0, 1.4], R), rng.choice([0, 0, 40, 5000], R), rng.choice([1.0, 0.9, 0.999], R),
+          rng.choice([0.0, 0.05], R), rng.random(R))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [300, 32003])
+def test_temperatures_and_logits_at_the_ends_of_32_bits(vocab):
+    rng = np.random.default_rng(vocab)
+    R = 24
+    x = np.stack([rng.normal(0, s, vocab) for s in (1e-30, 1.0, 1e30)]).astype(np.float32)
+    x[1, 7] = np.finfo(np.float32).max
+    x[1, 9] = np.finfo(np.float32).min
+    rows = np.arange(R) % 3
+    check(x, rows, rng.choice([1e-38, 1e-30, 1e-3, 1.0, 1e30, 3e38], R), rng.choice([0, 3, 250], R), rng.choice([1.0, 0.9, 0.3], R),
+          rng.choice([0.0, 0.05], R), rng.random(R))
 
 
 @pytest.mark.gpu
