@@ -105,6 +105,11 @@ class Scheduler:
         if rid is None:
             rid = self._next_id
             self._next_id += 1
+        live = [*self.waiting, *self.running]
+        taken = {r.rid for r in live} if params.n > 1 else set()
+        names = [(rid, j) for j in range(1, params.n)]
+        if taken.intersection(names) or any((r.rid, j) in (rid, *names) for r in live for j in range(1, r.to_fork + 1)):
+            raise SchedulerError(f"request {rid!r}: a continuation has or will have that name, or one of its own would have another request's")
         prompt = [int(t) for t in prompt]
         req = Request(rid=rid, prompt=prompt, params=params, max_tokens=params.max_tokens)
         vocab = self.engine.spec.vocab_size

@@ -12,7 +12,7 @@ from freetoken_b200.cache.pages import PagePool
 from freetoken_b200.config.spec import PagedKVNeed, StateNeed
 from freetoken_b200.engine.engine import StepEntry
 from freetoken_b200.engine.scheduler import Scheduler
-from freetoken_b200.errors import CacheError, ConfigError
+from freetoken_b200.errors import CacheError, ConfigError, SchedulerError
 from freetoken_b200.kernels import ops
 from freetoken_b200.sampling import Sampler, SamplingParams
 from helpers import make_engine, model_folder, tokens_for
@@ -365,3 +365,18 @@ def test_the_sampler_keeps_requests_that_do_not_draw_as_they_are(cpu, monkeypatc
             sampler.launch(logits[:2], [SamplingParams(n=3)] * 4, list("abcd"), [0] * 4, rows=bad)
     with pytest.raises(ValueError):
         sampler.launch(logits[:2], [SamplingParams()] * 2, list("ab"), [0] * 2, rows=[1, 1])
+
+
+def test_names_of_continuations_are_refused_to_others(cpu, tmp_path_factory):
+    sched, _ = scheduler(tmp_path_factory, reqs=6, pages=64)
+    several, one = SamplingParams(max_tokens=4, n=3, temperature=1.0, ignore_eos=True), SamplingParams(max_tokens=4, ignore_eos=True)
+    sched.add_request([1, 2, 3], several, rid="a")
+    for rid, params in ((("a", 2), one), (("a", 1), several)):
+        with pytest.raises(SchedulerError, match="name"):
+            sched.add_request([5], params, rid=rid)
+    sched.add_request([5, 6], one, rid=("a", 3))  # nobody's
+    sched.add_request([5, 6], one, rid=("b", 1))
+    with pytest.raises(SchedulerError, match="name"):
+        sched.add_request([5], several, rid="b")
+    sched.run()
+    assert all(len(sched.done[r].output) == 4 for r in ("a", ("a", 1), ("a", 2), ("a", 3), ("b", 1)))
