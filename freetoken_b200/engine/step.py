@@ -221,7 +221,8 @@ class StepBuilder:
 
     def shared_plan(self, need, n_heads: int, n_kv_heads: int, head_dim: int, dtype, worth) -> Any:
         """Key of the work list over shared keys for mixers whose cache is ``need``'s, or None where the step's requests share nothing that
-        is ``worth(saved keys, requests)`` it.  What of it does not depend on the requests' lengths is kept while they share the same pages."""
+        is ``worth(saved keys, own keys, requests, KV heads, head size, dtype)`` it.  What of it does not depend on the requests' lengths is
+        kept while they share the same pages."""
         if len(self.requests) < 2:
             return None
         cache = self.engine.cache
@@ -233,7 +234,11 @@ class StepBuilder:
             return self._shared[what]
         self._shared[what] = None
         spans = cache.shared_spans(group, self.requests)
-        if not spans or not worth(sum((len(m) - 1) * (end - start) for m, start, end in spans), len(self.requests)):
+        if not spans:
+            return None
+        read = sum(len(m) * (end - start) for m, start, end in spans)  # by those who share, each for itself
+        saved = read - sum(end - start for _, start, end in spans)
+        if not worth(saved, int(self._segments[:, 1].sum()) - read, len(self.requests), n_kv_heads, head_dim, dtype):
             return None
         known = self.engine.shared_layouts.get(what)
         if known is None or known[0] is not spans:  # (the same spans as long as nobody forks, ends or moves)

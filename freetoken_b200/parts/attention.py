@@ -45,6 +45,7 @@ TC_PAIR_MIN_SPAN = 16384       # (rounded up to 2^n): such tiles are cut along t
 AHEAD_MOST_BYTES = 40_000_000  # largest weight that a single token's attention brings into L2 (see GQAttention._weight_ahead)
 SHARED_MIN_KEYS = 512    # keys that sharing has to save a decode step, in all
 SHARED_MIN_KEYS_EACH = 100  # and for each of its requests
+SHARED_MOST_OWN = 1.0    # of the own keys that sharing_pays allows
 TC_MIN_DECODE_SPAN = 0   # decode steps go there from this length of the longest request (rounded up to 2^n) on
 
 
@@ -117,13 +118,20 @@ def attention_tile_rows(dtype: torch.dtype, decode_only: bool = False, group: in
     return attention_kernel_form(dtype, decode_only, group, n_tokens, head_dim, page_size, window, longest_span)[0]
 
 
-def sharing_pays(saved: int, requests: int) -> bool:
-    """Whether a decode step of ``requests`` that would read ``saved`` keys again that another of them reads is taken by
-    ``ops.shared_attention``: from a hundred keys a request on.  A layer's attention, ``ops.paged_attention`` against it, 48 heads on 8 of
-    128: 16 requests over 64 shared keys 8.2 and 10.0 us, over 256 11.0 and 11.1, over 1,024 17.9 and 14.1, over 16,384 156 and 38; 48 over 64
-    14.9 and 16.4, over 256 22.0 and 14.6, over 16,384 422 and 52; 3 over 256 10.3 and 9.0, over 4,096 16.4 and 17.7, over 16,384 36.1 and
-    27.9; 16 on 4 of 64, 48 over 256 16.9 and 7.9, in 32 bits 19.2 and 17.1."""
-    return saved >= SHARED_MIN_KEYS and saved >= SHARED_MIN_KEYS_EACH * requests
+def sharing_pays(saved: int, own: int, requests: int, kv_heads: int, head_dim: int, dtype: torch.dtype) -> bool:
+    """Whether a decode step of ``requests`` that would read ``saved`` keys again that another of them reads, and ``own`` keys that nobody
+    else does, is taken by ``ops.shared_attention``: from a hundred saved keys a request on.  A layer's attention, ``ops.paged_attention`` against
+    it, 48 heads on 8 of 128: 16 requests over 64 shared keys 8.2 and 10.0 us, over 256 11.0 and 11.1, over 1,024 17.9 and 14.1, over
+    16,384 156 and 38; 48 over 64 14.9 and 16.4, over 256 22.0 and 14.6, over 16,384 422 and 52; 3 over 256 10.3 and 9.0, over 4,096 16.4 and
+    17.7, over 16,384 36.1 and 27.9; 16 on 4 of 64, 48 over 256 16.9 and 7.9, in 32 bits 19.2 and 17.1.
+
+    Own keys are read by a few CTAs a request and KV head there, where the other spreads them over the GPU, so as they grow it falls behind, the
+    later the more requests and heads there are: 4 requests over 16,384 shared keys with 2,000 own keys each 50 and 44 us, with 4,000 56 and
+    59, with 16,000 84 and 130; 16 with 2,000 173 and 65, over 2,048 with 1,000 36 and 34, with 2,000 48 and 51; 2 over 16,384 with 500 27.4
+    and 26.9, with 2,000 30 and 38.  16 on 4 of 64: 4 over 16,384 with 4,000 26 and 20, with 16,000 37 and 42; 16 over 2,048 with 4,000 38 and
+    26, with 16,000 77 and 91; in 32 bits 4 over 2,048 with 1,000 24 and 22, with 2,000 30 and 33."""
+    part = requests * kv_heads / (24 if dtype == torch.float32 else 42 if head_dim <= 64 else 170)
+    return saved >= SHARED_MIN_KEYS and saved >= SHARED_MIN_KEYS_EACH * requests and own <= SHARED_MOST_OWN * part * saved
 
 
 @MIXERS.register("gqa_attention")

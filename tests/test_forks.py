@@ -14,6 +14,7 @@ from freetoken_b200.engine.engine import StepEntry
 from freetoken_b200.engine.scheduler import Scheduler
 from freetoken_b200.errors import CacheError, ConfigError, SchedulerError
 from freetoken_b200.kernels import ops
+from freetoken_b200.parts.attention import sharing_pays
 from freetoken_b200.sampling import Sampler, SamplingParams
 from helpers import make_engine, model_folder, tokens_for
 from plain.m3_plain import PlainM3
@@ -207,6 +208,7 @@ def test_forked_requests_give_the_plain_models_logits(name, cpu, monkeypatch, tm
     calls = []
     monkeypatch.setattr("freetoken_b200.parts.attention.SHARED_MIN_KEYS", 1)
     monkeypatch.setattr("freetoken_b200.parts.attention.SHARED_MIN_KEYS_EACH", 0)
+    monkeypatch.setattr("freetoken_b200.parts.attention.SHARED_MOST_OWN", 1e9)
     monkeypatch.setattr(ops, "shared_attention", lambda *a, **k: (calls.append(1), fork_refs.shared_attention(*a, **k))[1])
     folder = model_folder(tmp_path_factory.getbasetemp(), name, ALL[name])
     plain = PlainM3(folder)
@@ -380,3 +382,22 @@ def test_names_of_continuations_are_refused_to_others(cpu, tmp_path_factory):
         sched.add_request([5], several, rid="b")
     sched.run()
     assert all(len(sched.done[r].output) == 4 for r in ("a", ("a", 1), ("a", 2), ("a", 3), ("b", 1)))
+
+
+def test_sharing_is_used_where_it_pays(cpu, monkeypatch, tmp_path_factory):
+    pays = lambda n, shared, own, kv=8, dim=128, dt=torch.bfloat16: sharing_pays((n - 1) * shared, n * own, n, kv, dim, dt)  # noqa: E731
+    # the figures beside the rule: who is faster there
+    assert [pays(16, x, 60) for x in (64, 1024, 16384)] == [False, True, True] and [pays(48, x, 60) for x in (64, 256, 16384)] == [False, True, True]
+    assert [pays(4, 16384, x) for x in (500, 2000, 4000, 16000)] == [True, True, False, False]
+    assert [pays(16, 2048, x) for x in (1000, 2000)] == [True, False] and [pays(2, 16384, x) for x in (500, 2000)] == [True, False]
+    assert [pays(4, 16384, x, 4, 64) for x in (4000, 16000)] == [True, False] and [pays(4, 2048, x, 4, 64, torch.float32) for x in (1000, 2000)] == [True, False]
+    # and what a step says of itself: two of three requests share 8 keys, the third is long
+    folder = model_folder(tmp_path_factory.getbasetemp(), "A", TINY_A)
+    eng = make_engine(folder, "float32", "cpu", 4, 40, max_step=64, reqs=4)
+    eng.step([StepEntry("a", list(range(1, 11)))])
+    eng.step([StepEntry("c", list(range(1, 31)))])
+    eng.fork("a", ["b"])
+    seen = []
+    monkeypatch.setattr("freetoken_b200.parts.attention.sharing_pays", lambda *a: seen.append(a) or False)
+    eng.step([StepEntry("a", [3], [0]), StepEntry("b", [4], [0]), StepEntry("c", [5], [0])])
+    assert seen and all(a[:3] == (8, 3 + 3 + 31, 3) for a in seen)

@@ -27,6 +27,7 @@ def sharing(monkeypatch):
     """Every decode step whose requests share a page takes the shared list; how often that was."""
     monkeypatch.setattr("freetoken_b200.parts.attention.SHARED_MIN_KEYS", 1)
     monkeypatch.setattr("freetoken_b200.parts.attention.SHARED_MIN_KEYS_EACH", 0)
+    monkeypatch.setattr("freetoken_b200.parts.attention.SHARED_MOST_OWN", 1e9)
     ops.variant_counts(reset=True)
     return lambda: {k: v for k, v in ops.variant_counts().items() if k.startswith("shared attention")}
 
