@@ -193,15 +193,15 @@ class Engine:
         return self.model.workspace_bytes(self.max_step_tokens) + (1 << 28)
 
     def _metadata_capacity(self) -> int:
-        """int32 elements the packed metadata of the largest step can take."""
+        """int32 elements the packed metadata of the largest step can take (``plan_ints`` of them a work list)."""
         T = self.max_step_tokens
         S = self.config.max_running_req
         n_groups = max(1, len(self.cache.paged))
         core = 3 * T + 8 * S + 64
         per_group = T + 2 * (T // self.config.page_size + 2 * S + 4)
         n_plans = max(1, 2 * len({m.plan_key() for m in self.model.mixers() if hasattr(m, "plan_key")}))
-        items = 8 * (T + S + 2 * self.sm_count * 32)
-        return core + n_groups * per_group + n_plans * items + 4096
+        self.plan_ints = 8 * (T + S + 2 * self.sm_count * 32)
+        return core + n_groups * per_group + n_plans * self.plan_ints + 4096
 
     # ------------------------------------------------------------------ requests
     def open(self, rid: Hashable) -> None:

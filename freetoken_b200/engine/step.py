@@ -248,6 +248,8 @@ class StepBuilder:
         plan = known[1].plan(self._segments[:, 1])
         if self.fixed:
             plan = plan.rounded()
+        if sum(arr.size + ALIGN for _, arr in plan.sections()) > self.engine.plan_ints:
+            return None  # (more than the step's metadata has room for: long chains of forks)
         key = self._shared[what] = ("shared_attention", *what, *plan.key())
         self.plans[key] = plan
         for name, arr in plan.sections():

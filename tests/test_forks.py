@@ -401,3 +401,31 @@ def test_sharing_is_used_where_it_pays(cpu, monkeypatch, tmp_path_factory):
     monkeypatch.setattr("freetoken_b200.parts.attention.sharing_pays", lambda *a: seen.append(a) or False)
     eng.step([StepEntry("a", [3], [0]), StepEntry("b", [4], [0]), StepEntry("c", [5], [0])])
     assert seen and all(a[:3] == (8, 3 + 3 + 31, 3) for a in seen)
+
+
+def test_lists_that_have_no_room_are_not_made(cpu, monkeypatch, tmp_path_factory):
+    """A chain of forks, each of the one before: the list over what they share grows with the square of its length."""
+    for name, value in (("SHARED_MIN_KEYS", 1), ("SHARED_MIN_KEYS_EACH", 0), ("SHARED_MOST_OWN", 1e9)):
+        monkeypatch.setattr(f"freetoken_b200.parts.attention.{name}", value)
+    calls = []
+    monkeypatch.setattr(ops, "shared_attention", lambda *a, **k: (calls.append(1), fork_refs.shared_attention(*a, **k))[1])
+    folder = model_folder(tmp_path_factory.getbasetemp(), "A", TINY_A)
+    plain = PlainM3(folder)
+    eng = make_engine(folder, "float32", "cpu", 4, 300, max_step=64, reqs=12)
+    seqs = {0: tokens_for(plain.cfg.vocab, 4, 1)}
+    eng.step([StepEntry(0, seqs[0])])
+    for i in range(1, 12):
+        more = tokens_for(plain.cfg.vocab, 4, i)
+        eng.fork(i - 1, [i])
+        seqs[i] = seqs[i - 1] + more
+        eng.step([StepEntry(i, more)])
+    for room in (eng.plan_ints, 300):
+        eng.plan_ints, before = room, len(calls)
+        entries = []
+        for r in seqs:
+            seqs[r] = seqs[r] + [r + 1]
+            entries.append(StepEntry(r, [r + 1], [0]))
+        got = eng.step(entries).logits
+        assert (len(calls) > before) == (room > 300)
+        for row, r in zip(got, seqs):
+            torch.testing.assert_close(row, plain.logits(seqs[r])[-1], rtol=1e-4, atol=2e-5)
