@@ -18,8 +18,10 @@
 // the barrier would be one trip more a pass.
 // What bounds it: for one draw the passes one after the other (a barrier of the cluster each, a microsecond or so with the wait for the
 // slowest CTA); for many the instructions of the passes (0.7 of the issue slots taken, the 64-bit pipe 0.12): so logits lie in shared
-// memory as numbers, four to a load, and are compared as such.  Rows of 200,000 logits: one draw without filters 20 us, min-p 17,
-// top-k 50, top-p and min-p 32, top-p alone 38; 96 draws from 24 rows 78, 119 and (top-p) 172 us; 256 rows with min-p 128.
+// memory as numbers, four to a load, and are compared as such; and where top-k (of 128 at most) or top-p leaves no more than kListed of a
+// row, every CTA lists those and does the rest in the list (one draw with all filters 33 -> 24 us, 96 of them 119 -> 92).  Rows of
+// 200,000 logits: one draw without filters 20 us, min-p 17, top-k 50, top-p and min-p 24, top-p alone 38; 96 draws from 24 rows 77, 92 and
+// (top-p of flat rows) 168 us; 256 rows with min-p 126.
 #include "common.cuh"
 
 namespace ftk {
@@ -153,12 +155,16 @@ __device__ __forceinline__ T warp_sum_of(T v) {
 
 struct DrawShared {
   double powers[256];
-  double parts[kDrawWarps][8];  // the warps' sums
+  union {
+    double parts[kDrawWarps][8];  // the warps' sums
+    uint32_t listed_at[kListed];  // where the listed logits stand in the row
+  };
   int counts[kDrawWarps][4];
   double inbox[2][kMostCluster][8];  // what every CTA of the cluster has sent to this one: in turns, so that one barrier a pass is enough
   double listed_mass[kListed];
   uint32_t listed[kListed];
   uint32_t keys[kDrawWarps], low_keys[kDrawWarps];
+  double reached;
   int first, crossing;
 };
 
@@ -365,6 +371,16 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
     for (int e = 0; e < NC; ++e) n[e] = (int)__shfl_sync(0xffffffffu, sum, 4 + e);
     turn ^= 1;
   };
+  // The largest of a number of every thread.
+  auto block_max = [&](uint32_t v) -> uint32_t {
+    v = __reduce_max_sync(0xffffffffu, v);
+    __syncthreads();
+    if (lane == 0) sh.keys[warp] = v;
+    __syncthreads();
+    v = __reduce_max_sync(0xffffffffu, lane < kDrawWarps ? sh.keys[lane] : 0u);
+    __syncthreads();
+    return v;
+  };
   int token = 0;
   double whole_row = -1.0;  // the row's mass at temperature 1, where it is known
   if (top_key != 0u) {
@@ -410,6 +426,9 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
         q3 = min(max(q3, q2), max(hi, lo + 1u));
         return wide;
       };
+      // Where few logits are left of the row, every CTA lists them all, and what follows is done in the list.
+      int n_list = 0;
+      double held_here = 0.0;  // what reaches the logit that this thread has of the list
       // The largest key from `lo` on at which the number (by_mass: the mass) of the logits that reach it is `need` (by_mass: `need` of what
       // reaches `lo`) or more; `lo` where not even that has as many.  (Logits are compared as numbers: what lies above key `hi` reaches the
       // number of key hi + 1.)
@@ -417,7 +436,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
         uint32_t hi = top_key;
         double above = 0.0;    // of the logits above `hi`
         int inside = held_by_k, mine = 0;  // logits between, and this thread's of them
-        bool by_key = false, sure = false;
+        bool by_key = false, sure = false, list_all = !by_mass && need <= kListed / 2;
         int from_s = 0, to_s = -1;  // the counts of the last pass whose difference is what each CTA has between
         double part = -1.0;  // of what is between, how much lies above the place that is searched for, about
         if (by_mass) {
@@ -494,20 +513,28 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
             for (int e = 0; e < 4; ++e) {
               const double m = mass_of(x4[e]);
               if (x4[e] >= limit_x) v[0] += m;
-              if (x4[e] >= lo_x) { v[1] += m; ++n[0]; }
+              if (x4[e] >= lo_x) { v[1] += m; ++n[0]; ++n[1]; }
               if (x4[e] >= over_x) { v[2] += m; --n[0]; }
             }
           }
           mine = n[0];
+          const int reaching = n[1];
           over_mine = v[2];
           over_key = hi + 1u;
-          cluster_sums(SumCount<3>(), SumCount<1>(), v, v, n);
+          cluster_sums(SumCount<3>(), SumCount<2>(), v, v, n);
           if (limit == low_key) whole = v[0];
           need *= v[0];
           if (!(need > 0.0)) return top_key;
           above = v[2];
           inside = n[0];
           sure = v[1] >= need && v[2] < need;
+          list_all = sure && n[1] <= kListed;
+          if (list_all) {
+            above = 0.0;
+            inside = n[1];
+            mine = reaching;
+            from_s = 1;
+          }
           if (!sure) {  // (not the place after all: from the start)
             over_key = 0xffffffffu;
             lo = limit;
@@ -521,7 +548,8 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
           uint32_t k1, k2, k3;
           const bool wide = candidates(lo, hi, by_key || pass % 3 == 2, part, k1, k2, k3);
           const float lo_x = of_key(lo), over_x = of_key(hi + 1u), q1 = of_key(k1), q2 = of_key(k2), q3 = of_key(k3);
-          double v[4] = {0.0, 0.0, 0.0, 0.0};  // mass (or number) and number of the logits that reach lo, q1, q2, q3, and no more than hi
+          // mass (or number) and number of the logits that reach lo, q1, q2, q3, and (where not all of them will be listed) no more than hi
+          double v[4] = {0.0, 0.0, 0.0, 0.0};
           int n[4] = {0, 0, 0, 0}, own_over = 0;
           if (by_mass) {
             for (int i = i0; i < i1; i += 4) {
@@ -548,7 +576,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
                 n[1] += x4[e] >= q1;
                 n[2] += x4[e] >= q2;
                 n[3] += x4[e] >= q3;
-                own_over += x4[e] >= over_x;
+                own_over += !list_all && x4[e] >= over_x;
               }
             }
 #pragma unroll
@@ -568,14 +596,15 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
           }
           by_key = false;
           double held = v[0] - v[1];
+          const int beyond1 = list_all ? 0 : n[1], beyond2 = list_all ? 0 : n[2], beyond3 = list_all ? 0 : n[3];
           if (above + v[3] >= need) { lo = k3; inside = n[3]; mine = own3; held = v[3]; from_s = 3; to_s = -1; }
-          else if (above + v[2] >= need) { above += v[3]; lo = k2; hi = k3 - 1u; inside = n[2] - n[3]; mine = own2 - own3; held = v[2] - v[3]; from_s = 2; to_s = 3; }
-          else if (above + v[1] >= need) { above += v[2]; lo = k1; hi = k2 - 1u; inside = n[1] - n[2]; mine = own1 - own2; held = v[1] - v[2]; from_s = 1; to_s = 2; }
-          else { above += v[1]; hi = k1 - 1u; inside = n[0] - n[1]; by_key = wide; mine = own0 - own1; from_s = 0; to_s = 1; }
+          else if (above + v[2] >= need) { above += list_all ? 0.0 : v[3]; lo = k2; hi = k3 - 1u; inside = n[2] - beyond3; mine = own2 - (list_all ? 0 : own3); held = v[2] - v[3]; from_s = 2; to_s = list_all ? -1 : 3; }
+          else if (above + v[1] >= need) { above += list_all ? 0.0 : v[2]; lo = k1; hi = k2 - 1u; inside = n[1] - beyond2; mine = own1 - (list_all ? 0 : own2); held = v[1] - v[2]; from_s = 1; to_s = list_all ? -1 : 2; }
+          else { above += list_all ? 0.0 : v[1]; hi = k1 - 1u; inside = n[0] - beyond1; by_key = wide; mine = own0 - (list_all ? 0 : own1); from_s = 0; to_s = list_all ? -1 : 1; }
           over_key = 0xffffffffu;
           if (by_mass) part = (need - above) / fmax(held, 1e-300);  // (a tail's numbers fall off too fast for that)
         }
-        if (lo >= hi) return lo;
+        if (lo >= hi && !(list_all && inside <= kListed)) return lo;
         // the few between go to every CTA, in the order of their indices: behind those of the CTAs in front, as the last pass counted them
         int there = 0;
         if (lane < C) {
@@ -594,7 +623,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
         base += __reduce_add_sync(0xffffffffu, lane < warp ? sh.keys[lane] : 0u);
         int to = base + before - mine;
         const int full = base + before;
-        const float lo_x = of_key(lo), over_x = of_key(hi + 1u);
+        const float lo_x = of_key(lo), over_x = list_all ? NAN : of_key(hi + 1u);  // (nothing reaches NaN)
         for (int i = i0; to < full && i < i1; i += 4) {
           float v[4];
           four(i, v);
@@ -602,10 +631,11 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
           for (int e = 0; e < 4; ++e)
             if (v[e] >= lo_x && !(v[e] >= over_x) && to < kListed) {
               const uint32_t key = order_key(v[e]);
-              const double mass = by_mass ? mass_of(v[e]) : 1.0;
+              const double mass = by_mass || list_all ? mass_of(v[e]) : 1.0;
               for (int c = 0; c < C; ++c) {
                 put_u32(C > 1 ? draw_remote(&sh.listed[to], c) : draw_addr(&sh.listed[to]), key);
                 put_f64(C > 1 ? draw_remote(&sh.listed_mass[to], c) : draw_addr(&sh.listed_mass[to]), mass);
+                if (list_all) put_u32(C > 1 ? draw_remote(&sh.listed_at[to], c) : draw_addr(&sh.listed_at[to]), (uint32_t)(c0 + i + e));
               }
               ++to;
             }
@@ -618,18 +648,16 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
         const uint32_t key = tid < n_all ? sh.listed[tid] : 0u;
         if (tid < n_all) {
           double sum[4] = {above, 0.0, 0.0, 0.0};
+          int reach = 0;
           for (int j = 0; j < n_all; j += 4)  // (what is behind the last is key 0)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (sh.listed[j + e] >= key) sum[e] += sh.listed_mass[j + e];
-          if ((sum[0] + sum[1]) + (sum[2] + sum[3]) >= need) best = key;
+              if (sh.listed[j + e] >= key) { sum[e] += sh.listed_mass[j + e]; ++reach; }
+          held_here = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          if ((!by_mass && list_all ? (double)reach : held_here) >= need) best = key;
         }
-        best = __reduce_max_sync(0xffffffffu, best);
-        __syncthreads();
-        if (lane == 0) sh.keys[warp] = best;
-        __syncthreads();
-        best = __reduce_max_sync(0xffffffffu, lane < kDrawWarps ? sh.keys[lane] : 0u);
-        __syncthreads();
+        if (list_all) n_list = n_all;
+        best = block_max(best);
         return best;
       };
       uint32_t limit = low_key;  // (key 0 is never drawn)
@@ -639,9 +667,43 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
         held_by_k = k;  // (about: ties stay)
       }
       const float tp = p.top_p[draw];
-      if (tp < 1.f) limit = search(true, limit, fmax((double)tp, 0.0));
+      const bool k_listed = n_list > 0;
+      if (tp < 1.f && !k_listed) limit = search(true, limit, fmax((double)tp, 0.0));
       const float mp = p.min_p[draw];
       const double least = mp > 0.f ? fmin(log((double)mp), 0.0) : -INFINITY;
+      if (n_list > 0) {
+        const uint32_t key = tid < n_list ? sh.listed[tid] : 0u;
+        if (tp < 1.f && k_listed) {  // of what top-k left
+          if (key == limit) sh.reached = held_here;  // (the same from every thread)
+          __syncthreads();
+          const double need = fmax((double)tp, 0.0) * sh.reached;
+          limit = need > 0.0 ? block_max(key >= limit && held_here >= need ? key : limit) : top_key;
+        }
+        double m = tid < n_list ? sh.listed_mass[tid] : 0.0;
+        if (!(key >= limit && (mp > 0.f ? ((double)of_key(key) - (double)top) * inv_t >= least : true))) m = 0.0;
+        double behind = m;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double other = __shfl_up_sync(0xffffffffu, behind, o);
+          if (lane >= o) behind += other;
+        }
+        __syncthreads();
+        if (lane == 31) sh.listed_mass[warp] = behind;
+        __syncthreads();
+        double front = 0.0, total = 0.0;
+#pragma unroll
+        for (int w = 0; w < kListed / 32; ++w) {
+          if (w == warp) front = total;
+          total += sh.listed_mass[w];
+        }
+        const double target = (double)p.u[draw] * total;
+        // the first that passes the target, or (u of one and more, or by rounding) the last that is kept: as 2^31 less its place, or its place
+        const bool past = m > 0.0 && front + behind > target;
+        const uint32_t pick = block_max(past ? 0x80000000u - (uint32_t)tid : m > 0.0 ? (uint32_t)tid : 0u);
+        token = (int)sh.listed_at[pick > kListed ? 0x80000000u - pick : pick];
+        whole_row = t == 1.f ? whole : -1.0;
+        __syncthreads();  // (the places lie where sums will)
+      } else {
       uint32_t quick = limit;  // most of what min-p leaves out is told by its key (which is rounded, so four steps are left for the exact question)
       if (mp > 0.f) {
         const uint32_t near = order_key(clean((float)((double)top + least * (double)t)));
@@ -753,6 +815,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
       token = (int)__reduce_min_sync(0xffffffffu, lane < C ? (uint32_t)sh.inbox[turn][lane][0] : 0x7fffffffu);
       turn ^= 1;
       if (token == 0x7fffffff) token = last;  // (u of one and more, or none of the runs by rounding: the last kept one)
+      }
     }
   }
   if (p.logprobs) {
