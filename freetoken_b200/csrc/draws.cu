@@ -819,18 +819,24 @@ __global__ void __launch_bounds__(kDrawThreads, 2) draw_kernel(const __grid_cons
     }
   }
   if (p.logprobs) {
-    // In 32 bits: an exponential is within 2^-22.5 (and its argument's rounding), the errors of many are random.
+    // What lies within a factor of 20 of the largest in 64 bits, so that a few large terms leave no error; the others in 32 bits, where an
+    // exponential is within 2^-22.5 (and its argument's rounding) and the errors of many are random.
     double v[4] = {whole_row, 0.0, 0.0, 0.0};
     if (top_key != 0u && whole_row < 0.0) {
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
       for (int i = i0; i < i1; i += 4) {
         float v4[4];
         four(i, v4);
+        if (most_of(v4) - top > -3.f) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] += __expf(v4[e] - top);
+          for (int e = 0; e < 4; ++e) v[1] += exp2_down(((double)v4[e] - (double)top) * 1.4426950408889634074, sh.powers);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum[e] += __expf(v4[e] - top);
+        }
       }
       int n[4];
-      v[0] = (double)(sum[0] + sum[1]) + (double)(sum[2] + sum[3]);
+      v[0] = ((double)(sum[0] + sum[1]) + (double)(sum[2] + sum[3])) + v[1];
       cluster_sums(SumCount<1>(), SumCount<0>(), v, v, n);
     }
     if (rank == 0 && tid == 0) {

@@ -1204,8 +1204,8 @@ def sample_draws(logits: torch.Tensor, rows: Optional[torch.Tensor], temperature
     stays, equal logits stay or go together.  ``out[r]`` is the first index whose running kept mass exceeds ``u[r]`` times the
     kept mass.  ``logprobs[r]`` (float32, optional) is ``log_softmax(x)[out[r]]``, at temperature one and without the filters.
 
-    Sums and exponentials are 64-bit (those of the log-probability, beside a temperature other than one, 32-bit exponentials); how many draws
-    there are changes the order of the sums, and so the last bits of a log-probability at most.  NaN counts as ``-inf``; a row of nothing else gives token 0 and ``-inf``.  A draw whose row
+    Sums and exponentials are 64-bit (but small terms of the log-probability's, beside a temperature other than one, have 32-bit exponentials);
+    how many draws there are changes the order of the sums, and so the last bits of a log-probability at most.  NaN counts as ``-inf``; a row of nothing else gives token 0 and ``-inf``.  A draw whose row
     does not exist gives -1.  ``logits`` may be a view of rows that are farther apart.  :func:`sample` is the same without min-p, several
     draws a row and log-probabilities, in 32-bit sums; its results are its own."""
     if logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_cuda or (logits.shape[1] > 1 and logits.stride(1) != 1):
