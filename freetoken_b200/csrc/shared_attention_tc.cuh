@@ -37,7 +37,8 @@ constexpr int kShSmem(int d) { return (2 + kShKStages(d) + kShVStages(d)) * (d /
 // Exponentials: the special-function unit gives 16 an SM and cycle, 2,048 cycles for the 32,768 of a key tile and two query tiles, as much
 // as the products take.  Of every eight columns kShPoly pairs go another way: 2^x = 2^n 2^r with n = x rounded to the nearest integer (by adding and
 // taking off 1.5 2^23) and 2^r on [-1/2, 1/2] by a polynomial of degree four, the minimax fit of the relative error by Lawson's
-// iteration (2.7e-6 evaluated in 32 bits; the probability is rounded to 2^-9 right behind), two numbers an instruction.
+// iteration (2.7e-6 evaluated in 32 bits; the probability is rounded to 2^-8 right behind), two numbers an instruction.  None, one and two
+// of four pairs: 60.2, 58.3 and 60.1 us for 64 requests over nested spans, 26.9, 26.6 and 27.4 for 200 of heads of 64.
 constexpr int kShPoly = 1;
 __device__ __forceinline__ uint64_t sh_pair(float a, float b) {
   uint64_t r;
