@@ -297,7 +297,8 @@ class GQAttention(Mixer):
         # forward() of the same step runs the kernel this work list was made for
         self._step_span = builder.longest_span()
         self._step_shared = None
-        if builder.decode_only and self.own_kv and not self.log_dist_bias and self.window is None and getattr(builder, "requests", None):
+        if builder.decode_only and self.own_kv and not self.log_dist_bias and self.window is None and self.scale > 0 \
+                and getattr(builder, "requests", None):
             self._step_shared = builder.shared_plan(self.cache_need(), self.n_heads, self.n_kv_heads, self.pad_dim, self.env.dtype,
                                                     sharing_pays)
             if self._step_shared is not None:
