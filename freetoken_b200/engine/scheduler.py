@@ -24,6 +24,7 @@ not fit even in an empty cache is finished at once with ``finish_reason="error"`
 A request for several continuations (``SamplingParams.n``) is admitted with request slots and pages for all of them.  Its prompt is
 read once; in the step that ends it the request is forked (:meth:`Engine.fork`), and the continuations' first tokens are drawn from
 the same row of logits.  From then on they are requests like any other, named ``(rid, 1)`` to ``(rid, n - 1)`` beside ``rid``.
+The prompt's full pages are reserved for all of them together, until the last has ended, whichever that is.
 """
 
 from __future__ import annotations
@@ -38,6 +39,14 @@ from .engine import StepEntry
 
 
 @dataclass
+class Family:
+    """Requests that continue one prompt."""
+
+    members: int      # that have not ended
+    pages: List[int]  # reserved per cache group for what they all hold: the prompt's full pages
+
+
+@dataclass
 class Request:
     rid: Hashable
     prompt: List[int]
@@ -49,11 +58,12 @@ class Request:
     finished: bool = False
     finish_reason: Optional[str] = None
     error: Optional[str] = None
-    reserved: List[int] = field(default_factory=list)  # pages reserved per cache group
+    reserved: List[int] = field(default_factory=list)  # pages reserved per cache group (beside the family's)
     in_flight: int = 0  # tokens sampled on the device and not yet read by the host
     source: Optional[Tuple[Any, int]] = None  # (device tensor, index) of the newest such token
     logprob: Optional[float] = None  # sum over its tokens' log-probabilities, where they are known (SamplingParams.draws)
     to_fork: int = 0  # continuations beside this one that are still to begin
+    family: Optional[Family] = None
 
     @property
     def decoding(self) -> bool:
@@ -146,11 +156,26 @@ class Scheduler:
         self.engine.fork(req.rid, names)
         base = self.engine.cache.pages_to_admit(len(req.prompt) + req.max_tokens, min(self.max_step_tokens, self.max_extend))
         more = self._fork_needs(req, base)
-        req.to_fork, req.reserved = 0, base
-        copies = [Request(rid=name, prompt=req.prompt, params=req.params, max_tokens=req.max_tokens, fed=req.fed, reserved=more) for name in names]
+        req.family = Family(1 + len(names), [b - m for b, m in zip(base, more)])
+        req.to_fork, req.reserved = 0, more
+        copies = [Request(rid=name, prompt=req.prompt, params=req.params, max_tokens=req.max_tokens, fed=req.fed, reserved=more,
+                          family=req.family) for name in names]
         at = self.running.index(req) + 1
         self.running[at:at] = copies
         return copies
+
+    def _end(self, req: Request) -> None:
+        """A running request is over: its pages and slot go back, and what was reserved for it (for its family, with the last of it)."""
+        self.running.remove(req)
+        self.engine.close(req.rid)
+        back = [req.reserved]
+        if req.family is not None:
+            req.family.members -= 1
+            if not req.family.members:
+                back.append(req.family.pages)
+        for pages in back:
+            for i, n in enumerate(pages):
+                self.reserved[i] -= n
 
     def _reject(self, req: Request, why: str) -> Hashable:
         req.finished, req.finish_reason, req.error = True, "error", why
@@ -247,10 +272,7 @@ class Scheduler:
                 finished.append(req.rid)
                 # a step that already runs with this request is ordered before any later step
                 # on the stream, so its pages can go back now
-                self.running.remove(req)
-                self.engine.close(req.rid)
-                for i, n in enumerate(req.reserved):
-                    self.reserved[i] -= n
+                self._end(req)
                 self.done[req.rid] = req
         report = StepReport(flight.entries, sampled, finished, flight.admitted)
         if self.status is not None:
@@ -306,10 +328,7 @@ class Scheduler:
                 return True
         for req in self.running:
             if req.rid == rid:
-                self.running.remove(req)
-                self.engine.close(rid)
-                for i, n in enumerate(req.reserved):
-                    self.reserved[i] -= n
+                self._end(req)
                 req.finished, req.finish_reason = True, "abort"
                 self.done[rid] = req
                 return True
