@@ -64,6 +64,7 @@ class Request:
     logprob: Optional[float] = None  # sum over its tokens' log-probabilities, where they are known (SamplingParams.draws)
     to_fork: int = 0  # continuations beside this one that are still to begin
     family: Optional[Family] = None
+    continues: bool = False  # a prompt that another request has read
 
     @property
     def decoding(self) -> bool:
@@ -118,7 +119,8 @@ class Scheduler:
         live = [*self.waiting, *self.running]
         taken = {r.rid for r in live} if params.n > 1 else set()
         names = [(rid, j) for j in range(1, params.n)]
-        if taken.intersection(names) or any((r.rid, j) in (rid, *names) for r in live for j in range(1, r.to_fork + 1)):
+        has = any(r.continues and r.rid == rid for r in live)
+        if has or taken.intersection(names) or any((r.rid, j) in (rid, *names) for r in live for j in range(1, r.to_fork + 1)):
             raise SchedulerError(f"request {rid!r}: a continuation has or will have that name, or one of its own would have another request's")
         prompt = [int(t) for t in prompt]
         req = Request(rid=rid, prompt=prompt, params=params, max_tokens=params.max_tokens)
@@ -159,7 +161,7 @@ class Scheduler:
         req.family = Family(1 + len(names), [b - m for b, m in zip(base, more)])
         req.to_fork, req.reserved = 0, more
         copies = [Request(rid=name, prompt=req.prompt, params=req.params, max_tokens=req.max_tokens, fed=req.fed, reserved=more,
-                          family=req.family) for name in names]
+                          family=req.family, continues=True) for name in names]
         at = self.running.index(req) + 1
         self.running[at:at] = copies
         return copies

@@ -5,6 +5,7 @@ import torch
 
 import fork_refs
 from freetoken_b200.engine.scheduler import Scheduler
+from freetoken_b200.errors import SchedulerError
 from freetoken_b200.sampling import Sampler, SamplingParams
 from helpers import make_engine, model_folder, tokens_for
 from tiny_configs import ALL
@@ -60,3 +61,20 @@ def test_pages_of_a_prompt_stay_reserved_while_a_continuation_holds_them(how, or
     sched.drain()
     assert sched.reserved == [0] * len(sched.reserved) and held(sched) == [0] * len(sched.reserved)
     assert sched.done["later"].finish_reason == "length" and all(n in sched.done for n in names)
+
+
+def test_the_name_of_a_running_continuation_is_refused(cpu, tmp_path_factory):
+    sched = scheduler(tmp_path_factory, pages=40)
+    V = sched.engine.spec.vocab_size
+    several, one = SamplingParams(max_tokens=6, temperature=1.0, seed=1, n=2), SamplingParams(max_tokens=3)
+    sched.add_request(tokens_for(V, 5, 1), several, rid="a")
+    sched.step()
+    assert {r.rid for r in sched.running} == {"a", ("a", 1)}
+    for params in (one, several):
+        with pytest.raises(SchedulerError, match="name"):
+            sched.add_request(tokens_for(V, 5, 2), params, rid=("a", 1))
+    sched.run()
+    assert sched.reserved == [0]
+    sched.add_request(tokens_for(V, 5, 2), one, rid=("a", 1))  # free again
+    sched.run()
+    assert len(sched.done[("a", 1)].output) == 3 and sched.reserved == [0]
