@@ -193,10 +193,10 @@ class Scheduler:
                 break  # (slots that continuations will take are not free)
             if any(r + n > p for r, n, p in zip(self.reserved, req.reserved, self.pool_pages)):
                 break  # the first request that does not fit stops the pass
+            self.engine.open(req.rid)
             self.waiting.popleft()
             for i, n in enumerate(req.reserved):
                 self.reserved[i] += n
-            self.engine.open(req.rid)
             self.running.append(req)
             admitted.append(req.rid)
         return admitted

@@ -5,7 +5,7 @@ import torch
 
 import fork_refs
 from freetoken_b200.engine.scheduler import Scheduler
-from freetoken_b200.errors import SchedulerError
+from freetoken_b200.errors import CacheError, SchedulerError
 from freetoken_b200.sampling import Sampler, SamplingParams
 from helpers import make_engine, model_folder, tokens_for
 from tiny_configs import ALL
@@ -78,3 +78,19 @@ def test_the_name_of_a_running_continuation_is_refused(cpu, tmp_path_factory):
     sched.add_request(tokens_for(V, 5, 2), one, rid=("a", 1))  # free again
     sched.run()
     assert len(sched.done[("a", 1)].output) == 3 and sched.reserved == [0]
+
+
+def test_a_request_that_cannot_be_opened_stays_in_line(cpu, tmp_path_factory):
+    """Under the name of one that runs: nothing is reserved for it and it is not lost."""
+    sched = scheduler(tmp_path_factory, pages=40)
+    V = sched.engine.spec.vocab_size
+    sched.add_request(tokens_for(V, 5, 1), SamplingParams(max_tokens=6), rid="a")
+    sched.step()
+    before = list(sched.reserved)
+    sched.add_request(tokens_for(V, 5, 2), SamplingParams(max_tokens=3), rid="a")
+    with pytest.raises(CacheError, match="already open"):
+        sched.step()
+    assert sched.reserved == before and len(sched.waiting) == 1
+    assert sched.abort("a") and not sched.waiting  # (those in line first)
+    sched.run()
+    assert len(sched.done["a"].output) == 6 and sched.reserved == [0]
