@@ -97,6 +97,13 @@ class PagedGroup:
         at = row * self.width + block
         self.updates.extend(zip(range(at, at + len(pages)), pages))
 
+    def drop_stale(self) -> None:
+        """Forget the entries on their way to the device that say no longer what the table does: of a request that has ended or a step that
+        did not run.  (A fork copies rows on the device, so what comes behind it must hold; and a step's entries are written at
+        once, so no place may come twice.)"""
+        table = self.table_host.reshape(-1)
+        self.updates = [(at, page) for at, page in self.updates if table[at] == page]
+
     def held_pages(self, row: int, n_blocks: int) -> List[int]:
         pages = self.table_host[row, :n_blocks]
         return pages[pages != NULL_PAGE].tolist()
@@ -285,6 +292,8 @@ class CacheManager:
             first = g.first_live.pop(req.row, 0)
             g.table_host[req.row, :min(g.kept_blocks, first, n_blocks)] = NULL_PAGE
             g.table_host[req.row, first:n_blocks] = NULL_PAGE
+            if g.updates:
+                g.drop_stale()
         self.slots.free(req.state_slot)
         self._rows.append(req.row)
         self._spans.clear()
@@ -494,6 +503,8 @@ class CacheManager:
                     if g.table_host[r.row, b] != NULL_PAGE:
                         g.set_entry(r.row, b, NULL_PAGE)
             r.reserved = 0
+        for g in self.paged:
+            g.drop_stale()
         self._in_step = []
 
     def take_updates(self, group: int) -> List[Tuple[int, int]]:

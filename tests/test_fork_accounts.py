@@ -4,6 +4,8 @@ import pytest
 import torch
 
 import fork_refs
+from freetoken_b200.cache.manager import CacheManager
+from freetoken_b200.config.spec import PagedKVNeed
 from freetoken_b200.engine.scheduler import Scheduler
 from freetoken_b200.errors import CacheError, SchedulerError
 from freetoken_b200.sampling import Sampler, SamplingParams
@@ -94,3 +96,69 @@ def test_a_request_that_cannot_be_opened_stays_in_line(cpu, tmp_path_factory):
     assert sched.abort("a") and not sched.waiting  # (those in line first)
     sched.run()
     assert len(sched.done["a"].output) == 6 and sched.reserved == [0]
+
+
+def ship(cache):
+    for g in cache.paged:
+        for at, page in cache.take_updates(g.index):
+            g.table_dev.view(-1)[at] = page
+
+
+def fork(cache, src, copies):
+    for g, pairs in zip(cache.paged, cache.fork(src, copies).pages):
+        rows = [(cache.requests[src].row, cache.requests[c].row) for c in copies]
+        fork_refs.copy_slots([g.table_dev.unsqueeze(0)], torch.tensor(rows))
+
+
+def grow(cache, rid, n):
+    cache.begin_step([(rid, n)])
+    ship(cache)
+    cache.end_step()
+
+
+def tables_agree(cache):
+    cache.check()
+    for r in cache.requests.values():
+        blocks = -(-r.length // cache.page_size)
+        for g in cache.paged:
+            assert g.table_dev[r.row, :blocks].tolist() == g.table_host[r.row, :blocks].tolist()
+
+
+def cache_of(pages=40, reqs=4):
+    return CacheManager([(0, PagedKVNeed((("k", 1, 2),), None))], 4, pages, reqs, 64, torch.float32, torch.device("cpu"), max_step_tokens=16)
+
+
+@pytest.mark.parametrize("how", ["a step that did not run", "a fork that ended at once"])
+def test_what_a_row_was_to_become_ends_with_its_request(how):
+    """Changes of a block-table row that no step has carried yet must not reach the row's next owner, whose row a fork copies on the device."""
+    cache = cache_of()
+    cache.open("a")
+    grow(cache, "a", 14)
+    if how == "a step that did not run":
+        cache.open("x")
+        cache.begin_step([("x", 9)])
+        cache.abort_step()
+        cache.close("x")
+    else:
+        cache.open("y")
+        grow(cache, "y", 6)
+        cache.fork("y", ["x"])
+        cache.close("x")
+    fork(cache, "a", ["c"])  # on x's row
+    ship(cache)
+    tables_agree(cache)
+
+
+def test_a_step_that_is_tried_again_writes_every_place_once():
+    cache = cache_of()
+    cache.open("a")
+    cache.open("b")
+    cache.begin_step([("a", 9), ("b", 7)])
+    cache.abort_step()
+    cache.begin_step([("b", 7), ("a", 9)])  # (other pages)
+    updates = cache.take_updates(0)
+    assert len({at for at, _ in updates}) == len(updates) == 5
+    for at, page in updates:
+        cache.paged[0].table_dev.view(-1)[at] = page
+    cache.end_step()
+    tables_agree(cache)
