@@ -78,6 +78,7 @@ class PagedGroup:
         self.table_host = np.zeros((max_requests, width), dtype=np.int32)
         self.table_dev = torch.zeros((max_requests, width), dtype=torch.int32, device=device)
         self.updates: List[Tuple[int, int]] = []  # (flat index into the table, page)
+        self.taken: List[Tuple[int, int]] = []  # those that the step in flight carries
         self.first_live: Dict[int, int] = {}  # row -> first logical block still held (behind the kept ones)
 
     def bytes_per_page(self, itemsize: int) -> int:
@@ -487,6 +488,8 @@ class CacheManager:
             r.reserved = 0
             for g in self.paged:
                 self._release_dead(g, r)
+        for g in self.paged:
+            g.taken = []
         self._in_step = []
 
     def abort_step(self) -> None:
@@ -503,7 +506,8 @@ class CacheManager:
                     if g.table_host[r.row, b] != NULL_PAGE:
                         g.set_entry(r.row, b, NULL_PAGE)
             r.reserved = 0
-        for g in self.paged:
+        for g in self.paged:  # (what waited for the step, forks' own pages among it, waits for the next)
+            g.updates, g.taken = g.taken + g.updates, []
             g.drop_stale()
         self._in_step = []
 
@@ -511,6 +515,8 @@ class CacheManager:
         """Block-table changes since the last call, as (flat index, page), oldest first."""
         g = self.paged[group]
         out, g.updates = g.updates, []
+        if self._in_step:
+            g.taken = g.taken + out
         return out
 
     # ------------------------------------------------------------------ invariants

@@ -6,10 +6,12 @@ import torch
 import fork_refs
 from freetoken_b200.cache.manager import CacheManager
 from freetoken_b200.config.spec import PagedKVNeed
+from freetoken_b200.engine.engine import StepEntry
 from freetoken_b200.engine.scheduler import Scheduler
 from freetoken_b200.errors import CacheError, SchedulerError
 from freetoken_b200.sampling import Sampler, SamplingParams
 from helpers import make_engine, model_folder, tokens_for
+from plain.m3_plain import PlainM3
 from tiny_configs import ALL
 
 
@@ -162,3 +164,45 @@ def test_a_step_that_is_tried_again_writes_every_place_once():
         cache.paged[0].table_dev.view(-1)[at] = page
     cache.end_step()
     tables_agree(cache)
+
+
+def test_what_a_failed_step_was_to_carry_goes_with_the_next():
+    """A fork's own page waits for a step; where that step fails behind the point at which it took the changes, the next one takes them."""
+    cache = cache_of()
+    cache.open("a")
+    grow(cache, "a", 14)
+    fork(cache, "a", ["b"])
+    cache.begin_step([("b", 3)])
+    assert cache.take_updates(0)
+    cache.abort_step()
+    cache.begin_step([("a", 1)])
+    ship(cache)
+    cache.end_step()
+    tables_agree(cache)
+    grow(cache, "b", 5)
+    tables_agree(cache)
+
+
+def test_a_step_that_fails_before_its_launches_loses_no_pages(cpu, monkeypatch, tmp_path_factory):
+    """Through the engine: a fork, a step that fails while its metadata is made, and then the continuation's logits."""
+    folder = model_folder(tmp_path_factory.getbasetemp(), "A", ALL["A"])
+    plain = PlainM3(folder)
+    V = plain.cfg.vocab
+    eng = make_engine(folder, "float32", "cpu", 4, pages=40, reqs=4)
+    a = tokens_for(V, 14, 1)
+    eng.step([StepEntry("a", a)])
+    eng.fork("a", ["b"])
+    upload = eng.buffers.upload
+
+    def fails(sections):
+        raise RuntimeError("no room")
+
+    monkeypatch.setattr(eng.buffers, "upload", fails)
+    with pytest.raises(RuntimeError):
+        eng.step([StepEntry("b", [5], [0])])
+    monkeypatch.setattr(eng.buffers, "upload", upload)
+    eng.step([StepEntry("a", [7], [0])])  # (the parent goes on in its last page: the fork must not read that)
+    got = eng.step([StepEntry("b", [5], [0])]).logits
+    torch.testing.assert_close(got[0], plain.logits(a + [5])[-1], rtol=1e-4, atol=2e-5)
+    got = eng.step([StepEntry("b", [6], [0])]).logits
+    torch.testing.assert_close(got[0], plain.logits(a + [5, 6])[-1], rtol=1e-4, atol=2e-5)
