@@ -222,10 +222,21 @@ class Engine:
     def fork(self, rid: Hashable, copies: Sequence[Hashable]) -> None:
         """Open ``copies`` as requests that go on from where ``rid`` is: they share its full pages, and the last, partly filled one and
         recurrent states are copied (on the current stream, behind the steps launched so far).  From then on steps that decode several
-        of them read the shared pages once (:func:`freetoken_b200.kernels.ops.shared_attention`)."""
+        of them read the shared pages once (:func:`freetoken_b200.kernels.ops.shared_attention`).  Where a copy is refused, none is opened."""
         if not copies:
             return
         made = self.cache.fork(rid, copies)
+        try:
+            self._copy_for(made)
+        except Exception:
+            for name in copies:
+                self.cache.close(name)
+            raise
+        if self.config.check_cache:
+            self.cache.check()
+
+    def _copy_for(self, made) -> None:
+        """The copies that a fork leaves to do."""
         put = lambda pairs: torch.tensor(pairs, dtype=torch.int32).to(self.device, non_blocking=True)  # noqa: E731
         for g, pairs in zip(self.cache.paged, made.pages):
             if pairs:
@@ -236,8 +247,6 @@ class Engine:
         tables = [g.table_dev.unsqueeze(0) for g in self.cache.paged]
         if tables:
             ops.copy_slots(tables, put(made.rows))
-        if self.config.check_cache:
-            self.cache.check()
 
     def compact(self) -> List[int]:
         """Move the pages in use to the lowest page numbers and return how many that are, per paged group: behind them the slabs hold

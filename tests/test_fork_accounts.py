@@ -8,7 +8,8 @@ from freetoken_b200.cache.manager import CacheManager
 from freetoken_b200.config.spec import PagedKVNeed
 from freetoken_b200.engine.engine import StepEntry
 from freetoken_b200.engine.scheduler import Scheduler
-from freetoken_b200.errors import CacheError, SchedulerError
+from freetoken_b200.errors import CacheError, KernelError, SchedulerError
+from freetoken_b200.kernels import ops
 from freetoken_b200.sampling import Sampler, SamplingParams
 from helpers import make_engine, model_folder, tokens_for
 from plain.m3_plain import PlainM3
@@ -206,3 +207,23 @@ def test_a_step_that_fails_before_its_launches_loses_no_pages(cpu, monkeypatch, 
     torch.testing.assert_close(got[0], plain.logits(a + [5])[-1], rtol=1e-4, atol=2e-5)
     got = eng.step([StepEntry("b", [6], [0])]).logits
     torch.testing.assert_close(got[0], plain.logits(a + [5, 6])[-1], rtol=1e-4, atol=2e-5)
+
+
+def test_a_fork_whose_copies_fail_opens_nobody(cpu, monkeypatch, tmp_path_factory):
+    folder = model_folder(tmp_path_factory.getbasetemp(), "A", ALL["A"])
+    eng = make_engine(folder, "float32", "cpu", 4, pages=40, reqs=4)
+    eng.step([StepEntry("a", tokens_for(eng.spec.vocab_size, 14, 1))])
+    before = eng.cache.free_pages(), eng.cache.free_request_slots()
+
+    def refused(*args):
+        raise KernelError("tensor is on 'cuda:0', the current device is 'cuda:1'")
+
+    for name in ("copy_pages", "copy_slots"):
+        with monkeypatch.context() as m:
+            m.setattr(ops, name, refused)
+            with pytest.raises(KernelError):
+                eng.fork("a", ["b", "c"])
+        eng.cache.check()
+        assert not eng.is_open("b") and not eng.is_open("c") and (eng.cache.free_pages(), eng.cache.free_request_slots()) == before
+    eng.fork("a", ["b", "c"])
+    eng.cache.check()
