@@ -206,7 +206,6 @@ class CacheManager:
         self._rows: List[int] = list(range(max_requests - 1, -1, -1))
         self.requests: Dict[Hashable, _Request] = {}
         self._in_step: List[Tuple[Hashable, int]] = []
-        self.forks = 0  # forks so far: without one no page is shared
         self._spans: Dict[Any, List[Any]] = {}  # shared_spans of the requests asked about, while nobody forks or moves pages
 
     # ------------------------------------------------------------------ sizing
@@ -300,6 +299,11 @@ class CacheManager:
         self._spans.clear()
 
     # ------------------------------------------------------------------ requests that share
+    @property
+    def sharing(self) -> bool:
+        """Whether any page has several holders."""
+        return any(g.pool.shared for g in self.paged)
+
     def fork_needs(self, rid: Hashable, n: int = 1) -> List[int]:
         """Pages per paged group that ``n`` forks of ``rid`` take at once: one each where its last page is partly filled."""
         partly = int(self.requests[rid].length % self.page_size != 0)
@@ -337,14 +341,13 @@ class CacheManager:
                     page = g.pool.alloc(1)[0]
                     pairs.append((int(g.table_host[src.row, full]), page, partly))
                     g.set_entry(dst.row, full, page)  # (behind the copied row on the device: updates go out with the next step)
-        self.forks += len(copies)
         self._spans.clear()
         return out
 
     def shared_spans(self, group: PagedGroup, rids: Sequence[Hashable]) -> List[Tuple[List[int], int, int]]:
         """Which of ``rids`` (by their places) read the same pages of ``group`` for which positions: (members, start, end), the outermost
         first, positions in whole pages."""
-        if not self.forks or group.need.window is not None:  # (a window passes pages by: its requests read them each for itself)
+        if not group.pool.shared or group.need.window is not None:  # (a window passes pages by: its requests read them each for itself)
             return []
         rows = tuple(self.requests[r].row for r in rids)
         key = (group.index, rows)
@@ -352,7 +355,7 @@ class CacheManager:
         if known is not None:
             return known
         lengths = [self.requests[r].length // self.page_size for r in rids]  # full pages: the others are nobody else's
-        table = group.table_host[list(rows)]
+        table = group.table_host[list(rows), :max(lengths, default=0)]
         spans: List[Tuple[List[int], int, int]] = []
 
         def divide(members: List[int], at: int) -> None:
@@ -426,7 +429,7 @@ class CacheManager:
                 for rid, n in entries:
                     r = self.requests[rid]
                     lo, hi = max(g.first_live[r.row], g.kept_blocks), min(g.dead_blocks(r.length), -(-r.length // self.page_size))
-                    if self.forks:  # (what others hold too does not come back)
+                    if g.pool.shared:  # (what others hold too does not come back)
                         reclaim += sum(p != NULL_PAGE and g.pool.holders(p) == 1 for p in g.table_host[r.row, lo:hi].tolist())
                     else:
                         reclaim += max(0, hi - lo)

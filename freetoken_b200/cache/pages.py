@@ -25,6 +25,7 @@ class PagePool:
         self.num_pages = num_pages
         self._free: List[int] = list(range(num_pages, 0, -1))
         self._held = [0] * (num_pages + 1)  # holders
+        self.shared = 0  # pages of several holders
         self.handed_out = 0  # pages ever handed out (reuse shows as handed_out > num_pages)
 
     @property
@@ -49,6 +50,7 @@ class PagePool:
             if not 1 <= p <= self.num_pages or not self._held[p]:
                 raise CacheError(f"page {p} is held by nobody and cannot be shared")
         for p in pages:
+            self.shared += self._held[p] == 1
             self._held[p] += 1
 
     def holders(self, page: int) -> int:
@@ -61,6 +63,7 @@ class PagePool:
             if not self._held[p]:
                 raise CacheError(f"page {p} freed twice")
             self._held[p] -= 1
+            self.shared -= self._held[p] == 1
             if not self._held[p]:
                 self._free.append(p)
 
@@ -93,3 +96,5 @@ class PagePool:
                 raise CacheError(f"page {p} is in a block table but marked free")
             if self._held[p] != n:
                 raise CacheError(f"page {p} is in {n} block tables but has {self._held[p]} holders")
+        if self.shared != sum(n > 1 for n in times.values()):
+            raise CacheError(f"{self.shared} pages count as shared, {sum(n > 1 for n in times.values())} are")

@@ -355,7 +355,7 @@ class Engine:
                 positions[q0:q0 + n] = np.arange(kv - n, kv)
         builder = StepBuilder(self, [(s.q_len, s.kv_len) for s in segments], fixed=graphable,
                               sm_count=self.sm_count)
-        if self.cache.forks and decode_only:
+        if decode_only and self.cache.sharing:
             builder.requests, builder.table_rows = [e.request_id for e in entries], plan.rows
         builder.add("token_ids", token_ids)
         builder.add("positions", positions)

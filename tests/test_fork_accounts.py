@@ -5,6 +5,7 @@ import torch
 
 import fork_refs
 from freetoken_b200.cache.manager import CacheManager
+from freetoken_b200.cache.pages import PagePool
 from freetoken_b200.config.spec import PagedKVNeed
 from freetoken_b200.engine.engine import StepEntry
 from freetoken_b200.engine.scheduler import Scheduler
@@ -227,3 +228,57 @@ def test_a_fork_whose_copies_fail_opens_nobody(cpu, monkeypatch, tmp_path_factor
         assert not eng.is_open("b") and not eng.is_open("c") and (eng.cache.free_pages(), eng.cache.free_request_slots()) == before
     eng.fork("a", ["b", "c"])
     eng.cache.check()
+
+
+class Spied:
+    """A table that counts what is taken out of it."""
+
+    def __init__(self, table):
+        self.table, self.taken = table, 0
+
+    def __getitem__(self, at):
+        out = self.table[at]
+        self.taken += out.size
+        return out
+
+
+def test_tables_are_compared_only_while_pages_are_shared_and_only_as_far_as_they_reach():
+    cache = cache_of(reqs=6)
+    for rid, n in (("a", 9), ("b", 14), ("c", 3)):
+        cache.open(rid)
+        grow(cache, rid, n)
+    group = cache.paged[0]
+    table, group.table_host = group.table_host, Spied(group.table_host)
+    spy = group.table_host
+    assert cache.shared_spans(group, ["a", "b", "c"]) == [] and not spy.taken and not cache.sharing
+    group.table_host = table
+    fork(cache, "b", ["d"])
+    group.table_host = spy
+    assert cache.sharing and cache.shared_spans(group, ["a", "b", "c", "d"]) == [([1, 3], 0, 12)]
+    assert 0 < spy.taken <= 4 * 3  # (three full pages at most; a row of the table has 16)
+    group.table_host = table
+    cache.close("b")  # one holder is left
+    spy.taken, group.table_host = 0, spy
+    assert cache.shared_spans(group, ["a", "c", "d"]) == [] and not spy.taken and not cache.sharing
+    group.table_host = table
+    cache.check()
+    for rid in "acd":
+        cache.close(rid)
+    cache.check()
+
+
+def test_pages_of_several_holders_are_counted():
+    pool = PagePool(4)
+    a, b = pool.alloc(2)
+    pool.share([a, b, a])
+    assert pool.shared == 2
+    pool.free([a])
+    assert pool.shared == 2
+    pool.free([a, b])
+    pool.check([a, b])
+    assert pool.shared == 0
+    pool.share([b])
+    pool.renumber({b: 3})
+    assert pool.shared == 1
+    pool.free([3, 3, a])
+    assert pool.shared == 0 and pool.free_count == 4
