@@ -568,7 +568,7 @@ __global__ void __launch_bounds__(kRowThreads, DMAX <= 128 ? 4 : 2) own_keys_ker
       else if (part >= n_join && lane < n)
         ml = C > 1 ? make_float2(cluster_f32(of_rank(my_m + r * 4, part - n_join)), cluster_f32(of_rank(my_l + r * 4, part - n_join))) : make_float2(res.m[r], res.l[r]);
       const float m = fmaxf(M[e], warp_max(ml.x)), f = weight<T>(M[e], m), wgt = weight<T>(ml.x, m);
-      L[e] = L[e] * f + warp_sum(wgt != 0.f ? ml.y * wgt : 0.f);
+      L[e] = L[e] * f + warp_sum(ml.y * wgt);  // (a part that holds a NaN has a sum of NaN, whatever it weighs)
       M[e] = m;
       weights[lane][r] = wgt;
       if (lane == 0) {

@@ -1,0 +1,73 @@
+"""Attention over shared keys at its ends: what is not a number in a part that weighs next to nothing."""
+
+import pytest
+import torch
+
+from freetoken_b200.engine.shared_plan import build_shared_plan
+from test_shared_attention_gpu import BF16, DEV, F32, case, run
+
+HEADS, KV, DIM, PAGE = 16, 2, 128, 16
+SCALE = DIM ** -0.5
+
+
+def far_apart(lens, spans, dtype, high):
+    """Keys whose first element puts a score some 280 above the others' where ``high(positions)`` says so: e^-280 is zero in 32 bits."""
+    q, k, v, table = case(lens, spans, HEADS, KV, DIM, PAGE, dtype)
+    q[:, :, 0] = 8.0
+    for i, n in enumerate(lens):
+        pos = torch.arange(n)
+        k[table[i, pos // PAGE].long(), :, pos % PAGE, 0] = torch.where(high(pos), 400.0, 0.0).to(dtype)[:, None]
+    return q, k, v, table
+
+
+FORMS = [(F32, 16), (BF16, 16), (BF16, 256)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("whole", [False, True])
+@pytest.mark.parametrize("dtype,tile_rows", FORMS)
+def test_nan_in_shared_keys_far_below_the_own_ones(dtype, tile_rows, whole):
+    """A score that is no number makes the whole row none, however little its piece weighs beside the others."""
+    lens, spans = [300, 290, 280], [([0, 1], 0, 256)]
+    q, k, v, table = far_apart(lens, spans, dtype, lambda pos: pos >= 256)
+    plan = build_shared_plan(lens, spans, HEADS, KV, DIM, dtype, PAGE, tile_rows=tile_rows).to(DEV)
+    clean = run(q, k, v, table, plan, SCALE)
+    assert torch.isfinite(clean).all()
+    for pos in range(256) if whole else (37,):
+        k[table[0, pos // PAGE].long(), 1, pos % PAGE, 3] = float("nan")
+    got = run(q, k, v, table, plan, SCALE)
+    assert torch.isnan(got[:2, 8:]).all() and torch.equal(got[:2, :8], clean[:2, :8]) and torch.equal(got[2], clean[2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,tile_rows", FORMS)
+def test_nan_in_one_of_many_pieces(dtype, tile_rows):
+    """Pieces beyond one run of the join (32 partial results at a time), the highest scores in the last of them and in the first."""
+    for last in (True, False):
+        lens, spans = [20000, 19990], [([0, 1], 0, 19904)]
+        q, k, v, table = far_apart(lens, spans, dtype, lambda pos: ((19840 <= pos) & (pos < 19904)) if last else pos < 64)
+        plan = build_shared_plan(lens, spans, HEADS, KV, DIM, dtype, PAGE, tile_rows=tile_rows).to(DEV)
+        assert tile_rows == 256 or plan.host.requests[0, 5] > 32
+        clean = run(q, k, v, table, plan, SCALE)
+        assert torch.isfinite(clean).all()
+        for pos in (100, 10000, 19800, 19989):
+            bad = k.clone()
+            bad[table[0, pos // PAGE].long(), 0, pos % PAGE, 3] = float("nan")
+            got = run(q, bad, v, table, plan, SCALE)
+            rows = slice(0, 2) if pos < 19904 else slice(0, 1)
+            assert torch.isnan(got[rows, :8]).all() and torch.equal(got[:, 8:], clean[:, 8:]), (last, pos)
+            if pos >= 19904:
+                assert torch.equal(got[1], clean[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_nan_in_own_keys_of_one_cta_of_a_cluster(dtype):
+    lens, spans = [3000], []
+    q, k, v, table = far_apart(lens, spans, dtype, lambda pos: pos < 64)
+    plan = build_shared_plan(lens, spans, HEADS, KV, DIM, dtype, PAGE).to(DEV)
+    assert plan.host.cluster > 1
+    clean = run(q, k, v, table, plan, SCALE)
+    k[table[0, 2900 // PAGE].long(), 1, 2900 % PAGE, 3] = float("nan")
+    got = run(q, k, v, table, plan, SCALE)
+    assert torch.isfinite(clean).all() and torch.isnan(got[0, 8:]).all() and torch.equal(got[0, :8], clean[0, :8])
