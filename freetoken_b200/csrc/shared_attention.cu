@@ -592,11 +592,9 @@ __global__ void __launch_bounds__(kRowThreads, DMAX <= 128 ? 4 : 2) own_keys_ker
         acc[u].x *= f; acc[u].y *= f; acc[u].z *= f; acc[u].w *= f;
       }
     }
-    auto add = [&](int u, float f, float4 x) {
-      if (f != 0.f) {  // (a part of weight 0 may hold anything)
-        acc[u].x = fmaf(x.x, f, acc[u].x); acc[u].y = fmaf(x.y, f, acc[u].y);
-        acc[u].z = fmaf(x.z, f, acc[u].z); acc[u].w = fmaf(x.w, f, acc[u].w);
-      }
+    auto add = [&](int u, float f, float4 x) {  // (a part of weight 0 too: 0 x NaN is NaN, as it is within a part)
+      acc[u].x = fmaf(x.x, f, acc[u].x); acc[u].y = fmaf(x.y, f, acc[u].y);
+      acc[u].z = fmaf(x.z, f, acc[u].z); acc[u].w = fmaf(x.w, f, acc[u].w);
     };
 #pragma unroll 1
     for (int j = 0; j < n_slots; j += kBatch) {
@@ -609,6 +607,7 @@ __global__ void __launch_bounds__(kRowThreads, DMAX <= 128 ? 4 : 2) own_keys_ker
 #pragma unroll
         for (int e = 0; e < kBatch; ++e) {
           const int at = slots[(j + e) % kJoinRun];
+          x[u][e] = make_float4(0.f, 0.f, 0.f, 0.f);
           if (j + e < n_slots && at >= 0) x[u][e] = __ldcg(reinterpret_cast<const float4*>(o + (size_t)at * p.Hq * D));
         }
       }

@@ -71,3 +71,18 @@ def test_nan_in_own_keys_of_one_cta_of_a_cluster(dtype):
     k[table[0, 2900 // PAGE].long(), 1, 2900 % PAGE, 3] = float("nan")
     got = run(q, k, v, table, plan, SCALE)
     assert torch.isfinite(clean).all() and torch.isnan(got[0, 8:]).all() and torch.equal(got[0, :8], clean[0, :8])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,tile_rows", FORMS)
+def test_nan_values_of_a_piece_that_weighs_nothing(dtype, tile_rows):
+    """0 x NaN is NaN, in a piece of its own as in one tile."""
+    lens, spans = [300, 290, 280], [([0, 1], 0, 256)]
+    q, k, v, table = far_apart(lens, spans, dtype, lambda pos: pos >= 256)
+    plan = build_shared_plan(lens, spans, HEADS, KV, DIM, dtype, PAGE, tile_rows=tile_rows).to(DEV)
+    clean = run(q, k, v, table, plan, SCALE)
+    v[table[0, 37 // PAGE].long(), 1, 37 % PAGE, 5] = float("nan")
+    got = run(q, k, v, table, plan, SCALE)
+    assert torch.isnan(got[:2, 8:, 5]).all()
+    got[:2, 8:, 5], clean[:2, 8:, 5] = 0, 0
+    assert torch.equal(got, clean)
