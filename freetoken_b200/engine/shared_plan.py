@@ -103,7 +103,7 @@ class SharedDevicePlan:
     part_o: Optional[torch.Tensor]   # [slots, heads, head_dim] float32
     part_ml: Optional[torch.Tensor]  # [slots, heads, 2] float32
     host: SharedPlan
-    fixed: Optional[object] = None   # what its launches have in common (made by the first)
+    fixed: Optional[object] = None   # what its launches have in common, and the tensors it was made for
 
 
 def tile_members(n: int, most: int) -> List[Tuple[int, int]]:

@@ -1,4 +1,6 @@
-"""Attention over shared keys at its ends: what is not a number in a part that weighs next to nothing."""
+"""Attention over shared keys at its ends: what is not a number in a part that weighs next to nothing, scratch that was replaced."""
+
+import dataclasses
 
 import pytest
 import torch
@@ -86,3 +88,31 @@ def test_nan_values_of_a_piece_that_weighs_nothing(dtype, tile_rows):
     assert torch.isnan(got[:2, 8:, 5]).all()
     got[:2, 8:, 5], clean[:2, 8:, 5] = 0, 0
     assert torch.equal(got, clean)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,tile_rows", FORMS)
+def test_scratch_that_was_replaced_is_used(dtype, tile_rows):
+    lens, spans = [300, 290, 280], [([0, 1], 0, 256)]
+    q, k, v, table = case(lens, spans, HEADS, KV, DIM, PAGE, dtype)
+    plan = build_shared_plan(lens, spans, HEADS, KV, DIM, dtype, PAGE, tile_rows=tile_rows).to(DEV)
+    want = run(q, k, v, table, plan, SCALE)
+    old = plan.part_o, plan.part_ml
+    for t in old:
+        t.fill_(5.0)
+    plan.part_o, plan.part_ml = (torch.empty_like(t) for t in old)
+    assert torch.equal(run(q, k, v, table, plan, SCALE), want)
+    assert all((t == 5.0).all() for t in old)
+
+
+@pytest.mark.gpu
+def test_a_copy_of_a_plan_uses_what_it_was_given():
+    """``dataclasses.replace`` with scratch of its own: the two may run at once."""
+    lens, spans = [300, 290, 280], [([0, 1], 0, 256)]
+    q, k, v, table = case(lens, spans, HEADS, KV, DIM, PAGE, BF16)
+    plan = build_shared_plan(lens, spans, HEADS, KV, DIM, BF16, PAGE).to(DEV)
+    want = run(q, k, v, table, plan, SCALE)
+    other = dataclasses.replace(plan, part_o=torch.full_like(plan.part_o, 5.0), part_ml=torch.full_like(plan.part_ml, 5.0))
+    plan.part_o.fill_(5.0)
+    assert torch.equal(run(q, k, v, table, other, SCALE), want)
+    assert (plan.part_o == 5.0).all() and not (other.part_o == 5.0).all()
