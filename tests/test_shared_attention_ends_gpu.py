@@ -1,11 +1,13 @@
-"""Attention over shared keys at its ends: what is not a number in a part that weighs next to nothing, scratch that was replaced."""
+"""Attention over shared keys at its ends: what is not a number in a part that weighs next to nothing, scratch that was replaced, calls at once."""
 
 import dataclasses
+import threading
 
 import pytest
 import torch
 
 from freetoken_b200.engine.shared_plan import build_shared_plan
+from freetoken_b200.kernels import ops
 from test_shared_attention_gpu import BF16, DEV, F32, case, run
 
 HEADS, KV, DIM, PAGE = 16, 2, 128, 16
@@ -116,3 +118,37 @@ def test_a_copy_of_a_plan_uses_what_it_was_given():
     plan.part_o.fill_(5.0)
     assert torch.equal(run(q, k, v, table, other, SCALE), want)
     assert (plan.part_o == 5.0).all() and not (other.part_o == 5.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_calls_of_different_sizes_from_two_threads(dtype):
+    """A launch with room for many keys beside launches with room for few: none may take the other's room away."""
+    sizes = [([2000] * 12, [(list(range(12)), 0, 1600)], DIM), ([40] * 12, [(list(range(12)), 0, 32)], DIM), ([300] * 3, [], 80), ([300] * 3, [], 96)]
+    wrong = []
+    ops.check_status()  # (the library is there)
+
+    def calls(lens, spans, dim):
+        try:
+            q, k, v, table = [t.to(DEV) for t in case(lens, spans, HEADS, KV, dim, PAGE, dtype)]
+            plan = build_shared_plan(lens, spans, HEADS, KV, dim, dtype, PAGE).to(DEV)
+            stream = torch.cuda.Stream()
+            stream.wait_stream(torch.cuda.default_stream())
+            with torch.cuda.stream(stream):
+                want, out = torch.empty_like(q), torch.empty_like(q)
+                ops.shared_attention(q, k, v, table, plan, want, dim ** -0.5)
+                for _ in range(3000):
+                    ops.shared_attention(q, k, v, table, plan, out, dim ** -0.5)
+                stream.synchronize()
+            assert torch.equal(out, want)
+        except Exception as e:
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=calls, args=s) for s in sizes]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    ops.check_status()
+    assert not wrong, wrong
