@@ -1,5 +1,8 @@
 """What requests that share pages owe and hold, on the host: reservations, names, block-table changes that wait for a step."""
 
+import random
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -124,8 +127,11 @@ def tables_agree(cache):
     cache.check()
     for r in cache.requests.values():
         blocks = -(-r.length // cache.page_size)
-        for g in cache.paged:
-            assert g.table_dev[r.row, :blocks].tolist() == g.table_host[r.row, :blocks].tolist()
+        for g in cache.paged:  # (what is given back is not read, and what waits for a step comes with it)
+            wait = dict(g.updates)
+            for b in range(blocks):
+                page = int(g.table_host[r.row, b])
+                assert not page or page == wait.get(r.row * g.width + b, int(g.table_dev[r.row, b]))
 
 
 def cache_of(pages=40, reqs=4):
@@ -282,3 +288,64 @@ def test_pages_of_several_holders_are_counted():
     assert pool.shared == 1
     pool.free([3, 3, a])
     assert pool.shared == 0 and pool.free_count == 4
+
+
+class HostEngine:
+    """What the scheduler asks of an engine, on block tables alone: full pages, a window, a window that keeps its first tokens."""
+
+    NEEDS = [(0, PagedKVNeed((("k", 1, 2),), None)), (1, PagedKVNeed((("k", 1, 2),), 7)), (2, PagedKVNeed((("k", 1, 2),), 9, 5))]
+
+    def __init__(self, pages, reqs, step):
+        self.cache = CacheManager(self.NEEDS, 4, pages, reqs, 96, torch.float32, torch.device("cpu"), max_step_tokens=step)
+        self.config = SimpleNamespace(max_running_req=reqs, max_extend_tokens=step, overlap_scheduling=True)
+        self.spec = SimpleNamespace(vocab_size=50)
+        self.max_step_tokens, self.max_seq_len = step, 96
+        self.open, self.close = self.cache.open, self.cache.close
+
+    def fork(self, rid, copies):
+        fork(self.cache, rid, copies)
+
+    def step(self, entries):
+        self.cache.begin_step([(e.request_id, len(e.tokens)) for e in entries])
+        ship(self.cache)
+        self.cache.end_step()
+        rows = [(e.request_id, w) for e in entries for w in e.want]
+        return SimpleNamespace(rows=rows, logits=torch.zeros(len(rows), 1))
+
+
+class HostSampler:
+    def __init__(self, rng, eos):
+        self.rng, self.eos = rng, eos
+
+    def launch(self, logits, params, requests, steps, rows=None):
+        assert len(params) == len(requests) == len(steps) == (logits.shape[0] if rows is None else len(rows))
+        return SimpleNamespace(device_tokens=torch.zeros(1), tokens=[0 if self.rng.random() < self.eos else 5 for _ in params])
+
+    def result(self, ticket):
+        return ticket.tokens
+
+
+@pytest.mark.parametrize("overlap", [False, True])
+@pytest.mark.parametrize("seed", range(12))
+def test_admitted_requests_always_find_their_pages(seed, overlap):
+    """Random prompts, continuations, ends and aborts in a small cache of three kinds of groups."""
+    rng = random.Random(seed)
+    eng = HostEngine(pages=rng.choice([26, 34, 50]), reqs=rng.choice([4, 6, 9]), step=rng.choice([8, 16]))
+    sched = Scheduler(eng, HostSampler(rng, rng.choice([0.0, 0.1, 0.3])), (0,))
+    wanted = {}
+    for i in range(40):
+        n = rng.choice([1, 1, 2, 3, 4])
+        wanted[i] = n
+        sched.add_request([1] * rng.randint(1, 60), SamplingParams(max_tokens=rng.randint(1, 30), n=n, temperature=1.0), rid=i)
+    while not sched.idle:
+        sched.step_overlapped() if overlap else sched.step()
+        eng.cache.check()
+        if rng.random() < 0.1:
+            tables_agree(eng.cache)
+        assert all(h <= r <= p for h, r, p in zip([g.pool.num_pages - g.pool.free_count for g in eng.cache.paged], sched.reserved, sched.pool_pages))
+        assert len(sched.running) <= sched.max_running
+        if rng.random() < 0.1 and sched.running:
+            sched.abort(rng.choice(sched.running).rid)
+    sched.drain()
+    assert sched.reserved == [0, 0, 0] and all(g.pool.free_count == g.pool.num_pages for g in eng.cache.paged)
+    assert set(wanted) <= set(sched.done) and any(r.continues for r in sched.done.values())
