@@ -17,11 +17,12 @@
 // What a CTA has to tell the others it writes into their shared memory in front of the cluster's barrier: reading it there behind
 // the barrier would be one trip more a pass.
 // What bounds it: for one draw the passes one after the other (a barrier of the cluster each, a microsecond or so with the wait for the
-// slowest CTA); for many the instructions of the passes (0.6 of the issue slots taken, the 64-bit pipe 0.1): so logits lie in shared
+// slowest CTA); for many the instructions of the passes (0.63 of the issue slots taken, the 64-bit pipe 0.1): so logits lie in shared
 // memory as numbers, four to a load, and are compared as such; and where top-k (of 128 at most) or top-p leaves no more than kListed of a
-// row, every CTA lists those and does the rest in the list (one draw with all filters 33 -> 24 us, 96 of them 119 -> 92).  Rows of
-// 200,000 logits: one draw without filters 20 us, min-p 17, top-k 50, top-p and min-p 24, top-p alone 38; 96 draws from 24 rows 77, 92 and
-// (top-p of flat rows) 168 us; 256 rows with min-p 126.
+// row, every CTA lists those and does the rest in the list (one draw with all filters 33 -> 27 us, 96 of them from 24 rows 128 -> 102).
+// Measured, rows of 200,000 normal logits (deviation 3) at T = 0.8, with log-probabilities, one launch between two events on cold caches: one
+// draw without filters 22 us, with min-p 18, top-k 50, top-p 0.9 and min-p 27, top-p 0.95 alone 45; 96 draws from 24 rows 86, 55, 102
+// and 217 us, from 96 rows 94, 64, 112 and 224.
 #include "common.cuh"
 
 namespace ftk {
@@ -114,8 +115,8 @@ __device__ const double kPowers[256] = {
     1.99459211217094023e+00,
 };
 // 2^y for y <= 0: with k = 256 n + j the integer nearest to 256 y and r = y - k / 256 (exact, |r| <= 2^-9), 2^y = 2^n 2^(j / 256) 2^r, where the
-// series up to r^3 is within 2.3e-15.  Below 2^-1000: zero.  (Nine operations in 64 bits; powers of 1/32 and the series up to r^5
-// took thirteen.)
+// series up to r^3 is within 1.4e-13 (the term behind it, (ln 2 / 512)^4 / 24), and so is every sum of such numbers, some 2^-42.7.  Below
+// 2^-1000: zero.  (Nine operations in 64 bits; powers of 1/32 and the series up to r^5, within 2.3e-15, took thirteen.)
 __device__ __forceinline__ double exp2_down(double y, const double* powers) {
   double k = fma(y, 256.0, 6755399441055744.0);
   const int n = __double2loint(k);
@@ -860,8 +861,9 @@ extern "C" int ftk_sample_draws(const float* logits, long long row_stride, int n
   FTK_REQUIRE(rows || n_draws <= n_rows, "sample_draws: %d draws from %d rows", n_draws, n_rows);
   FTK_REQUIRE(n_draws <= (1 << 24), "sample_draws: %d draws", n_draws);
   DrawParams p{logits, row_stride, n_rows, vocab, rows, temperature, top_k, top_p, min_p, u, out, logprobs, 1, 1};
-  // A CTA for every 4,096 logits, eight at most; sixteen for up to four draws.  Rows of 200,000, eight and sixteen: one draw 24.6 and 21.3 us,
-  // with top-p 51 and 42; four 26 and 20, 57 and 43; eight 26.7 and 24.6, 57 and 59, with all filters 31 and 33; sixteen 35 and 37, 80 and 84.
+  // A CTA for every 4,096 logits, eight at most; sixteen for up to four draws.  Rows of 200,000 (as at the top), eight and sixteen: one draw 29
+  // and 22 us, with top-p 57 and 45; four 27 and 20, 55 and 44; eight 27 and 25, with top-p 57 and 55 (57 and 61 where 40 logits stand out of a
+  // row), with all filters 33 and 32; sixteen 35 and 37, 80 and 84; 96 from 24 rows 86 and 121.
   while (p.cluster < (n_draws <= 4 ? 16 : 8) && vocab > p.cluster * 4096) p.cluster *= 2;
   p.run = 4 * (((vocab + 4 * p.cluster * kDrawThreads - 1) / (4 * p.cluster * kDrawThreads)) | 1);
   const bool held = p.run <= kMostRun;  // (442,000 logits; longer rows are read again in every pass)
