@@ -50,7 +50,6 @@ long steps and decode steps), 256 (the same with two query tiles per CTA: very l
 from __future__ import annotations
 
 import ctypes
-import operator
 from typing import Any, Optional, Sequence, Tuple
 
 import torch
@@ -733,12 +732,12 @@ def shared_attention(q: torch.Tensor, k_slab: torch.Tensor, v_slab: torch.Tensor
     ``sink``: a logit, a float32 tensor ``[Hq]`` of one per query head, or None, as in :func:`paged_attention`.
 
     The plan's scratch belongs to one launch at a time: calls that may run at once need plans of their own."""
-    host = plan.host
-    has = (host, plan.items, plan.members, plan.requests, plan.joins, plan.part_o, plan.part_ml)
-    if plan.fixed is None or not all(map(operator.is_, plan.fixed[1], has)):
-        plan.fixed = (_shared_fixed(plan), has)
+    fixed = plan.fixed
+    if fixed is None:
+        fixed = plan.fixed = _shared_fixed(plan)
     elif plan.requests.device.index != torch._C._cuda_getDevice():
         raise KernelError(f"shared_attention: the plan is on '{plan.requests.device}', the current device is 'cuda:{torch._C._cuda_getDevice()}'")
+    host = plan.host
     shape, slab = q.shape, k_slab.shape
     if len(shape) != 3 or len(slab) != 4:
         raise KernelError("shared_attention: q must be [T, Hq, D], slabs [pages, Hkv, page_size, D]")
@@ -752,7 +751,7 @@ def shared_attention(q: torch.Tensor, k_slab: torch.Tensor, v_slab: torch.Tensor
         raise KernelError(f"shared_attention: {T} query rows and a block table of {block_table.dim()} dimensions for a plan of {host.n_rows} requests")
     if not host.n_rows:
         return
-    a = _Shared.from_buffer_copy(plan.fixed[0])
+    a = _Shared.from_buffer_copy(fixed)
     if sink is not None:
         a.has_sink = 1
         if isinstance(sink, torch.Tensor):
