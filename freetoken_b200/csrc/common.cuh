@@ -10,6 +10,9 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <atomic>
+#include <mutex>
+
 #include "api.h"
 
 namespace ftk {
@@ -80,6 +83,33 @@ inline cudaError_t launch_kernel_clusters(void (*kernel)(KArgs...), int cluster,
 }
 #define FTK_LAUNCH(kernel, grid, block, smem, stream, ...) \
   ftk::launch_kernel(kernel, dim3(grid), dim3(block), (size_t)(smem), (cudaStream_t)(stream), __VA_ARGS__)
+
+// Sets a kernel up on the current device, once, in front of its first launch there.  (An attribute that a thread changes while another
+// launches the same kernel can make that launch fail.)
+class OncePerDevice {
+ public:
+  template <typename F>
+  bool operator()(F set_up) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
+    if (done_.load(std::memory_order_acquire) & bit) return true;
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (done_.load(std::memory_order_relaxed) & bit) return true;
+    if (!set_up()) return false;
+    done_.fetch_or(bit, std::memory_order_release);
+    return true;
+  }
+
+ private:
+  std::atomic<unsigned long long> done_{0};
+  std::mutex mutex_;
+};
+// The most shared memory that any launch of the kernel asks for.
+template <typename K>
+inline bool set_shared_limit(K kernel, size_t most) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) == cudaSuccess;
+}
 
 inline bool dtype_ok(int d) { return d == FTK_F32 || d == FTK_BF16; }
 inline int dtype_size(int d) { return d == FTK_F32 ? 4 : 2; }

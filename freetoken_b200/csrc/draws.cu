@@ -869,10 +869,11 @@ extern "C" int ftk_sample_draws(const float* logits, long long row_stride, int n
   const bool held = p.run <= kMostRun;  // (442,000 logits; longer rows are read again in every pass)
   const size_t smem = held ? (size_t)p.run * kDrawThreads * sizeof(float) : 0;
   auto kern = held ? draw_kernel<true> : draw_kernel<false>;
-  // (as much as any call takes, so that calls from several threads set the same)
-  constexpr int most = kMostRun * kDrawThreads * (int)sizeof(float);
-  FTK_REQUIRE((!held || cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most) == cudaSuccess) &&
-                  (p.cluster <= 8 || cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess),
+  static OncePerDevice once[2];
+  FTK_REQUIRE(once[held]([&] {
+                return set_shared_limit(kern, held ? kMostRun * kDrawThreads * sizeof(float) : 0) &&
+                       cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
+              }),
               "sample_draws: cannot set up the kernel");
   note_variant(held ? "draws: rows in shared memory" : "draws: rows read again in every pass");
   const dim3 grid((unsigned)(n_draws * p.cluster));

@@ -649,18 +649,19 @@ static size_t rows_smem(int d, int stages) {
 
 template <typename T, int DMAX, bool EXACT>
 static int launch_shared_rows(const SharedParams& p, cudaStream_t s) {
-  const size_t smem = rows_smem<T>(p.D, p.stages), most = rows_smem<T>(DMAX, kTileStages);
   auto kern = shared_rows_kernel<T, DMAX, EXACT>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess) return 2;  // (see launch_own_keys)
+  static OncePerDevice once;
+  if (!once([&] { return set_shared_limit(kern, rows_smem<T>(DMAX, kTileStages)); })) return 2;
+  const size_t smem = rows_smem<T>(p.D, p.stages);
   FTK_LAUNCH(kern, dim3(p.n_items, p.Hkv * p.chunks), kRowThreads, smem, s, p);
   return 0;
 }
 template <typename T, int DMAX, bool EXACT>
 static int launch_own_keys(const SharedParams& p, cudaStream_t s) {
-  // as much as any call of this kernel takes, so that calls from several threads set the same
-  const size_t smem = rows_smem<T>(p.D, p.stages), most = rows_smem<T>(DMAX, kTileStages);
   auto kern = own_keys_kernel<T, DMAX, EXACT>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess) return 2;
+  static OncePerDevice once;
+  if (!once([&] { return set_shared_limit(kern, rows_smem<T>(DMAX, kTileStages)); })) return 2;
+  const size_t smem = rows_smem<T>(p.D, p.stages);
   const dim3 grid((unsigned)(p.n_requests * p.Hkv * p.chunks * p.cluster));
   if (p.cluster > 1) launch_kernel_clusters(kern, p.cluster, grid, dim3(kRowThreads), smem, s, p);
   else FTK_LAUNCH(kern, grid, kRowThreads, smem, s, p);

@@ -530,7 +530,8 @@ inline bool shared_tc_fits(int head_dim, int page_size, int group) {
 template <int D>
 static int launch_shared_tc(const SharedParams& p, cudaStream_t s) {
   auto kern = shared_tc_kernel<D>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kShSmem(D)) != cudaSuccess) return 2;
+  static OncePerDevice once;
+  if (!once([&] { return set_shared_limit(kern, kShSmem(D)); })) return 2;
   CUtensorMap mk, mv;
   // a slab [pages, KV heads, P, D] seen as rows of D; a box is 16 rows of one page x 64 elements
   const uint64_t dims[2] = {(uint64_t)D, (uint64_t)p.num_pages * p.Hkv * p.P};
